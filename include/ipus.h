@@ -174,6 +174,61 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        s / h of an unsplit [streams / h, rows, h * width] tensor (h = 1:
  *        contiguous; streams % h == 0).  The zero-copy form of SplitHeads
  *        (operator.rs:213-279) feeding attention; build_package emits it.
+ *   Decoder serving (no reference counterpart; positions, offsets, lengths and
+ *   tables are int32 device arrays that the host never reads, frequencies fp32
+ *   in rad per position, e.g. ipus_rotary_frequencies; f32 scalars as bits):
+ *   ipu_stack_rotary_f16, ipu_stack_rotary_f32   out; input, positions [rows],
+ *        frequencies [rotary_width / 2]; rows, heads, width, rotary_width,
+ *        interleaved, input_row_stride, input_head_stride, output_row_stride,
+ *        output_head_stride (elements), magnitude_bits (0 = 1).  Turns pair
+ *        i of every head by positions[row] * frequencies[i] (reduced in 64
+ *        bits), scaled by the magnitude: elements (i, rotary_width / 2 + i),
+ *        interleaved = 1: (2 i, 2 i + 1); elements from rotary_width on are
+ *        copied.  fp32 arithmetic, one rounding.  The output is the input
+ *        (with its strides) or does not overlap it; its own heads must not
+ *        overlap.  width <= 2048, rotary_width even.
+ *   ipu_stack_norm_rotary_f16, ipu_stack_norm_rotary_f32   out; input,
+ *        query_weight, key_weight [width] (in the input's type), positions,
+ *        frequencies; rows, query_heads, key_heads, width, rotary_width,
+ *        interleaved, input_row_stride, output_row_stride, epsilon_bits,
+ *        magnitude_bits.  A row's heads lie side by side, queries before keys
+ *        (the value heads of a fused projection may follow in the row): each
+ *        becomes x * weight / sqrt(mean(x^2) + epsilon), then is turned as
+ *        above, with one rounding.  key_heads or query_heads may be 0 (its
+ *        weight pointer is then not read, but not null either).
+ *   ipu_stack_append_pages_f16   out the cache, fp16 [pages][2][key_heads]
+ *        [page_rows][width] (keys, then values); new keys and values
+ *        [rows][key_heads][width] (row strides in elements), frequencies,
+ *        page_table [sequences][table_columns], row_offsets [sequences + 1],
+ *        lengths [sequences]; sequences, rows, key_heads, width,
+ *        key_row_stride, value_row_stride, rotary_width (0: no rotation),
+ *        interleaved, magnitude_bits, pages, page_rows (a power of two up to
+ *        65536), table_columns.  Rows row_offsets[s] .. row_offsets[s + 1] - 1
+ *        are the last of sequence s, whose length with them is lengths[s]: the
+ *        i-th of n goes to position p = lengths[s] - n + i, row p % page_rows
+ *        of page page_table[s][p / page_rows], its key turned by p.  Rows past
+ *        row_offsets[sequences], negative positions, positions past the table
+ *        and entries outside [0, pages) write nothing.  The offsets do not
+ *        decrease; a page that new rows go to belongs to one sequence.
+ *   ipu_stack_attention_pages_f16   out f16 [rows][query_heads][width]; query
+ *        f16 (heads side by side, query_row_stride elements from row to row),
+ *        the cache, page_table, row_offsets, lengths; sequences, rows,
+ *        max_rows, query_heads, key_heads (a divisor: query head h reads key
+ *        head h / (query_heads / key_heads)), width, query_row_stride, pages,
+ *        page_rows, table_columns, causal, scale_bits (0 = 1 / sqrt(width)).
+ *        Row i of the n of sequence s reads the keys below lengths[s], when
+ *        causal those up to its position lengths[s] - n + i.  Keys without a
+ *        page carry no weight; a row whose weights are all zero (no key, or
+ *        only scores of -inf) gives zeros; rows outside every sequence are
+ *        left as they were.  max_rows, the most rows of a sequence (0 = rows),
+ *        only picks the kernel.  fp32 scores, maxima and sums; probabilities
+ *        are rounded to fp16 for the second product.  width <= 1024; widths
+ *        that are multiples of 8 up to 256 with 16-byte aligned pointers and
+ *        strides run on the matrix units.
+ *   ipu_stack_attention_shared_pages_f16   the same with shared_rows behind
+ *        the scalars: positions below it lie in the pages of the first
+ *        sequence's table for every sequence (a shared prompt), and are read
+ *        once for many sequences where that pays.
  *   ipu_stack_gelu_tanh_approx_f16     out f16; input f16; element_count
  *        (kernel.rs:1251-1263; count must be even, kernel.rs:1400-1413).
  *   ipu_stack_reduce_sum_f16           out f16; initial, packed remotes f16;
@@ -312,6 +367,27 @@ int ipus_gemm_f16_split_noalloc(ipus_context *context, void *output, const void 
                                 uint32_t columns, uint32_t inner, int transpose_left,
                                 int transpose_right, uint64_t left_batch_stride,
                                 uint64_t right_batch_stride, uint32_t splits, int gelu);
+
+/* ---- rotary frequencies (host) ----
+ * frequencies[i] = base^(-2 i / rotary_width), i < rotary_width / 2, in rad per
+ * position, and the magnitude of the rotated elements, for
+ * ipu_stack_rotary_* and the kernels that rotate on the way.  scaling, for
+ * contexts `factor` times the trained one:
+ *   PLAIN   as they are (factor is not read);
+ *   LINEAR  all divided by factor (positions interpolated);
+ *   BASE    of base * factor^(rotary_width / (rotary_width - 2)), which divides
+ *           the slowest by factor and leaves the fastest (rotary_width > 2);
+ *   BANDED  by the turns each makes over the trained_rows of training: up to
+ *           slow_turns divided by factor, from fast_turns on as they are, a
+ *           linear ramp between; magnitude 0.1 ln(factor) + 1 for factor > 1.
+ * The magnitude is 1 otherwise.  Computed in 64 bits, rounded once. */
+#define IPUS_ROTARY_PLAIN 0
+#define IPUS_ROTARY_LINEAR 1
+#define IPUS_ROTARY_BASE 2
+#define IPUS_ROTARY_BANDED 3
+int ipus_rotary_frequencies(float *frequencies, float *magnitude, uint32_t rotary_width,
+                            double base, int scaling, double factor, double trained_rows,
+                            double slow_turns, double fast_turns);
 
 /* ---- synthetic inputs (host, deterministic, multithreaded) ----
  * value(seed, tensor, i) from SplitMix64(seed ^ (tensor << 48) ^ i):

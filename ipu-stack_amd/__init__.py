@@ -188,6 +188,9 @@ _SIGNATURES = {
         ctypes.c_int,
         [_P, ctypes.c_char_p, _P, ctypes.POINTER(_P), ctypes.c_int, _U32P, ctypes.c_int],
     ),
+    "ipus_rotary_frequencies": (
+        ctypes.c_int, [_P, _P, ctypes.c_uint32, ctypes.c_double, ctypes.c_int, ctypes.c_double,
+                       ctypes.c_double, ctypes.c_double, ctypes.c_double]),
     "ipus_synth_f16": (
         ctypes.c_int,
         [_P, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int, ctypes.c_float],
@@ -381,6 +384,26 @@ def synth_f32(count: int, seed: int, tensor: int, distribution: int = UNIFORM,
 
 def _f32_bits(value: float) -> int:
     return struct.unpack("<I", struct.pack("<f", float(value)))[0]
+
+
+ROTARY_PLAIN = 0
+ROTARY_LINEAR = 1
+ROTARY_BASE = 2
+ROTARY_BANDED = 3
+
+
+def rotary_frequencies(rotary_width: int, base: float = 10000.0, scaling: int = ROTARY_PLAIN,
+                       factor: float = 1.0, trained_rows: float = 0.0, slow_turns: float = 1.0,
+                       fast_turns: float = 32.0) -> tuple[np.ndarray, float]:
+    """(float32 [rotary_width / 2] rad per position, magnitude) for the rotary
+    kernels; ROTARY_LINEAR, _BASE and _BANDED (by the turns over trained_rows)
+    reach contexts `factor` times the trained one."""
+    out = np.empty(max(0, int(rotary_width)) // 2, dtype=np.float32)
+    magnitude = ctypes.c_float(0)
+    _check(_lib().ipus_rotary_frequencies(
+        out.ctypes.data, ctypes.addressof(magnitude), int(rotary_width), float(base),
+        int(scaling), float(factor), float(trained_rows), float(slow_turns), float(fast_turns)))
+    return out, magnitude.value
 
 
 def scale_bits(scale: float | None) -> int:

@@ -104,6 +104,60 @@ int launch_gemm_f32(hipStream_t stream, const GemmArgs& a);
 // Fused online-softmax attention (k_attention.hip).
 int launch_attention_f16(hipStream_t stream, const AttentionArgs& a);
 
+// Rotary positions (k_rotary.hip): heads of `width` elements, strides in
+// elements; positions int32 [rows], frequencies fp32 [rotary_width / 2] in rad per
+// position.  With weights each head is normed first: heads below query_heads by
+// query_weight, the others by key_weight.
+struct RotaryArgs {
+  void* out;
+  const void* input;
+  const void* query_weight = nullptr;
+  const void* key_weight = nullptr;
+  const int* positions;
+  const float* frequencies;
+  uint32_t rows, heads, query_heads, width, rotary_width;
+  uint32_t input_row_stride, input_head_stride, output_row_stride, output_head_stride;
+  float epsilon = 0.0f, magnitude;
+  bool interleaved, f32;
+};
+int launch_rotary(hipStream_t stream, const RotaryArgs& a);
+
+// A ragged batch over a paged cache (pages.h).
+struct PagedBatch {
+  const int* table;        // [sequences][table_columns]
+  const int* row_offsets;  // [sequences + 1]
+  const int* lengths;      // [sequences]
+  uint32_t sequences, table_columns, pages, page_rows, page_shift;
+  uint32_t shared_rows = 0;  // positions that every sequence reads through the first one's table
+  uint64_t page_elements;    // 2 x key heads x page_rows x width
+};
+
+// New keys and values of the batch's rows into the cache (k_rotary.hip).
+struct AppendArgs {
+  void* cache;
+  const void* keys;
+  const void* values;
+  const float* frequencies;
+  PagedBatch batch;
+  uint32_t rows, key_heads, width, rotary_width, key_row_stride, value_row_stride;
+  float magnitude;
+  bool interleaved;
+};
+int launch_append_pages(hipStream_t stream, const AppendArgs& a);
+
+// Attention of the batch's rows over the cache (k_attention_pages.hip).
+struct PagedAttentionArgs {
+  void* out;  // fp16 [rows][query_heads][width]
+  const void* query;
+  const void* cache;
+  PagedBatch batch;
+  uint32_t rows, max_rows, query_heads, key_heads, width, query_row_stride;
+  float scale;
+  bool causal;
+  Workspace workspace;
+};
+int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a);
+
 // Bandwidth kernels (k_memory.hip).
 int launch_transpose_f16(hipStream_t stream, void* dst, const void* src, uint32_t matrices,
                          uint32_t rows, uint32_t columns);

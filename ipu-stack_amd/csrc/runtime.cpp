@@ -460,6 +460,162 @@ int run_attention(ipus_context* c, void* o, const void* const* i, const uint32_t
   return launch_attention_f16(c->stream, a);
 }
 
+// ---- rotary positions and the paged cache ----
+
+// A float scalar's bits, or what 0 stands for.
+float bits_or(uint32_t bits, float zero) { return bits == 0 ? zero : bits_to_float(bits); }
+
+// Widths of the rotated part and the layout flag; magnitude: finite.
+constexpr uint32_t kMaxRotaryHead = 2048;
+int check_rotation(uint32_t width, uint32_t rotary_width, uint32_t interleaved, uint32_t magnitude_bits) {
+  if (width == 0 || rotary_width > width || rotary_width % 2 != 0 || interleaved > 1)
+    return IPUS_ERROR_INVALID_ARGUMENT;
+  if (!std::isfinite(bits_or(magnitude_bits, 1.0f))) return IPUS_ERROR_INVALID_ARGUMENT;
+  return width > kMaxRotaryHead ? IPUS_ERROR_UNAVAILABLE : 0;
+}
+
+// rows, heads, width, rotary_width, interleaved, input row and head stride,
+// output row and head stride, magnitude_bits.  Output heads must not overlap.
+int check_rotary(const uint32_t* s) {
+  if (int e = check_rotation(s[2], s[3], s[4], s[9])) return e;
+  const uint64_t rows = s[0], heads = s[1], width = s[2], row = s[7], head = s[8];
+  if (rows == 0 || heads == 0) return 0;
+  if (rows > 0x7fffffff || heads > 0x7fffffff) return IPUS_ERROR_INVALID_ARGUMENT;
+  const bool rows_outer = (heads == 1 || head >= width) && (rows == 1 || row >= (heads - 1) * head + width);
+  const bool heads_outer = (rows == 1 || row >= width) && (heads == 1 || head >= (rows - 1) * row + width);
+  return rows_outer || heads_outer ? 0 : IPUS_ERROR_INVALID_ARGUMENT;
+}
+int run_rotary(ipus_context* c, void* o, const void* const* i, const uint32_t* s, bool f32) {
+  RotaryArgs a;
+  a.out = o;
+  a.input = i[0];
+  a.positions = (const int*)i[1];
+  a.frequencies = (const float*)i[2];
+  a.rows = s[0];
+  a.heads = a.query_heads = s[1];
+  a.width = s[2];
+  a.rotary_width = s[3];
+  a.interleaved = s[4] != 0;
+  a.input_row_stride = s[5];
+  a.input_head_stride = s[6];
+  a.output_row_stride = s[7];
+  a.output_head_stride = s[8];
+  a.magnitude = bits_or(s[9], 1.0f);
+  a.f32 = f32;
+  return launch_rotary(c->stream, a);
+}
+
+// rows, query_heads, key_heads, width, rotary_width, interleaved, input and
+// output row stride, epsilon_bits, magnitude_bits.
+int check_norm_rotary(const uint32_t* s) {
+  if (int e = check_rotation(s[3], s[4], s[5], s[9])) return e;
+  const float epsilon = bits_to_float(s[8]);
+  if (!std::isfinite(epsilon) || epsilon < 0.0f) return IPUS_ERROR_INVALID_ARGUMENT;
+  const uint64_t heads = (uint64_t)s[1] + s[2];
+  if (s[0] > 0x7fffffff || heads > 0x7fffffff) return IPUS_ERROR_INVALID_ARGUMENT;
+  return s[0] <= 1 || s[7] >= heads * s[3] ? 0 : IPUS_ERROR_INVALID_ARGUMENT;
+}
+int run_norm_rotary(ipus_context* c, void* o, const void* const* i, const uint32_t* s, bool f32) {
+  RotaryArgs a;
+  a.out = o;
+  a.input = i[0];
+  a.query_weight = i[1];
+  a.key_weight = i[2];
+  a.positions = (const int*)i[3];
+  a.frequencies = (const float*)i[4];
+  a.rows = s[0];
+  a.query_heads = s[1];
+  a.heads = s[1] + s[2];
+  a.width = s[3];
+  a.rotary_width = s[4];
+  a.interleaved = s[5] != 0;
+  a.input_row_stride = s[6];
+  a.output_row_stride = s[7];
+  a.input_head_stride = a.output_head_stride = a.width;
+  a.epsilon = bits_to_float(s[8]);
+  a.magnitude = bits_or(s[9], 1.0f);
+  a.f32 = f32;
+  return launch_rotary(c->stream, a);
+}
+
+// Rows of a page: a power of two, so that positions split by a shift.
+int check_pages(uint32_t rows, uint32_t key_heads, uint32_t page_rows) {
+  if (rows > 0x7fffffff || key_heads == 0 || key_heads > 32767) return IPUS_ERROR_INVALID_ARGUMENT;
+  if (page_rows == 0 || page_rows > 65536 || (page_rows & (page_rows - 1)) != 0)
+    return IPUS_ERROR_INVALID_ARGUMENT;
+  return 0;
+}
+PagedBatch paged_batch(const void* table, const void* row_offsets, const void* lengths,
+                       uint32_t sequences, uint32_t pages, uint32_t page_rows,
+                       uint32_t table_columns, uint32_t key_heads, uint32_t width) {
+  PagedBatch b;
+  b.table = (const int*)table;
+  b.row_offsets = (const int*)row_offsets;
+  b.lengths = (const int*)lengths;
+  b.sequences = sequences;
+  b.pages = pages;
+  b.page_rows = page_rows;
+  b.page_shift = (uint32_t)__builtin_ctz(page_rows);
+  b.table_columns = table_columns;
+  b.page_elements = 2ull * key_heads * page_rows * width;
+  return b;
+}
+
+// sequences, rows, key_heads, width, key and value row stride, rotary_width,
+// interleaved, magnitude_bits, pages, page_rows, table_columns.
+int check_append(const uint32_t* s) {
+  if (int e = check_rotation(s[3], s[6], s[7], s[8])) return e;
+  return check_pages(s[1], s[2], s[10]);
+}
+int run_append(ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+  AppendArgs a;
+  a.cache = o;
+  a.keys = i[0];
+  a.values = i[1];
+  a.frequencies = (const float*)i[2];
+  a.batch = paged_batch(i[3], i[4], i[5], s[0], s[9], s[10], s[11], s[2], s[3]);
+  a.rows = s[1];
+  a.key_heads = s[2];
+  a.width = s[3];
+  a.key_row_stride = s[4];
+  a.value_row_stride = s[5];
+  a.rotary_width = s[6];
+  a.interleaved = s[7] != 0;
+  a.magnitude = bits_or(s[8], 1.0f);
+  return launch_append_pages(c->stream, a);
+}
+
+// sequences, rows, max_rows, query_heads, key_heads, width, query_row_stride,
+// pages, page_rows, table_columns, causal, scale_bits[, shared_rows].
+constexpr uint32_t kMaxPagedWidth = 1024;
+int check_attention_pages(const uint32_t* s) {
+  if (int e = check_pages(s[1], s[4], s[8])) return e;
+  if (s[3] == 0 || s[3] > 65535 || s[3] % s[4] != 0 || s[5] == 0 || s[10] > 1)
+    return IPUS_ERROR_INVALID_ARGUMENT;
+  const float scale = bits_or(s[11], 1.0f);
+  if (!std::isfinite(scale) || scale <= 0.0f) return IPUS_ERROR_INVALID_ARGUMENT;
+  return s[5] > kMaxPagedWidth ? IPUS_ERROR_UNAVAILABLE : 0;
+}
+int run_attention_pages(ipus_context* c, void* o, const void* const* i, const uint32_t* s,
+                        uint32_t shared_rows) {
+  PagedAttentionArgs a;
+  a.out = o;
+  a.query = i[0];
+  a.cache = i[1];
+  a.batch = paged_batch(i[2], i[3], i[4], s[0], s[7], s[8], s[9], s[4], s[5]);
+  a.batch.shared_rows = shared_rows;
+  a.rows = s[1];
+  a.max_rows = s[2] == 0 || s[2] > s[1] ? s[1] : s[2];
+  a.query_heads = s[3];
+  a.key_heads = s[4];
+  a.width = s[5];
+  a.query_row_stride = s[6];
+  a.causal = s[10] != 0;
+  a.scale = s[11] == 0 ? 1.0f / std::sqrt((float)s[5]) : bits_to_float(s[11]);
+  a.workspace = context_workspace(c);
+  return launch_attention_pages(c->stream, a);
+}
+
 const std::vector<KernelEntry>& registry() {
   static const std::vector<KernelEntry> entries = {
       {"ipu_stack_gemm_f16", 2,
@@ -548,6 +704,54 @@ const std::vector<KernelEntry>& registry() {
        [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
          return run_attention(c, o, i, s, s + 8);
        }},
+      // Rotary positions, norms of query and key heads with them, and the paged
+      // cache (no reference counterpart).
+      {"ipu_stack_rotary_f16", 3,
+       {"rows", "heads", "width", "rotary_width", "interleaved", "input_row_stride",
+        "input_head_stride", "output_row_stride", "output_head_stride", "magnitude_bits"},
+       [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+         return run_rotary(c, o, i, s, false);
+       },
+       check_rotary},
+      {"ipu_stack_rotary_f32", 3,
+       {"rows", "heads", "width", "rotary_width", "interleaved", "input_row_stride",
+        "input_head_stride", "output_row_stride", "output_head_stride", "magnitude_bits"},
+       [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+         return run_rotary(c, o, i, s, true);
+       },
+       check_rotary},
+      {"ipu_stack_norm_rotary_f16", 5,
+       {"rows", "query_heads", "key_heads", "width", "rotary_width", "interleaved",
+        "input_row_stride", "output_row_stride", "epsilon_bits", "magnitude_bits"},
+       [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+         return run_norm_rotary(c, o, i, s, false);
+       },
+       check_norm_rotary},
+      {"ipu_stack_norm_rotary_f32", 5,
+       {"rows", "query_heads", "key_heads", "width", "rotary_width", "interleaved",
+        "input_row_stride", "output_row_stride", "epsilon_bits", "magnitude_bits"},
+       [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+         return run_norm_rotary(c, o, i, s, true);
+       },
+       check_norm_rotary},
+      {"ipu_stack_append_pages_f16", 6,
+       {"sequences", "rows", "key_heads", "width", "key_row_stride", "value_row_stride",
+        "rotary_width", "interleaved", "magnitude_bits", "pages", "page_rows", "table_columns"},
+       run_append, check_append},
+      {"ipu_stack_attention_pages_f16", 5,
+       {"sequences", "rows", "max_rows", "query_heads", "key_heads", "width", "query_row_stride",
+        "pages", "page_rows", "table_columns", "causal", "scale_bits"},
+       [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+         return run_attention_pages(c, o, i, s, 0);
+       },
+       check_attention_pages},
+      {"ipu_stack_attention_shared_pages_f16", 5,
+       {"sequences", "rows", "max_rows", "query_heads", "key_heads", "width", "query_row_stride",
+        "pages", "page_rows", "table_columns", "causal", "scale_bits", "shared_rows"},
+       [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+         return run_attention_pages(c, o, i, s, s[12]);
+       },
+       check_attention_pages},
       {"ipu_stack_gelu_tanh_approx_f16", 1, {"element_count"},
        [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
          return launch_gelu_f16(c->stream, o, i[0], s[0]);
@@ -914,6 +1118,8 @@ int validate_run(const char* symbol, int input_count, const uint32_t* scalars, i
   if (r->family) status = r->family->check(r->shape, scalars);
   if (status == IPUS_ERROR_UNSUPPORTED_COUNT)
     return fail(status, "kernel %s does not support this element count", symbol);
+  if (status == IPUS_ERROR_UNAVAILABLE)
+    return fail(status, "kernel %s has no device implementation for these arguments", symbol);
   if (status) return fail(status, "kernel %s: scalars do not meet its ABI", symbol);
   return 0;
 }
@@ -1067,6 +1273,44 @@ extern "C" int ipus_gemm_f16_split_noalloc(ipus_context* ctx, void* output, cons
   a.gelu = gelu != 0;
   return check_launch(launch_gemm_f16_split_noalloc(ctx->stream, ctx->device, a, splits),
                       "ipus_gemm_f16_split_noalloc");
+}
+
+// ---------------------------------------------------------------------------
+// Rotary frequencies
+// ---------------------------------------------------------------------------
+extern "C" int ipus_rotary_frequencies(float* frequencies, float* magnitude, uint32_t rotary_width,
+                                       double base, int scaling, double factor, double trained_rows,
+                                       double slow_turns, double fast_turns) {
+  if (!frequencies || !magnitude) return fail(IPUS_ERROR_INVALID_ARGUMENT, "null argument");
+  if (rotary_width == 0 || rotary_width % 2 != 0)
+    return fail(IPUS_ERROR_INVALID_ARGUMENT, "rotary_width %u is not a positive even number", rotary_width);
+  if (!std::isfinite(base) || base <= 0.0)
+    return fail(IPUS_ERROR_INVALID_ARGUMENT, "base must be finite and positive");
+  if (scaling < IPUS_ROTARY_PLAIN || scaling > IPUS_ROTARY_BANDED)
+    return fail(IPUS_ERROR_INVALID_ARGUMENT, "unknown scaling %d", scaling);
+  if (scaling != IPUS_ROTARY_PLAIN && !(std::isfinite(factor) && factor > 0.0))
+    return fail(IPUS_ERROR_INVALID_ARGUMENT, "factor must be finite and positive");
+  if (scaling == IPUS_ROTARY_BASE && rotary_width == 2)
+    return fail(IPUS_ERROR_INVALID_ARGUMENT, "one frequency alone has no base to scale");
+  if (scaling == IPUS_ROTARY_BANDED &&
+      !(std::isfinite(trained_rows) && trained_rows > 0.0 && slow_turns >= 0.0 &&
+        std::isfinite(fast_turns) && slow_turns < fast_turns))
+    return fail(IPUS_ERROR_INVALID_ARGUMENT,
+                "banded scaling needs trained_rows > 0 and 0 <= slow_turns < fast_turns");
+  const double r = rotary_width;
+  if (scaling == IPUS_ROTARY_BASE) base *= std::pow(factor, r / (r - 2.0));
+  for (uint32_t i = 0; i < rotary_width / 2; ++i) {
+    double f = std::pow(base, -2.0 * i / r);
+    if (scaling == IPUS_ROTARY_LINEAR) f /= factor;
+    if (scaling == IPUS_ROTARY_BANDED) {
+      const double turns = trained_rows * f / 6.28318530717958647693;
+      const double keep = std::fmin(std::fmax((turns - slow_turns) / (fast_turns - slow_turns), 0.0), 1.0);
+      f *= keep + (1.0 - keep) / factor;
+    }
+    frequencies[i] = (float)f;
+  }
+  *magnitude = scaling == IPUS_ROTARY_BANDED && factor > 1.0 ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+  return 0;
 }
 
 // ---------------------------------------------------------------------------
