@@ -16,33 +16,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 inline int hip_status(hipError_t e) { return e == hipSuccess ? 0 : IPUS_ERROR_HIP_BASE - (int)e; }
 
-// Keys that row t may read: [0, count) of a sequence.  sequence >= sequences:
-// the row belongs to none.  Called by a whole wave.
-struct RowKeys {
-  uint32_t sequence, count;
-};
-__device__ __forceinline__ RowKeys row_keys(const PagedBatch& b, uint32_t t, bool causal) {
-  RowKeys k{find_sequence(b, t), 0};
-  if (k.sequence >= b.sequences) return k;
-  const int64_t start = b.row_offsets[k.sequence], end = b.row_offsets[k.sequence + 1];
-  if ((int64_t)t < start) {
-    k.sequence = b.sequences;
-    return k;
-  }
-  const int64_t length = b.lengths[k.sequence];
-  const int64_t count = causal ? length - (end - (int64_t)t) + 1 : length;
-  k.count = count > 0 ? (uint32_t)count : 0;
-  return k;
-}
-
 // Any width up to 1024, any alignment: a wave per row and query head, one key
 // after the other.
 constexpr uint32_t kGeneralPerLane = 16;
 __global__ __launch_bounds__(kWave) void attention_pages_general_kernel(PagedAttentionArgs a, uint32_t first_row,
                                                                         float scale_log2) {
   const uint32_t row = first_row + blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-  const RowKeys k = row_keys(a.batch, row, a.causal);
-  if (k.sequence >= a.batch.sequences) return;
+  const RowPlace place = find_row(a.batch, row);
+  if (place.sequence >= a.batch.sequences) return;
+  const uint32_t count = readable_keys(sequence_at(a.batch, place.sequence, a.rows), place.position, a.causal);
   const half_t* q = (const half_t*)a.query + (uint64_t)row * a.query_row_stride + (uint64_t)head * a.width;
   const uint32_t key_head = head / (a.query_heads / a.key_heads);
   const uint64_t head_elements = (uint64_t)a.batch.page_rows * a.width;
@@ -50,9 +32,8 @@ __global__ __launch_bounds__(kWave) void attention_pages_general_kernel(PagedAtt
 #pragma unroll
   for (uint32_t i = 0; i < kGeneralPerLane; ++i) acc[i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
-  for (uint32_t j = 0; j < k.count; ++j) {
-    if (j >> a.batch.page_shift >= a.batch.table_columns) break;
-    const int64_t page = page_of(a.batch, k.sequence, j);
+  for (uint32_t j = 0; j < count; ++j) {
+    const int page = page_of(a.batch, place.sequence, j);
     if (page < 0) continue;
     const half_t* key = (const half_t*)a.cache + (uint64_t)page * a.batch.page_elements + key_head * head_elements +
                         (uint64_t)(j & (a.batch.page_rows - 1)) * a.width;
@@ -80,6 +61,565 @@ __global__ __launch_bounds__(kWave) void attention_pages_general_kernel(PagedAtt
   }
 }
 
+// ---------------------------------------------------------------------------
+// Few query rows per key head: the keys are read once, bound by HBM.
+//
+// A sequence's rows times the query heads of one key head are packed into tiles
+// of 16 or 32 queries, so a key head's keys and values serve all of its query
+// heads.  The work of the whole batch - every (sequence, query tile, key head)
+// with its tiles of kKeys keys - is one line of units, cut into equal chunks, one
+// per workgroup: sequences of any mix of lengths load the chip evenly.  A
+// (sequence, query tile, key head) that lies in several chunks is merged by the
+// last of their workgroups to finish, in the order of the keys.  Every workgroup finds
+// its place by a scan over the sequences' lengths (two reads of a few words, in L2).
+//
+// Waves work alone: wave w takes the chunk's key tiles w, w + 4, ...  A tile's keys go
+// to registers in the layout of the first MFMA operand, its values by LDS DMA into the wave's own stage (the
+// transposing LDS read needs them there), the next tile's loads run
+// under this one's arithmetic, and the page numbers of the one after under both.  At 8 waves
+// per CU 128 KiB are in flight, without a barrier until the waves' results are
+// joined at the end of a segment.
+//
+// Scores are computed transposed, S^T = K Q^T, and the output as O^T += V^T P^T
+// (v_mfma_f32_16x16x32_f16, fp32 accumulation), as in k_attention.hip.  The probabilities enter
+// the second product as the sum of two fp16 values (22 bits): the matrix pipes have time for it here,
+// and the result is off by little more than its own rounding.
+
+#define LDS_AS __attribute__((address_space(3)))
+#define GLOBAL_AS __attribute__((address_space(1)))
+typedef short short4_t __attribute__((vector_size(8)));
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kWaves = kThreads / kWave;
+
+// 16 bytes of zeros: what a lane loads for keys that are not to be read and for columns
+// past the width, so that loads need no branch (with branches the compiler cannot count
+// them and waits for all) and nothing that is not the sequence's meets a product.
+__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+// LDS rows of D fp16, 16-byte chunk c of row r at chunk c ^ value_swizzle(r): both the DMA's
+// 64 chunks and ds_read_b64_tr_b16's (4 rows x 32 bytes per 16 lanes) touch every bank once.
+template <int D>
+__device__ __forceinline__ uint32_t value_swizzle(uint32_t row) {
+  return D >= 128 ? (row & 7u) << 1 : row & 7u;
+}
+
+// Loads from addresses as numbers, of global memory (without the address space they
+// would be flat loads, which count as LDS accesses too).
+__device__ __forceinline__ void dma16(uint64_t from, uint8_t* lds) {
+  __builtin_amdgcn_global_load_lds((const GLOBAL_AS void*)from, (LDS_AS void*)lds, 16, 0, 0);
+}
+__device__ __forceinline__ u32x4 load16_at(uint64_t from) { return *(const GLOBAL_AS u32x4*)from; }
+// at if use, else otherwise, selected without a branch.
+__device__ __forceinline__ uint64_t pick(bool use, uint64_t at, uint64_t otherwise) {
+  asm volatile("" : "+v"(at));
+  return use ? at : otherwise;
+}
+
+__device__ __forceinline__ float max_of_query(float x) {  // the four lanes that hold one query
+  x = fmaxf(x, __shfl_xor(x, 16, kWave));
+  return fmaxf(x, __shfl_xor(x, 32, kWave));
+}
+__device__ __forceinline__ float sum_of_query(float x) {
+  x += __shfl_xor(x, 16, kWave);
+  return x + __shfl_xor(x, 32, kWave);
+}
+
+// Partial results of a launch: slots of a workgroup's first and last segment, each
+// 16 * MT rows of D fp32 and their (reference point, sum) pairs; without
+// memory every segment is one workgroup's.
+struct DecodeSplit {
+  float* rows;
+  float* sums;
+  uint32_t* counters;  // by the workgroup that holds a segment's first part
+};
+// Results over the shared keys, from a launch before this one: for every (row,
+// query head) `parts` unnormalised rows and (reference point, sum) pairs.
+struct SharedParts {
+  const float* rows;
+  const float* sums;
+  uint32_t parts;
+};
+constexpr uint32_t kMaxParts = 128;       // of one segment
+constexpr uint32_t kMaxSharedParts = 32;
+constexpr uint32_t kFullChip = 512;       // workgroups that are resident at once
+constexpr uint32_t kMostChunks = 2048;    // workgroups of a launch at most
+
+template <int D, int DC, int MT>
+struct Decode {
+  static constexpr uint32_t kKeys = D > 64 ? 32 : 64;  // keys per tile: 4 KiB of keys per wave at least
+  static constexpr uint32_t kTileBytes = kKeys * D * 2;
+  static constexpr uint32_t kKT = kKeys / 16, kKS = DC / 32, kDT = DC / 16, kHalves = kKeys / 32;
+  static constexpr uint32_t kQueries = 16 * MT;
+  static constexpr uint32_t kDma = kTileBytes / 1024;  // DMA instructions of a wave per tile
+  static constexpr uint32_t kDmaRows = 1024 / (D * 2);
+};
+
+// Units of sequence q: query tiles x key heads, each of `tiles` key tiles (at
+// least one, so that rows without keys are written).
+struct Units {
+  uint64_t segments;
+  uint32_t tiles;
+};
+template <uint32_t Keys, uint32_t Queries>
+__device__ __forceinline__ Units units_of(const BatchSequence& q, uint32_t group, uint32_t key_heads, uint32_t first_key) {
+  Units u;
+  u.segments = ((uint64_t)q.rows * group + Queries - 1) / Queries * key_heads;
+  const uint32_t keys = q.keys > first_key ? q.keys - first_key : 0;
+  u.tiles = keys == 0 ? 1 : (uint32_t)(((uint64_t)keys + Keys - 1) / Keys);
+  return u;
+}
+
+__device__ __forceinline__ uint64_t shuffle_up(uint64_t x, uint32_t by) {
+  const uint32_t lo = __shfl_up((uint32_t)x, by, kWave), hi = __shfl_up((uint32_t)(x >> 32), by, kWave);
+  return lo | (uint64_t)hi << 32;
+}
+__device__ __forceinline__ uint64_t from_lane(uint64_t x, uint32_t lane) {
+  const uint32_t lo = __shfl((uint32_t)x, lane, kWave), hi = __shfl((uint32_t)(x >> 32), lane, kWave);
+  return lo | (uint64_t)hi << 32;
+}
+// Values that all lanes hold alike, into scalar registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  return uniform((uint32_t)x) | (uint64_t)uniform((uint32_t)(x >> 32)) << 32;
+}
+__device__ __forceinline__ BatchSequence uniform(BatchSequence q) {
+  return {uniform(q.first), uniform(q.rows), uniform(q.keys), (int)uniform((uint32_t)q.length)};
+}
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint64_t scan(uint64_t x) {
+  for (uint32_t o = 1; o < (uint32_t)kWave; o *= 2) {
+    const uint64_t y = shuffle_up(x, o);
+    if (threadIdx.x % kWave >= o) x += y;
+  }
+  return x;
+}
+
+template <int D, int DC, int MT>
+__global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_decode_kernel(
+    PagedAttentionArgs a, float scale_log2, uint32_t first_key, uint32_t most_chunks, DecodeSplit split,
+    SharedParts shared) {
+  using C = Decode<D, DC, MT>;
+  constexpr uint32_t kKeys = C::kKeys, kKT = C::kKT, kKS = C::kKS, kDT = C::kDT, kHalves = C::kHalves;
+  constexpr uint32_t kQueries = C::kQueries, kTile = C::kTileBytes, kRowBytes = D * 2;
+  // Two stages, distinct objects, so that the compiler sees that the DMA into
+  // one never meets the reads of the other; a wave's tile at wave * kTile.
+  __shared__ __attribute__((aligned(1024))) uint8_t stage0[kWaves * kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t stage1[kWaves * kTile];
+  __shared__ float wave_sums[kWaves][kQueries][2];
+  // Weights of a query's parts: the waves' and the shared keys'.  Where a segment
+  // of several workgroups is merged, its parts' and the shared keys', in stage 0.
+  constexpr uint32_t kFewParts = kWaves + kMaxSharedParts, kManyParts = kMaxParts + kMaxSharedParts;
+  __shared__ float few_weights[kQueries * kFewParts];
+  static_assert(kQueries * kManyParts * 4 <= kWaves * kTile, "the weights of a merge fit a stage");
+  __shared__ uint32_t arrived;
+
+  const uint32_t lane = threadIdx.x % kWave, r16 = lane % 16, g4 = lane / 16;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t group = a.query_heads / a.key_heads;
+  const PagedBatch& b = a.batch;
+  const bool may_split = split.rows != nullptr;
+
+  // ---- this workgroup's chunk of the line of units ----
+  uint64_t total = 0, segments = 0;
+  uint32_t longest = 1;
+  for (uint32_t s = lane; s < b.sequences; s += kWave) {
+    const Units u = units_of<kKeys, kQueries>(sequence_at(b, s, a.rows), group, a.key_heads, first_key);
+    total += u.segments * u.tiles;
+    segments += u.segments;
+    if (u.segments > 0 && u.tiles > longest) longest = u.tiles;
+  }
+  total = uniform(from_lane(scan(total), kWave - 1));
+  segments = uniform(from_lane(scan(segments), kWave - 1));
+  for (uint32_t o = 32; o > 0; o >>= 1) {
+    const uint32_t other = __shfl_xor(longest, o, kWave);
+    longest = other > longest ? other : longest;
+  }
+  longest = uniform(longest);
+  if (total == 0) return;
+  // At least a tile per wave where segments are that long, and enough chunks to fill the
+  // chip; from 8 tiles per wave on one chunk per resident workgroup, so that the scan, a
+  // segment's start and its merge are paid once.
+  uint64_t chunk = (total + most_chunks - 1) / most_chunks;
+  const uint64_t usual = total / segments < kWaves ? total / segments : kWaves;
+  if (chunk < usual) chunk = usual;
+  const uint64_t resident = (total + kFullChip - 1) / kFullChip;
+  if (resident >= 8 * kWaves && chunk < resident) chunk = resident;
+  if (chunk < (longest + kMaxParts - 2) / (kMaxParts - 1)) chunk = (longest + kMaxParts - 2) / (kMaxParts - 1);
+  const uint64_t begin = blockIdx.x * chunk;
+  if (begin >= total) return;
+  const uint64_t end = begin + chunk < total ? begin + chunk : total;
+  uint32_t s = 0;
+  uint64_t sequence_begin = 0;  // first unit of sequence s
+  for (uint32_t base = 0; base < b.sequences; base += kWave) {
+    uint64_t mine = 0;
+    if (base + lane < b.sequences) {
+      const Units u = units_of<kKeys, kQueries>(sequence_at(b, base + lane, a.rows), group, a.key_heads, first_key);
+      mine = u.segments * u.tiles;
+    }
+    const uint64_t upto = scan(mine), all = uniform(from_lane(upto, kWave - 1));
+    if (begin < sequence_begin + all) {
+      const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(sequence_begin + upto > begin));
+      s = base + at;
+      sequence_begin += uniform(from_lane(upto - mine, at));
+      break;
+    }
+    sequence_begin += all;
+  }
+
+  // Per-lane offsets of the tile accesses.
+  const uint64_t head_bytes = (uint64_t)b.page_rows * a.width * 2;
+  const uint32_t row_mask = b.page_rows - 1;
+  uint32_t vbase;
+  {
+    const uint32_t row = 4 * g4 + r16 / 4, c1 = (r16 % 4) / 2;
+    vbase = row * kRowBytes + ((c1 ^ value_swizzle<D>(row)) << 4) + 8 * (r16 % 2);
+  }
+  uint8_t* const my0 = stage0 + wave * kTile;
+  uint8_t* const my1 = stage1 + wave * kTile;
+
+  uint64_t unit = begin;
+  while (unit < end) {
+    const BatchSequence q = uniform(sequence_at(b, s, a.rows));
+    const Units u = units_of<kKeys, kQueries>(q, group, a.key_heads, first_key);
+    const uint64_t units = u.segments * u.tiles;
+    if (unit >= sequence_begin + units) {  // also a sequence without rows
+      sequence_begin += units;
+      ++s;
+      continue;
+    }
+    const uint64_t within = unit - sequence_begin;
+    const uint32_t tile_first = (uint32_t)(within % u.tiles);
+    const uint64_t segment = within / u.tiles, segment_begin = unit - tile_first, segment_end = segment_begin + u.tiles;
+    const uint32_t key_head = (uint32_t)(segment % a.key_heads);
+    const uint64_t query0 = segment / a.key_heads * kQueries;  // of the sequence's rows x group
+    if (!may_split && tile_first != 0) {  // begun, and finished, by the workgroup before
+      unit = segment_end;
+      continue;
+    }
+    const uint64_t stop = may_split && segment_end > end ? end : segment_end;
+    const uint32_t tile_last = tile_first + (uint32_t)(stop - unit);  // one past
+
+    // The wave's queries: fragment (mt, ks) holds columns 32 ks + 8 (l / 16) .. + 7 of
+    // query 16 mt + l % 16; padding queries repeat the last one, with no key allowed.
+    const uint64_t queries = (uint64_t)q.rows * group - query0;  // left, at least 1
+    half8_t qf[MT][kKS];
+    uint32_t limit[MT];  // keys that this lane's query may read
+#pragma unroll
+    for (uint32_t mt = 0; mt < MT; ++mt) {
+      uint32_t m = 16 * mt + r16;
+      const bool real = m < queries;
+      m = real ? m : (uint32_t)queries - 1;
+      const uint32_t row = q.first + (uint32_t)((query0 + m) / group), head = (uint32_t)((query0 + m) % group);
+      const half_t* from = (const half_t*)a.query + (uint64_t)row * a.query_row_stride +
+                           (uint64_t)(key_head * group + head) * a.width;
+      const int position = row_position(q.length, (int)(q.first + q.rows), row);
+      limit[mt] = real ? readable_keys(q, position, a.causal) : 0;
+#pragma unroll
+      for (uint32_t ks = 0; ks < kKS; ++ks) {
+        const uint32_t d0 = ks * 32 + g4 * 8;
+        qf[mt][ks] = __builtin_bit_cast(half8_t, d0 < a.width ? load16(from + d0) : u32x4{0, 0, 0, 0});
+      }
+    }
+    float4_t o[kDT][MT];
+    float m_run[MT], l_run[MT];
+#pragma unroll
+    for (uint32_t mt = 0; mt < MT; ++mt) {
+      m_run[mt] = -INFINITY;
+      l_run[mt] = 0.0f;
+#pragma unroll
+      for (uint32_t dt = 0; dt < kDT; ++dt) o[dt][mt] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    const uint64_t cache = (uint64_t)a.cache + key_head * head_bytes, value_bytes = a.key_heads * head_bytes;
+    const uint32_t page_bytes = (uint32_t)(b.page_elements * 2);  // launch_attention_pages
+    const uint64_t zeros = (uint64_t)kZeros;
+    // Keys of this part, from first_key on; lanes past a tile's rows have none.
+    const uint32_t all_keys = q.keys > first_key ? q.keys - first_key : 0;
+    const uint32_t part_keys = (uint64_t)tile_last * kKeys < all_keys ? tile_last * kKeys : all_keys;
+    const uint32_t lane_keys = lane < kKeys ? part_keys : 0;
+    // Table entry of this lane's row of tile t; page_at: its page, -1 for none.
+    auto entry = [&](uint32_t t) __attribute__((always_inline)) {
+      const uint32_t key = first_key + t * kKeys + lane;
+      const uint64_t at = (uint64_t)(b.table + (uint64_t)(key < b.shared_rows ? 0 : s) * b.table_columns + (key >> b.page_shift));
+      return *(const GLOBAL_AS int*)pick(t * kKeys + lane < lane_keys, at, zeros);
+    };
+    auto page_at = [&](uint32_t t, int e) __attribute__((always_inline)) {
+      const bool has = (t * kKeys + lane < lane_keys) & ((uint32_t)e < b.pages);
+      return has ? e : -1;
+    };
+    auto row_address = [&](uint32_t t, uint32_t row, int p) __attribute__((always_inline)) {
+      const uint32_t key = first_key + t * kKeys + row;
+      return cache + (uint64_t)(uint32_t)p * page_bytes + (key & row_mask) * (a.width * 2);
+    };
+    // Opaque, so that rows and chunks are not kept in registers between tiles.
+    auto opaque = [](uint32_t x) __attribute__((always_inline)) {
+      asm volatile("" : "+v"(x));
+      return x;
+    };
+    // Tile t's keys into registers and its values into LDS; zeros for rows without a page.
+    half8_t kf[kKT][kKS];
+    auto fetch_keys = [&](uint32_t t, int page) __attribute__((always_inline)) {
+      const uint32_t lane_v = opaque(lane);
+#pragma unroll
+      for (uint32_t kt = 0; kt < kKT; ++kt) {
+        const uint32_t row = 16 * kt + lane_v % 16;
+        const int p = __shfl(page, row, kWave);
+        const uint64_t at = row_address(t, row, p);
+#pragma unroll
+        for (uint32_t ks = 0; ks < kKS; ++ks) {
+          const uint32_t d0 = ks * 32 + (lane_v / 16) * 8;
+          kf[kt][ks] = __builtin_bit_cast(half8_t, load16_at(pick((p >= 0) & (d0 < a.width), at + d0 * 2, zeros)));
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);  // on the way before the arithmetic that follows
+    };
+    auto fetch_values = [&](uint32_t t, int page, uint8_t* lv) __attribute__((always_inline)) {
+      const uint32_t lane_v = opaque(lane);
+#pragma unroll
+      for (uint32_t i = 0; i < C::kDma; ++i) {
+        const uint32_t row = i * C::kDmaRows + lane_v / (D / 8);
+        const uint32_t column = ((lane_v % (D / 8)) ^ value_swizzle<D>(row)) * 8;
+        const int p = __shfl(page, row, kWave);
+        dma16(pick((p >= 0) & (column < a.width), row_address(t, row, p) + value_bytes + column * 2, zeros), lv + i * 1024);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto scores = [&](float4_t (&sc)[kKT][MT]) __attribute__((always_inline)) {
+#pragma unroll
+      for (uint32_t kt = 0; kt < kKT; ++kt)
+#pragma unroll
+        for (uint32_t mt = 0; mt < MT; ++mt) {
+          sc[kt][mt] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (uint32_t ks = 0; ks < kKS; ++ks)
+            sc[kt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][ks], qf[mt][ks], sc[kt][mt], 0, 0, 0);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // Softmax of tile t's scores, rows of `valid`, and the output with the values in lv.
+    auto update = [&](uint32_t t, uint64_t valid, float4_t (&sc)[kKT][MT], const uint8_t* lv) __attribute__((always_inline)) {
+      const uint32_t key0 = first_key + t * kKeys;
+      half8_t high[kHalves][MT], low[kHalves][MT];
+#pragma unroll
+      for (uint32_t mt = 0; mt < MT; ++mt) {
+        // sc[kt][mt][e]: key 16 kt + 4 (l / 16) + e of query 16 mt + l % 16.
+        const uint64_t mine = valid >> (4 * g4);
+        const uint32_t left = limit[mt] > key0 + 4 * g4 ? limit[mt] - (key0 + 4 * g4) : 0;
+        float top = -INFINITY;
+#pragma unroll
+        for (uint32_t kt = 0; kt < kKT; ++kt)
+#pragma unroll
+          for (uint32_t e = 0; e < 4; ++e) {
+            const uint32_t x = 16 * kt + e;
+            sc[kt][mt][e] = (mine >> x & 1) && x < left ? sc[kt][mt][e] * scale_log2 : -INFINITY;
+            top = fmaxf(top, sc[kt][mt][e]);
+          }
+        top = max_of_query(top);
+        const float m_new = fmaxf(m_run[mt], top);
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;  // no NaN from (-inf) - (-inf)
+        const float alpha = __builtin_amdgcn_exp2f(m_run[mt] - m_use);
+        m_run[mt] = m_new;
+        float sum = 0.0f;
+#pragma unroll
+        for (uint32_t kk = 0; kk < kHalves; ++kk)
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e) {
+            const float p = __builtin_amdgcn_exp2f(sc[2 * kk + e / 4][mt][e % 4] - m_use);
+            sum += p;
+            high[kk][mt][e] = (half_t)p;
+            low[kk][mt][e] = (half_t)(p - (float)high[kk][mt][e]);
+          }
+        l_run[mt] = l_run[mt] * alpha + sum;
+#pragma unroll
+        for (uint32_t dt = 0; dt < kDT; ++dt) o[dt][mt] *= alpha;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      uint32_t vbase_v = vbase;
+      asm volatile("" : "+v"(vbase_v));
+#pragma unroll
+      for (uint32_t kk = 0; kk < kHalves; ++kk)
+#pragma unroll
+        for (uint32_t dt = 0; dt < kDT; ++dt) {
+          const uint8_t* p = lv + (vbase_v ^ (dt << 5)) + 32 * kk * kRowBytes;
+          const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS short4_t*)p);
+          const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS short4_t*)(p + 16 * kRowBytes));
+          const half8_t v = __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (uint32_t mt = 0; mt < MT; ++mt) {
+            o[dt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, high[kk][mt], o[dt][mt], 0, 0, 0);
+            o[dt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, low[kk][mt], o[dt][mt], 0, 0, 0);
+          }
+        }
+    };
+    // What this wave has asked for has arrived, and its reads of the other
+    // stage are done.
+    auto settle = [&]() __attribute__((always_inline)) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    };
+
+    uint32_t t = tile_first + wave;
+    if (t < tile_last) {
+      int page = page_at(t, entry(t));
+      int e = entry(t + kWaves);
+      uint64_t valid = __ballot(page >= 0);
+      fetch_values(t, page, my0);
+      fetch_keys(t, page);
+      // One tile: the next one's values on their way, the scores, the next one's keys on
+      // their way into the registers just read, the rest.
+      auto step = [&](uint8_t* lv, uint8_t* next) __attribute__((always_inline)) {
+        settle();
+        page = page_at(t + kWaves, e);
+        e = entry(t + 2 * kWaves);
+        fetch_values(t + kWaves, page, next);
+        float4_t sc[kKT][MT];
+        scores(sc);
+        fetch_keys(t + kWaves, page);
+        update(t, valid, sc, lv);
+        valid = __ballot(page >= 0);
+        t += kWaves;
+      };
+      while (true) {
+        step(my0, my1);
+        if (t >= tile_last) break;
+        step(my1, my0);
+        if (t >= tile_last) break;
+      }
+    }
+    settle();
+
+    // ---- the waves' results joined ----
+    // Lane numbers made opaque, so that nothing of this is computed before the key loop.
+    const uint32_t tid = opaque(threadIdx.x), r16 = tid % 16, g4 = tid % kWave / 16;
+    // A wave's rows, fp32 [kQueries][D], fill its stage 0 and 1 (16 rows of each).
+    static_assert(16 * D * 4 <= kTile || D == 64, "a stage holds 16 rows");
+#pragma unroll
+    for (uint32_t mt = 0; mt < MT; ++mt) {
+      const float l = sum_of_query(l_run[mt]);
+      if (g4 == 0) {
+        wave_sums[wave][16 * mt + r16][0] = m_run[mt];
+        wave_sums[wave][16 * mt + r16][1] = l;
+      }
+      float* mine = reinterpret_cast<float*>(mt == 0 ? my0 : my1) + r16 * D;
+#pragma unroll
+      for (uint32_t dt = 0; dt < kDT; ++dt)
+        *reinterpret_cast<float4_t*>(mine + ((dt * 4 + g4) ^ (r16 & 7)) * 4) = o[dt][mt];
+    }
+    __syncthreads();
+    const uint32_t real = queries < kQueries ? (uint32_t)queries : kQueries;
+    const uint32_t quads = a.width / 4;
+    // (row, head) of query m, for the shared keys' parts and the output.
+    auto output_row = [&](uint32_t m) __attribute__((always_inline)) {
+      const uint64_t x = query0 + m;
+      return (uint64_t)(q.first + (uint32_t)(x / group)) * a.query_heads + key_head * group + (uint32_t)(x % group);
+    };
+    auto wave_quad = [&](uint32_t w, uint32_t m, uint32_t c) __attribute__((always_inline)) {
+      const float* from = reinterpret_cast<const float*>((m < 16 ? stage0 : stage1) + w * kTile) + (m % 16) * D;
+      return *reinterpret_cast<const float4_t*>(from + (c ^ (m & 7)) * 4);
+    };
+    auto store = [&](uint32_t m, uint32_t c, float4_t x) __attribute__((always_inline)) {
+      half4_t h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = (half_t)x[e];
+      *reinterpret_cast<half4_t*>((half_t*)a.out + output_row(m) * a.width + c * 4) = h;
+    };
+    // Weights of `parts` results and of the shared keys' parts of each query, of
+    // which `load` gives the (reference point, sum) pairs: exp2(m - max m) / sum.
+    auto weigh = [&](float* weights, uint32_t most, uint32_t parts, auto load) __attribute__((always_inline)) {
+      const uint32_t all = parts + shared.parts;
+      for (uint32_t m = tid; m < real; m += kThreads) {
+        float* w = weights + m * most;
+        const float* pairs = shared.sums + output_row(m) * shared.parts * 2;
+        float top = -INFINITY, sum = 0.0f;
+        for (uint32_t z = 0; z < all; ++z) {
+          w[z] = z < parts ? load(z, m, 0) : pairs[2 * (z - parts)];
+          top = fmaxf(top, w[z]);
+        }
+        top = top == -INFINITY ? 0.0f : top;
+        for (uint32_t z = 0; z < all; ++z) {
+          w[z] = __builtin_amdgcn_exp2f(w[z] - top);
+          sum += w[z] * (z < parts ? load(z, m, 1) : pairs[2 * (z - parts) + 1]);
+        }
+        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (uint32_t z = 0; z < all; ++z) w[z] *= inverse;
+      }
+      __syncthreads();
+    };
+    auto shared_quads = [&](const float* w, uint32_t m, uint32_t c, float4_t x) __attribute__((always_inline)) {
+      const float* from = shared.rows + output_row(m) * shared.parts * a.width + c * 4;
+      for (uint32_t z = 0; z < shared.parts; ++z)
+        x += *reinterpret_cast<const float4_t*>(from + (uint64_t)z * a.width) * w[z];
+      return x;
+    };
+
+    if (stop - unit == u.tiles) {  // the whole segment
+      weigh(few_weights, kFewParts, kWaves, [&](uint32_t z, uint32_t m, uint32_t which) { return wave_sums[z][m][which]; });
+      for (uint32_t i = tid; i < real * quads; i += kThreads) {
+        const uint32_t m = i / quads, c = i % quads;
+        float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) x += wave_quad(w, m, c) * few_weights[m * kFewParts + w];
+        store(m, c, shared_quads(few_weights + m * kFewParts + kWaves, m, c, x));
+      }
+    } else {
+      // This part: slot 2 w of workgroup w for the segment it began in (or
+      // before), 2 w + 1 for one begun later in its chunk.
+      const uint64_t first_part = segment_begin / chunk, last_part = (segment_end - 1) / chunk;
+      const uint32_t parts = (uint32_t)(last_part - first_part) + 1;
+      auto slot_of = [&](uint64_t w) { return 2 * w + (segment_begin > w * chunk ? 1 : 0); };
+      const uint64_t slot = slot_of(blockIdx.x);
+      float* rows = split.rows + slot * kQueries * D;
+      float* sums = split.sums + slot * kQueries * 2;
+      for (uint32_t i = tid; i < real * quads; i += kThreads) {
+        const uint32_t m = i / quads, c = i % quads;
+        float top = -INFINITY;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, wave_sums[w][m][0]);
+        const float use = top == -INFINITY ? 0.0f : top;
+        float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+        float l = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) {
+          const float f = __builtin_amdgcn_exp2f(wave_sums[w][m][0] - use);
+          l += f * wave_sums[w][m][1];
+          x += wave_quad(w, m, c) * f;
+        }
+        store_device4(rows + m * D + c * 4, x);
+        if (c == 0) {
+          store_device(sums + 2 * m, top);
+          store_device(sums + 2 * m + 1, l);
+        }
+      }
+      if (arrive(split.counters + first_part, parts, &arrived)) {
+        float* weights = reinterpret_cast<float*>(stage0);
+        weigh(weights, kManyParts, parts, [&](uint32_t z, uint32_t m, uint32_t which) {
+          return load_device(split.sums + (slot_of(first_part + z) * kQueries + m) * 2 + which);
+        });
+        for (uint32_t i = tid; i < real * quads; i += kThreads) {
+          const uint32_t m = i / quads, c = i % quads;
+          const float* w = weights + m * kManyParts;
+          float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+          // Eight loads in flight (past the last part: the last one again, not added).
+          for (uint32_t z0 = 0; z0 < parts; z0 += 8) {
+            float4_t y[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+              const uint32_t z = z0 + j < parts ? z0 + j : parts - 1;
+              y[j] = load_device4(split.rows + (slot_of(first_part + z) * kQueries + m) * D + c * 4);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+              if (z0 + j < parts) x += y[j] * w[z0 + j];
+          }
+          store(m, c, shared_quads(w + parts, m, c, x));
+        }
+      }
+    }
+    __syncthreads();  // the stages, sums and weights are free for the next segment
+    unit = stop;
+  }
+}
+
 int launch_general(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2) {
   constexpr uint32_t kMostRows = 1u << 24;  // a grid dimension holds less than 2^32 threads
   for (uint64_t done = 0; done < a.rows; done += kMostRows) {
@@ -91,6 +631,47 @@ int launch_general(hipStream_t stream, const PagedAttentionArgs& a, float scale_
   return 0;
 }
 
+template <int D, int DC, int MT>
+int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t first_key,
+                     const SharedParts& shared) {
+  constexpr uint64_t kSlotFloats = Decode<D, DC, MT>::kQueries * (D + 2);
+  DecodeSplit split{nullptr, nullptr, nullptr};
+  uint64_t chunks = kMostChunks;
+  if (a.workspace.data) {
+    const uint64_t fit = a.workspace.bytes / (2 * kSlotFloats * sizeof(float));
+    if (chunks > fit) chunks = fit;
+    if (chunks > a.workspace.counter_count) chunks = a.workspace.counter_count;
+  }
+  if (a.workspace.data && chunks > 0) {
+    split.rows = (float*)a.workspace.data;
+    split.sums = split.rows + 2 * chunks * Decode<D, DC, MT>::kQueries * D;
+    split.counters = a.workspace.counters;
+  } else {
+    chunks = kMostChunks;
+  }
+  hipLaunchKernelGGL((attention_pages_decode_kernel<D, DC, MT>), dim3((uint32_t)chunks), dim3(kThreads), 0, stream,
+                     a, scale_log2, first_key, (uint32_t)chunks, split, shared);
+  return hip_status(hipGetLastError());
+}
+template <int D, int DC>
+int launch_decode_queries(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t first_key,
+                          const SharedParts& shared) {
+  const uint64_t queries = (uint64_t)a.max_rows * (a.query_heads / a.key_heads);
+  // Two tiles of queries at 256 columns do not fit the registers.
+  if constexpr (D <= 128)
+    if (queries > 16) return launch_decode_as<D, DC, 2>(stream, a, scale_log2, first_key, shared);
+  return launch_decode_as<D, DC, 1>(stream, a, scale_log2, first_key, shared);
+}
+int launch_decode(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t first_key,
+                  const SharedParts& shared) {
+  if (a.width > 192) return launch_decode_queries<256, 256>(stream, a, scale_log2, first_key, shared);
+  if (a.width > 128) return launch_decode_queries<256, 192>(stream, a, scale_log2, first_key, shared);
+  if (a.width > 96) return launch_decode_queries<128, 128>(stream, a, scale_log2, first_key, shared);
+  if (a.width > 64) return launch_decode_queries<128, 96>(stream, a, scale_log2, first_key, shared);
+  if (a.width > 32) return launch_decode_queries<64, 64>(stream, a, scale_log2, first_key, shared);
+  return launch_decode_queries<64, 32>(stream, a, scale_log2, first_key, shared);
+}
+
 }  // namespace
 
 int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a) {
@@ -98,7 +679,11 @@ int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a) {
   if (((uintptr_t)a.query | (uintptr_t)a.cache | (uintptr_t)a.out) % 2 != 0 || batch_addresses(a.batch) % 4 != 0)
     return IPUS_ERROR_INVALID_ARGUMENT;
   const float scale_log2 = a.scale * kLog2e;
-  return launch_general(stream, a, scale_log2);
+  const bool vectors = a.width % 8 == 0 && a.query_row_stride % 8 == 0 &&
+                       ((uintptr_t)a.query | (uintptr_t)a.cache) % 16 == 0 && (uintptr_t)a.out % 8 == 0;
+  // A page's bytes fit 32 bits, for the tile loads' addresses.
+  if (!vectors || a.width > 256 || a.batch.page_elements * 2 > 0xffffffffull) return launch_general(stream, a, scale_log2);
+  return launch_decode(stream, a, scale_log2, 0, SharedParts{nullptr, nullptr, 0});
 }
 
 }  // namespace ipus

@@ -279,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, uint32_t
   // A wave finds each row's place.
   for (uint32_t r = threadIdx.x / kWave; r < rows; r += kThreads / kWave) {
     const RowPlace p = find_row(a.batch, row0 + r);
-    const int64_t page = p.position < 0 ? -1 : page_of(a.batch, p.sequence, (uint32_t)p.position);
+    const int page = p.position < 0 ? -1 : page_of(a.batch, p.sequence, (uint32_t)p.position);
     if (threadIdx.x % kWave == 0) {
       const uint64_t in_page = (uint32_t)p.position & (a.batch.page_rows - 1);
       target[r] = page < 0 ? -1 : (int64_t)((uint64_t)page * a.batch.page_elements + in_page * a.width);

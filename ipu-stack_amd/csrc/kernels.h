@@ -7,6 +7,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "page_lookup.h"
 #include "tile_choice.h"
 
 namespace ipus {
@@ -121,16 +122,6 @@ struct RotaryArgs {
   bool interleaved, f32;
 };
 int launch_rotary(hipStream_t stream, const RotaryArgs& a);
-
-// A ragged batch over a paged cache (pages.h).
-struct PagedBatch {
-  const int* table;        // [sequences][table_columns]
-  const int* row_offsets;  // [sequences + 1]
-  const int* lengths;      // [sequences]
-  uint32_t sequences, table_columns, pages, page_rows, page_shift;
-  uint32_t shared_rows = 0;  // positions that every sequence reads through the first one's table
-  uint64_t page_elements;    // 2 x key heads x page_rows x width
-};
 
 // New keys and values of the batch's rows into the cache (k_rotary.hip).
 struct AppendArgs {
