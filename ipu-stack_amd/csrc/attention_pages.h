@@ -1,0 +1,129 @@
+// Device helpers of the paged attention kernels: loads that need no branch, LDS tiles,
+// and the scan that finds a workgroup's place in a ragged batch.
+#pragma once
+
+#include "../../include/ipus.h"
+#include "kernels.h"
+#include "pages.h"
+
+#define LDS_AS __attribute__((address_space(3)))
+#define GLOBAL_AS __attribute__((address_space(1)))
+typedef short short4_t __attribute__((vector_size(8)));
+
+namespace ipus {
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kWaves = kThreads / kWave;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+inline int hip_status(hipError_t e) { return e == hipSuccess ? 0 : IPUS_ERROR_HIP_BASE - (int)e; }
+
+// 16 bytes of zeros: what a lane loads for keys that are not to be read and for columns
+// past the width, so that loads need no branch (with branches the compiler cannot count
+// them and waits for all) and nothing that is not the sequence's meets a product.
+__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+// LDS rows of D fp16, 16-byte chunk c of row r at chunk c ^ value_swizzle(r): both the DMA's
+// 64 chunks and ds_read_b64_tr_b16's (4 rows x 32 bytes per 16 lanes) touch every bank once.
+template <int D>
+__device__ __forceinline__ uint32_t value_swizzle(uint32_t row) {
+  return D >= 128 ? (row & 7u) << 1 : row & 7u;
+}
+
+// Loads from addresses as numbers, of global memory (without the address space they
+// would be flat loads, which count as LDS accesses too).
+__device__ __forceinline__ void dma16(uint64_t from, uint8_t* lds) {
+  __builtin_amdgcn_global_load_lds((const GLOBAL_AS void*)from, (LDS_AS void*)lds, 16, 0, 0);
+}
+__device__ __forceinline__ u32x4 load16_at(uint64_t from) { return *(const GLOBAL_AS u32x4*)from; }
+// at if use, else otherwise, selected without a branch.
+__device__ __forceinline__ uint64_t pick(bool use, uint64_t at, uint64_t otherwise) {
+  asm volatile("" : "+v"(at));
+  return use ? at : otherwise;
+}
+
+__device__ __forceinline__ float max_of_query(float x) {  // the four lanes that hold one query
+  x = fmaxf(x, __shfl_xor(x, 16, kWave));
+  return fmaxf(x, __shfl_xor(x, 32, kWave));
+}
+__device__ __forceinline__ float sum_of_query(float x) {
+  x += __shfl_xor(x, 16, kWave);
+  return x + __shfl_xor(x, 32, kWave);
+}
+
+__device__ __forceinline__ uint64_t shuffle_up(uint64_t x, uint32_t by) {
+  const uint32_t lo = __shfl_up((uint32_t)x, by, kWave), hi = __shfl_up((uint32_t)(x >> 32), by, kWave);
+  return lo | (uint64_t)hi << 32;
+}
+__device__ __forceinline__ uint64_t from_lane(uint64_t x, uint32_t lane) {
+  const uint32_t lo = __shfl((uint32_t)x, lane, kWave), hi = __shfl((uint32_t)(x >> 32), lane, kWave);
+  return lo | (uint64_t)hi << 32;
+}
+// Values that all lanes hold alike, into scalar registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  return uniform((uint32_t)x) | (uint64_t)uniform((uint32_t)(x >> 32)) << 32;
+}
+__device__ __forceinline__ BatchSequence uniform(BatchSequence q) {
+  return {uniform(q.first), uniform(q.rows), uniform(q.keys), (int)uniform((uint32_t)q.length)};
+}
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint64_t scan(uint64_t x) {
+  for (uint32_t o = 1; o < (uint32_t)kWave; o *= 2) {
+    const uint64_t y = shuffle_up(x, o);
+    if (threadIdx.x % kWave >= o) x += y;
+  }
+  return x;
+}
+
+// The batch's work as one line of units, `units(sequence)` of them for each in turn:
+// how many there are, and the sequence that holds unit `at` (with its first unit).
+// Called by whole waves; the lengths are read twice, from the caches.
+template <typename F>
+__device__ __forceinline__ uint64_t count_units(const PagedBatch& b, F units) {
+  uint64_t total = 0;
+  for (uint32_t s = threadIdx.x % kWave; s < b.sequences; s += kWave) total += units(s);
+  return uniform(from_lane(scan(total), kWave - 1));
+}
+struct UnitPlace {
+  uint32_t sequence;
+  uint64_t first;
+};
+template <typename F>
+__device__ __forceinline__ UnitPlace find_unit(const PagedBatch& b, uint64_t at, F units) {
+  const uint32_t lane = threadIdx.x % kWave;
+  UnitPlace p{0, 0};
+  for (uint32_t base = 0; base < b.sequences; base += kWave) {
+    const uint64_t mine = base + lane < b.sequences ? units(base + lane) : 0;
+    const uint64_t upto = scan(mine), all = uniform(from_lane(upto, kWave - 1));
+    if (at < p.first + all) {
+      const uint32_t holder = (uint32_t)__builtin_ctzll(__ballot(p.first + upto > at));
+      p.sequence = base + holder;
+      p.first += uniform(from_lane(upto - mine, holder));
+      break;
+    }
+    p.first += all;
+  }
+  return p;
+}
+
+// Results over the shared keys, from a launch before the one that joins them: for
+// every (row, query head) `parts` unnormalised rows and (reference point, sum) pairs.
+struct SharedParts {
+  float* rows;
+  float* sums;
+  uint32_t parts;
+};
+constexpr uint32_t kMaxSharedParts = 32;
+constexpr uint32_t kFullChip = 512;  // workgroups that the chip holds at once, two per CU
+
+// The kernels for many query rows per key head (k_attention_blocks.hip): sequences of more
+// than `few` queries (rows x query heads of a key head); and the rows of the whole
+// batch over the shared keys alone.  shared_part_count: into how many parts, at
+// most `most`, those keys are split to fill the chip.
+int launch_attention_blocks(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t few);
+int launch_shared_parts(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const SharedParts& parts);
+uint32_t shared_part_count(const PagedAttentionArgs& a, uint32_t most);
+
+}  // namespace ipus

@@ -5,16 +5,10 @@
 // position lengths[s] - n + i; it reads the keys below lengths[s], when causal
 // those up to its own position.  Keys without a page carry no weight, and a row
 // whose weights are all zero (no key, or only scores of -inf) gives zeros.
-#include "../../include/ipus.h"
-#include "kernels.h"
-#include "pages.h"
+#include "attention_pages.h"
 
 namespace ipus {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-inline int hip_status(hipError_t e) { return e == hipSuccess ? 0 : IPUS_ERROR_HIP_BASE - (int)e; }
 
 // Any width up to 1024, any alignment: a wave per row and query head, one key
 // after the other.
@@ -85,46 +79,6 @@ __global__ __launch_bounds__(kWave) void attention_pages_general_kernel(PagedAtt
 // the second product as the sum of two fp16 values (22 bits): the matrix pipes have time for it here,
 // and the result is off by little more than its own rounding.
 
-#define LDS_AS __attribute__((address_space(3)))
-#define GLOBAL_AS __attribute__((address_space(1)))
-typedef short short4_t __attribute__((vector_size(8)));
-
-constexpr uint32_t kThreads = 256;
-constexpr uint32_t kWaves = kThreads / kWave;
-
-// 16 bytes of zeros: what a lane loads for keys that are not to be read and for columns
-// past the width, so that loads need no branch (with branches the compiler cannot count
-// them and waits for all) and nothing that is not the sequence's meets a product.
-__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
-
-// LDS rows of D fp16, 16-byte chunk c of row r at chunk c ^ value_swizzle(r): both the DMA's
-// 64 chunks and ds_read_b64_tr_b16's (4 rows x 32 bytes per 16 lanes) touch every bank once.
-template <int D>
-__device__ __forceinline__ uint32_t value_swizzle(uint32_t row) {
-  return D >= 128 ? (row & 7u) << 1 : row & 7u;
-}
-
-// Loads from addresses as numbers, of global memory (without the address space they
-// would be flat loads, which count as LDS accesses too).
-__device__ __forceinline__ void dma16(uint64_t from, uint8_t* lds) {
-  __builtin_amdgcn_global_load_lds((const GLOBAL_AS void*)from, (LDS_AS void*)lds, 16, 0, 0);
-}
-__device__ __forceinline__ u32x4 load16_at(uint64_t from) { return *(const GLOBAL_AS u32x4*)from; }
-// at if use, else otherwise, selected without a branch.
-__device__ __forceinline__ uint64_t pick(bool use, uint64_t at, uint64_t otherwise) {
-  asm volatile("" : "+v"(at));
-  return use ? at : otherwise;
-}
-
-__device__ __forceinline__ float max_of_query(float x) {  // the four lanes that hold one query
-  x = fmaxf(x, __shfl_xor(x, 16, kWave));
-  return fmaxf(x, __shfl_xor(x, 32, kWave));
-}
-__device__ __forceinline__ float sum_of_query(float x) {
-  x += __shfl_xor(x, 16, kWave);
-  return x + __shfl_xor(x, 32, kWave);
-}
-
 // Partial results of a launch: slots of a workgroup's first and last segment, each
 // 16 * MT rows of D fp32 and their (reference point, sum) pairs; without
 // memory every segment is one workgroup's.
@@ -133,16 +87,7 @@ struct DecodeSplit {
   float* sums;
   uint32_t* counters;  // by the workgroup that holds a segment's first part
 };
-// Results over the shared keys, from a launch before this one: for every (row,
-// query head) `parts` unnormalised rows and (reference point, sum) pairs.
-struct SharedParts {
-  const float* rows;
-  const float* sums;
-  uint32_t parts;
-};
 constexpr uint32_t kMaxParts = 128;       // of one segment
-constexpr uint32_t kMaxSharedParts = 32;
-constexpr uint32_t kFullChip = 512;       // workgroups that are resident at once
 constexpr uint32_t kMostChunks = 2048;    // workgroups of a launch at most
 
 template <int D, int DC, int MT>
@@ -156,48 +101,26 @@ struct Decode {
 };
 
 // Units of sequence q: query tiles x key heads, each of `tiles` key tiles (at
-// least one, so that rows without keys are written).
+// least one, so that rows without keys are written).  A sequence of more than `few`
+// queries is the other kernel's.
 struct Units {
   uint64_t segments;
   uint32_t tiles;
 };
 template <uint32_t Keys, uint32_t Queries>
-__device__ __forceinline__ Units units_of(const BatchSequence& q, uint32_t group, uint32_t key_heads, uint32_t first_key) {
+__device__ __forceinline__ Units units_of(const BatchSequence& q, uint32_t group, uint32_t key_heads, uint32_t first_key,
+                                          uint64_t few) {
   Units u;
-  u.segments = ((uint64_t)q.rows * group + Queries - 1) / Queries * key_heads;
+  const uint64_t queries = (uint64_t)q.rows * group;
+  u.segments = queries <= few ? (queries + Queries - 1) / Queries * key_heads : 0;
   const uint32_t keys = q.keys > first_key ? q.keys - first_key : 0;
   u.tiles = keys == 0 ? 1 : (uint32_t)(((uint64_t)keys + Keys - 1) / Keys);
   return u;
 }
 
-__device__ __forceinline__ uint64_t shuffle_up(uint64_t x, uint32_t by) {
-  const uint32_t lo = __shfl_up((uint32_t)x, by, kWave), hi = __shfl_up((uint32_t)(x >> 32), by, kWave);
-  return lo | (uint64_t)hi << 32;
-}
-__device__ __forceinline__ uint64_t from_lane(uint64_t x, uint32_t lane) {
-  const uint32_t lo = __shfl((uint32_t)x, lane, kWave), hi = __shfl((uint32_t)(x >> 32), lane, kWave);
-  return lo | (uint64_t)hi << 32;
-}
-// Values that all lanes hold alike, into scalar registers.
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ uint64_t uniform(uint64_t x) {
-  return uniform((uint32_t)x) | (uint64_t)uniform((uint32_t)(x >> 32)) << 32;
-}
-__device__ __forceinline__ BatchSequence uniform(BatchSequence q) {
-  return {uniform(q.first), uniform(q.rows), uniform(q.keys), (int)uniform((uint32_t)q.length)};
-}
-// Sum over the lanes up to this one.
-__device__ __forceinline__ uint64_t scan(uint64_t x) {
-  for (uint32_t o = 1; o < (uint32_t)kWave; o *= 2) {
-    const uint64_t y = shuffle_up(x, o);
-    if (threadIdx.x % kWave >= o) x += y;
-  }
-  return x;
-}
-
 template <int D, int DC, int MT>
 __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_decode_kernel(
-    PagedAttentionArgs a, float scale_log2, uint32_t first_key, uint32_t most_chunks, DecodeSplit split,
+    PagedAttentionArgs a, float scale_log2, uint32_t first_key, uint64_t few, uint32_t most_chunks, DecodeSplit split,
     SharedParts shared) {
   using C = Decode<D, DC, MT>;
   constexpr uint32_t kKeys = C::kKeys, kKT = C::kKT, kKS = C::kKS, kDT = C::kDT, kHalves = C::kHalves;
@@ -221,22 +144,25 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
   const bool may_split = split.rows != nullptr;
 
   // ---- this workgroup's chunk of the line of units ----
-  uint64_t total = 0, segments = 0;
+  uint64_t segments = 0;
   uint32_t longest = 1;
-  for (uint32_t s = lane; s < b.sequences; s += kWave) {
-    const Units u = units_of<kKeys, kQueries>(sequence_at(b, s, a.rows), group, a.key_heads, first_key);
-    total += u.segments * u.tiles;
+  auto units_in = [&](uint32_t s) __attribute__((always_inline)) {
+    const Units u = units_of<kKeys, kQueries>(sequence_at(b, s, a.rows), group, a.key_heads, first_key, few);
+    return u.segments * u.tiles;
+  };
+  const uint64_t total = count_units(b, [&](uint32_t s) __attribute__((always_inline)) {
+    const Units u = units_of<kKeys, kQueries>(sequence_at(b, s, a.rows), group, a.key_heads, first_key, few);
     segments += u.segments;
     if (u.segments > 0 && u.tiles > longest) longest = u.tiles;
-  }
-  total = uniform(from_lane(scan(total), kWave - 1));
+    return u.segments * u.tiles;
+  });
+  if (total == 0) return;
   segments = uniform(from_lane(scan(segments), kWave - 1));
   for (uint32_t o = 32; o > 0; o >>= 1) {
     const uint32_t other = __shfl_xor(longest, o, kWave);
     longest = other > longest ? other : longest;
   }
   longest = uniform(longest);
-  if (total == 0) return;
   // At least a tile per wave where segments are that long, and enough chunks to fill the
   // chip; from 8 tiles per wave on one chunk per resident workgroup, so that the scan, a
   // segment's start and its merge are paid once.
@@ -249,23 +175,9 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
   const uint64_t begin = blockIdx.x * chunk;
   if (begin >= total) return;
   const uint64_t end = begin + chunk < total ? begin + chunk : total;
-  uint32_t s = 0;
-  uint64_t sequence_begin = 0;  // first unit of sequence s
-  for (uint32_t base = 0; base < b.sequences; base += kWave) {
-    uint64_t mine = 0;
-    if (base + lane < b.sequences) {
-      const Units u = units_of<kKeys, kQueries>(sequence_at(b, base + lane, a.rows), group, a.key_heads, first_key);
-      mine = u.segments * u.tiles;
-    }
-    const uint64_t upto = scan(mine), all = uniform(from_lane(upto, kWave - 1));
-    if (begin < sequence_begin + all) {
-      const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(sequence_begin + upto > begin));
-      s = base + at;
-      sequence_begin += uniform(from_lane(upto - mine, at));
-      break;
-    }
-    sequence_begin += all;
-  }
+  const UnitPlace place = find_unit(b, begin, units_in);
+  uint32_t s = place.sequence;
+  uint64_t sequence_begin = place.first;  // first unit of sequence s
 
   // Per-lane offsets of the tile accesses.
   const uint64_t head_bytes = (uint64_t)b.page_rows * a.width * 2;
@@ -281,7 +193,7 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
   uint64_t unit = begin;
   while (unit < end) {
     const BatchSequence q = uniform(sequence_at(b, s, a.rows));
-    const Units u = units_of<kKeys, kQueries>(q, group, a.key_heads, first_key);
+    const Units u = units_of<kKeys, kQueries>(q, group, a.key_heads, first_key, few);
     const uint64_t units = u.segments * u.tiles;
     if (unit >= sequence_begin + units) {  // also a sequence without rows
       sequence_begin += units;
@@ -631,9 +543,14 @@ int launch_general(hipStream_t stream, const PagedAttentionArgs& a, float scale_
   return 0;
 }
 
+// One launch over the sequences of at most `few` queries, keys from first_key on.
+struct DecodeLaunch {
+  uint32_t first_key;
+  uint64_t few;
+  SharedParts shared;
+};
 template <int D, int DC, int MT>
-int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t first_key,
-                     const SharedParts& shared) {
+int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
   constexpr uint64_t kSlotFloats = Decode<D, DC, MT>::kQueries * (D + 2);
   DecodeSplit split{nullptr, nullptr, nullptr};
   uint64_t chunks = kMostChunks;
@@ -642,7 +559,7 @@ int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scal
     if (chunks > fit) chunks = fit;
     if (chunks > a.workspace.counter_count) chunks = a.workspace.counter_count;
   }
-  if (a.workspace.data && chunks > 0) {
+  if (a.workspace.data && chunks >= kWaves) {
     split.rows = (float*)a.workspace.data;
     split.sums = split.rows + 2 * chunks * Decode<D, DC, MT>::kQueries * D;
     split.counters = a.workspace.counters;
@@ -650,26 +567,45 @@ int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scal
     chunks = kMostChunks;
   }
   hipLaunchKernelGGL((attention_pages_decode_kernel<D, DC, MT>), dim3((uint32_t)chunks), dim3(kThreads), 0, stream,
-                     a, scale_log2, first_key, (uint32_t)chunks, split, shared);
+                     a, scale_log2, l.first_key, l.few, (uint32_t)chunks, split, l.shared);
   return hip_status(hipGetLastError());
 }
 template <int D, int DC>
-int launch_decode_queries(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t first_key,
-                          const SharedParts& shared) {
-  const uint64_t queries = (uint64_t)a.max_rows * (a.query_heads / a.key_heads);
+int launch_decode_queries(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
   // Two tiles of queries at 256 columns do not fit the registers.
   if constexpr (D <= 128)
-    if (queries > 16) return launch_decode_as<D, DC, 2>(stream, a, scale_log2, first_key, shared);
-  return launch_decode_as<D, DC, 1>(stream, a, scale_log2, first_key, shared);
+    if ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16) return launch_decode_as<D, DC, 2>(stream, a, scale_log2, l);
+  return launch_decode_as<D, DC, 1>(stream, a, scale_log2, l);
 }
-int launch_decode(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t first_key,
-                  const SharedParts& shared) {
-  if (a.width > 192) return launch_decode_queries<256, 256>(stream, a, scale_log2, first_key, shared);
-  if (a.width > 128) return launch_decode_queries<256, 192>(stream, a, scale_log2, first_key, shared);
-  if (a.width > 96) return launch_decode_queries<128, 128>(stream, a, scale_log2, first_key, shared);
-  if (a.width > 64) return launch_decode_queries<128, 96>(stream, a, scale_log2, first_key, shared);
-  if (a.width > 32) return launch_decode_queries<64, 64>(stream, a, scale_log2, first_key, shared);
-  return launch_decode_queries<64, 32>(stream, a, scale_log2, first_key, shared);
+int launch_decode(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
+  if (a.width > 192) return launch_decode_queries<256, 256>(stream, a, scale_log2, l);
+  if (a.width > 128) return launch_decode_queries<256, 192>(stream, a, scale_log2, l);
+  if (a.width > 96) return launch_decode_queries<128, 128>(stream, a, scale_log2, l);
+  if (a.width > 64) return launch_decode_queries<128, 96>(stream, a, scale_log2, l);
+  if (a.width > 32) return launch_decode_queries<64, 64>(stream, a, scale_log2, l);
+  return launch_decode_queries<64, 32>(stream, a, scale_log2, l);
+}
+
+// Queries of a key head (rows x query heads) up to which a sequence is the decode kernel's.
+constexpr uint32_t kFewQueries = 32;
+
+// The shared keys in a launch of their own: their parts in the workspace's lower
+// end, what is left to the launch that joins them.
+bool plan_shared(const PagedAttentionArgs& a, SharedParts* parts, Workspace* rest) {
+  if (a.batch.shared_rows == 0 || a.batch.sequences < 2 || !a.workspace.data) return false;
+  const uint64_t row_floats = (uint64_t)a.rows * a.query_heads * (a.width + 2);
+  // At least 4 MiB stay for the parts of the keys behind the shared ones.
+  const uint64_t room = a.workspace.bytes > (4u << 20) ? (a.workspace.bytes - (4u << 20)) / sizeof(float) : 0;
+  const uint64_t most = room / row_floats < kMaxSharedParts ? room / row_floats : kMaxSharedParts;
+  parts->parts = most == 0 ? 0 : shared_part_count(a, (uint32_t)most);
+  if (parts->parts == 0) return false;
+  parts->rows = (float*)a.workspace.data;
+  parts->sums = parts->rows + (uint64_t)a.rows * a.query_heads * parts->parts * a.width;
+  const uint64_t used = (row_floats * parts->parts * sizeof(float) + 255) & ~255ull;
+  *rest = a.workspace;
+  rest->data = (uint8_t*)a.workspace.data + used;
+  rest->bytes = a.workspace.bytes - used;
+  return true;
 }
 
 }  // namespace
@@ -683,7 +619,23 @@ int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a) {
                        ((uintptr_t)a.query | (uintptr_t)a.cache) % 16 == 0 && (uintptr_t)a.out % 8 == 0;
   // A page's bytes fit 32 bits, for the tile loads' addresses.
   if (!vectors || a.width > 256 || a.batch.page_elements * 2 > 0xffffffffull) return launch_general(stream, a, scale_log2);
-  return launch_decode(stream, a, scale_log2, 0, SharedParts{nullptr, nullptr, 0});
+  const uint64_t queries = (uint64_t)a.max_rows * (a.query_heads / a.key_heads);
+  if (queries <= kFewQueries) {
+    SharedParts parts;
+    Workspace rest;
+    if (plan_shared(a, &parts, &rest)) {
+      if (int e = launch_shared_parts(stream, a, scale_log2, parts)) return e;
+      PagedAttentionArgs behind = a;
+      behind.workspace = rest;
+      return launch_decode(stream, behind, scale_log2, {a.batch.shared_rows, ~0ull, parts});
+    }
+    return launch_decode(stream, a, scale_log2, {0, ~0ull, {nullptr, nullptr, 0}});
+  }
+  // Sequences of many rows, and those of few beside them, of which there are none
+  // where every sequence has max_rows.
+  const bool mixed = (uint64_t)a.batch.sequences * a.max_rows != a.rows;
+  if (int e = launch_attention_blocks(stream, a, scale_log2, mixed ? kFewQueries : 0)) return e;
+  return mixed ? launch_decode(stream, a, scale_log2, {0, kFewQueries, {nullptr, nullptr, 0}}) : 0;
 }
 
 }  // namespace ipus
