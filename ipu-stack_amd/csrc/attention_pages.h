@@ -77,34 +77,52 @@ __device__ __forceinline__ uint64_t scan(uint64_t x) {
   return x;
 }
 
+// Quotient of values that mostly fit 32 bits (a 64-bit division takes about 100
+// instructions).
+__device__ __forceinline__ uint64_t quotient(uint64_t x, uint64_t y) {
+  return ((x | y) >> 32) == 0 ? (uint32_t)x / (uint32_t)y : x / y;
+}
+
 // The batch's work as one line of units, `units(sequence)` of them for each in turn:
 // how many there are, and the sequence that holds unit `at` (with its first unit).
-// Called by whole waves; the lengths are read twice, from the caches.
+// Used by whole waves.  The lengths of up to 64 sequences are read once.
+struct UnitLine {
+  uint64_t upto, total;  // units up to and with this lane's sequence of the first 64; of all
+};
 template <typename F>
-__device__ __forceinline__ uint64_t count_units(const PagedBatch& b, F units) {
-  uint64_t total = 0;
-  for (uint32_t s = threadIdx.x % kWave; s < b.sequences; s += kWave) total += units(s);
-  return uniform(from_lane(scan(total), kWave - 1));
+__device__ __forceinline__ UnitLine count_units(const PagedBatch& b, F units) {
+  const uint32_t lane = threadIdx.x % kWave;
+  UnitLine l;
+  l.upto = scan(lane < b.sequences ? units(lane) : 0);
+  l.total = uniform(from_lane(l.upto, kWave - 1));
+  if (b.sequences > (uint32_t)kWave) {
+    uint64_t more = 0;
+    for (uint32_t s = kWave + lane; s < b.sequences; s += kWave) more += units(s);
+    l.total += uniform(from_lane(scan(more), kWave - 1));
+  }
+  return l;
 }
 struct UnitPlace {
   uint32_t sequence;
   uint64_t first;
 };
 template <typename F>
-__device__ __forceinline__ UnitPlace find_unit(const PagedBatch& b, uint64_t at, F units) {
+__device__ __forceinline__ UnitPlace find_unit(const PagedBatch& b, const UnitLine& line, uint64_t at, F units) {
   const uint32_t lane = threadIdx.x % kWave;
   UnitPlace p{0, 0};
-  for (uint32_t base = 0; base < b.sequences; base += kWave) {
-    const uint64_t mine = base + lane < b.sequences ? units(base + lane) : 0;
-    const uint64_t upto = scan(mine), all = uniform(from_lane(upto, kWave - 1));
-    if (at < p.first + all) {
-      const uint32_t holder = (uint32_t)__builtin_ctzll(__ballot(p.first + upto > at));
-      p.sequence = base + holder;
-      p.first += uniform(from_lane(upto - mine, holder));
-      break;
-    }
+  uint64_t upto = line.upto;
+  while (true) {
+    const uint64_t all = uniform(from_lane(upto, kWave - 1));
+    if (at < p.first + all) break;
     p.first += all;
+    p.sequence += kWave;
+    if (p.sequence >= b.sequences) break;  // not in the line
+    upto = scan(p.sequence + lane < b.sequences ? units(p.sequence + lane) : 0);
   }
+  const uint64_t past = __ballot(p.first + upto > at);
+  const uint32_t holder = past ? (uint32_t)__builtin_ctzll(past) : 0;
+  p.sequence += holder;
+  if (holder > 0) p.first += uniform(from_lane(upto, holder - 1));
   return p;
 }
 

@@ -16,7 +16,9 @@
 // take a contiguous range of blocks, the query blocks of one (sequence, key head)
 // together, the longest first, so that its keys and values stay in that XCD's L2.
 // Where the blocks are too few for the chip, each one's keys are split over several
-// workgroups, and the last of them to finish joins the parts.
+// workgroups, whose parts a second launch joins: the parts are 128 rows each, and joined
+// in the same launch they would go past the XCD's L2 (about 2 us per MB) to one workgroup
+// per block (333 rows x 16 heads x 72 columns against 2800 keys, 16 MB of parts: 62 us).
 #include "attention_pages.h"
 
 namespace ipus {
@@ -27,13 +29,12 @@ constexpr float kSumLimit = 256.0f;  // as in k_attention.hip
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 // Split keys: unnormalised rows [rows * query_heads][parts][width] fp32, their
-// (reference point, sum) pairs, and a counter per block, 0 between launches
-// (none: another launch joins the parts).
+// (reference point, sum) pairs, and how many parts a row has (unless all have `parts`).
 struct SplitKeys {
   float* rows;
   float* sums;
-  uint32_t* counters;
-  uint32_t parts;  // 1: not split
+  uint32_t* counts;
+  uint32_t parts;  // at most; 1: not split
 };
 constexpr uint32_t kMaxSplits = 16;
 
@@ -56,8 +57,8 @@ __device__ __forceinline__ uint32_t key_swizzle(uint32_t row) {
 // the other kernel takes it.
 template <uint32_t Queries>
 __device__ __forceinline__ uint64_t blocks_of(const BatchSequence& q, uint32_t group, uint32_t key_heads, uint32_t few) {
-  const uint64_t queries = (uint64_t)q.rows * group;
-  return queries <= few ? 0 : (queries + Queries - 1) / Queries * key_heads;
+  const uint32_t queries = q.rows * group;  // launch_attention_pages
+  return queries <= few ? 0 : (uint64_t)((queries + Queries - 1) / Queries) * key_heads;
 }
 
 // Shared: the rows of the whole batch over the keys below shared_rows, as parts for
@@ -75,7 +76,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   __shared__ __attribute__((aligned(1024))) uint8_t lds_v0[kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t lds_k1[kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t lds_v1[kTile];
-  __shared__ uint32_t arrived;
 
   const uint32_t lane = threadIdx.x % kWave, r16 = lane % 16, g4 = lane / 16;
   const uint32_t wave = uniform(threadIdx.x / kWave);
@@ -84,16 +84,18 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
 
   // ---- this workgroup's block: sequence s, key head, queries from query0 on ----
   uint32_t s = 0, key_head;
-  uint64_t query0;
+  uint32_t query0;
   BatchSequence q{0, a.rows, 0, 0};  // Shared: all rows
-  uint64_t queries;                   // of the sequence
+  uint32_t queries;                   // of the sequence
   uint64_t block;                     // in the line of all blocks
   uint32_t part, splits = split.parts;
   {
     auto blocks_in = [&](uint32_t x) __attribute__((always_inline)) {
       return blocks_of<kQueries>(sequence_at(b, x, a.rows), group, a.key_heads, few);
     };
-    const uint64_t total = Shared ? blocks_of<kQueries>(q, group, a.key_heads, 0) : count_units(b, blocks_in);
+    UnitLine line{0, blocks_of<kQueries>(q, group, a.key_heads, 0)};
+    if (!Shared) line = count_units(b, blocks_in);
+    const uint64_t total = line.total;
     if (total == 0) return;
     // Parts of the keys where the blocks are fewer than half of the workgroups that
     // the chip holds at once.
@@ -103,22 +105,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     }
     const uint64_t items = total * splits, per_xcd = (items + 7) / 8;
     const uint64_t item = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
-    block = item / splits;
-    part = (uint32_t)(item % splits);
+    block = quotient(item, splits);
+    part = (uint32_t)(item - block * splits);
     // Offsets that decrease can make more blocks than the host expects (and has
     // counters for); what lies past the grid is not computed.
     if (blockIdx.x / 8 >= per_xcd || item >= items || item >= gridDim.x) return;
     uint64_t within = block;
     if (!Shared) {
-      const UnitPlace place = find_unit(b, block, blocks_in);
+      const UnitPlace place = find_unit(b, line, block, blocks_in);
       s = place.sequence;
       within -= place.first;
       q = uniform(sequence_at(b, s, a.rows));
     }
-    queries = (uint64_t)q.rows * group;
-    const uint64_t per_head = (queries + kQueries - 1) / kQueries;
-    key_head = (uint32_t)(within / per_head);
-    query0 = (per_head - 1 - within % per_head) * kQueries;  // the longest first
+    queries = q.rows * group;
+    const uint32_t per_head = (queries + kQueries - 1) / kQueries;
+    key_head = (uint32_t)within / per_head;
+    query0 = (per_head - 1 - (uint32_t)within % per_head) * kQueries;  // the longest first
   }
 
   // ---- the wave's queries ----
@@ -127,13 +129,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   half8_t qf[QT][kKS];
   uint32_t limit[QT];         // keys that this lane's query may read
   uint32_t least = 0xffffffffu;
-  const uint64_t wave0 = query0 + wave * kQPW;
+  const uint32_t wave0 = query0 + wave * kQPW;
 #pragma unroll
   for (uint32_t qt = 0; qt < QT; ++qt) {
-    uint64_t m = wave0 + 16 * qt + r16;
+    uint32_t m = wave0 + 16 * qt + r16;
     const bool real = m < queries;
     m = real ? m : queries - 1;
-    const uint32_t row = q.first + (uint32_t)(m / group), head = (uint32_t)(m % group);
+    const uint32_t row = q.first + m / group, head = m % group;
     const half_t* from = (const half_t*)a.query + (uint64_t)row * a.query_row_stride +
                          (uint64_t)(key_head * group + head) * a.width;
     BatchSequence mine = q;
@@ -174,14 +176,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     const uint64_t reach = (uint64_t)b.table_columns * b.page_rows;
     key_end = b.shared_rows < reach ? b.shared_rows : (uint32_t)reach;
   } else {
-    const uint64_t last = query0 + kQueries < queries ? query0 + kQueries - 1 : queries - 1;
-    const uint32_t row = q.first + (uint32_t)(last / group);
+    const uint32_t last = query0 + kQueries < queries ? query0 + kQueries - 1 : queries - 1;
+    const uint32_t row = q.first + last / group;
     key_end = readable_keys(q, row_position(q.length, (int)(q.first + q.rows), row), a.causal);
   }
   // This part's: every part has a block of keys, but for the first of none at all.
   const uint32_t all_blocks = (key_end + kKeys - 1) / kKeys;
   uint32_t per_part = (all_blocks + splits - 1) / splits;
-  if (!Shared && splits > 1 && per_part < 4) per_part = 4;  // a part's start and merge cost about as much
+  if (!Shared && splits > 1 && per_part < 4) per_part = 4;  // a part's start and its join cost about as much
   if (per_part == 0) per_part = 1;
   uint32_t parts = (all_blocks + per_part - 1) / per_part;
   if (parts == 0) parts = 1;
@@ -427,15 +429,21 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   }
 
   // ---- results: o[dt][qt][e] = O^T[16 dt + 4 (l / 16) + e][query], unnormalised ----
-  auto output_row = [&](uint64_t m) __attribute__((always_inline)) {
-    return (uint64_t)(q.first + (uint32_t)(m / group)) * a.query_heads + key_head * group + (uint32_t)(m % group);
+  auto output_row = [&](uint32_t m) __attribute__((always_inline)) {
+    const uint32_t row = m / group;
+    return (uint64_t)(q.first + row) * a.query_heads + key_head * group + (m - row * group);
   };
   if (!Shared && parts == 1) {
+    if (split.parts > 1 && g4 == 0) {
+#pragma unroll
+      for (uint32_t qt = 0; qt < QT; ++qt)
+        if (wave0 + 16 * qt + r16 < queries) split.counts[output_row(wave0 + 16 * qt + r16)] = 1;
+    }
 #pragma unroll
     for (uint32_t qt = 0; qt < QT; ++qt) {
       const float l = sum_of_query(l_run[qt]);
       const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-      const uint64_t m = wave0 + 16 * qt + r16;
+      const uint32_t m = wave0 + 16 * qt + r16;
       if (m < queries) {
         half_t* to = (half_t*)a.out + output_row(m) * a.width;
 #pragma unroll
@@ -454,70 +462,64 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
 #pragma unroll
   for (uint32_t qt = 0; qt < QT; ++qt) {
     const float l = sum_of_query(l_run[qt]);
-    const uint64_t m = wave0 + 16 * qt + r16;
+    const uint32_t m = wave0 + 16 * qt + r16;
     if (m < queries) {
-      const uint64_t at = output_row(m) * split.parts + part;
+      const uint64_t row = output_row(m), at = row * split.parts + part;
       if (g4 == 0) {
-        store_device(split.sums + at * 2, m_run[qt]);
-        store_device(split.sums + at * 2 + 1, l);
+        split.sums[at * 2] = m_run[qt];
+        split.sums[at * 2 + 1] = l;
+        if (!Shared && part == 0) split.counts[row] = parts;
       }
 #pragma unroll
       for (uint32_t dt = 0; dt < kDT; ++dt) {
         const uint32_t d = dt * 16 + 4 * g4;
-        if (d < a.width) store_device4(split.rows + at * a.width + d, o[dt][qt]);
+        if (d < a.width) *reinterpret_cast<float4_t*>(split.rows + at * a.width + d) = o[dt][qt];
       }
     }
   }
-  if constexpr (!Shared) {
-    if (!arrive(split.counters + block, parts, &arrived)) return;
-    // Weight of each part of each query in LDS: one thread loads each pair, one folds each query.
-    float* weight = reinterpret_cast<float*>(lds_k0);  // [query][kMaxSplits]
-    float* part_sum = reinterpret_cast<float*>(lds_k1);
-    static_assert(kQueries * kMaxSplits * 4 <= kTile, "the weights fit a K stage");
-    const uint32_t rows = queries - query0 < kQueries ? (uint32_t)(queries - query0) : kQueries;
-    for (uint32_t i = threadIdx.x; i < rows * parts; i += kThreads) {
-      const uint32_t r = i / parts, z = i % parts;
-      const float* pair = split.sums + (output_row(query0 + r) * split.parts + z) * 2;
-      weight[r * kMaxSplits + z] = load_device(pair);
-      part_sum[r * kMaxSplits + z] = load_device(pair + 1);
-    }
-    __syncthreads();
-    if (threadIdx.x < rows) {
-      float* w = weight + threadIdx.x * kMaxSplits;
-      const float* l = part_sum + threadIdx.x * kMaxSplits;
-      float top = -INFINITY, sum = 0.0f;
-      for (uint32_t z = 0; z < parts; ++z) top = fmaxf(top, w[z]);
-      top = top == -INFINITY ? 0.0f : top;
-      for (uint32_t z = 0; z < parts; ++z) {
-        w[z] = __builtin_amdgcn_exp2f(w[z] - top);
-        sum += w[z] * l[z];
-      }
-      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-      for (uint32_t z = 0; z < parts; ++z) w[z] *= inverse;
-    }
-    __syncthreads();
-    const uint32_t quads = a.width / 4;
-    for (uint32_t i = threadIdx.x; i < rows * quads; i += kThreads) {
-      const uint32_t r = i / quads, d = i % quads * 4;
-      const uint64_t row = output_row(query0 + r);
-      const float* from = split.rows + row * split.parts * a.width + d;
-      const float* w = weight + r * kMaxSplits;
-      float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (uint32_t z0 = 0; z0 < parts; z0 += 8) {  // eight loads in flight
-        float4_t x[8];
+}
+
+// Joins the parts of the split blocks: a wave per row and query head.
+__global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs a, uint32_t few, SplitKeys split) {
+  const uint32_t row = blockIdx.x, lane = threadIdx.x % kWave;
+  const uint32_t head = blockIdx.y * kWaves + threadIdx.x / kWave;
+  const uint32_t s = find_sequence(a.batch, row);
+  if (s >= a.batch.sequences || head >= a.query_heads) return;
+  const BatchSequence q = sequence_at(a.batch, s, a.rows);
+  if (row < q.first || q.rows * (a.query_heads / a.key_heads) <= few) return;
+  const uint64_t at = (uint64_t)row * a.query_heads + head;
+  const uint32_t parts = split.counts[at];
+  if (parts < 2 || parts > split.parts) return;  // 1: its block has written the output
+  // Lane z holds part z's weight, exp2(m - max m) / sum.
+  const float* pair = split.sums + (at * split.parts + (lane < parts ? lane : 0)) * 2;
+  const float m = lane < parts ? pair[0] : -INFINITY, l = lane < parts ? pair[1] : 0.0f;
+  float top = m;
+  for (uint32_t o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+  const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+  const float sum = wave_sum(lane < parts ? f * l : 0.0f);
+  const float weight = sum == 0.0f ? 0.0f : f / sum;
+  const float* rows = split.rows + at * split.parts * a.width;
+  for (uint32_t d = lane * 4; d < ((a.width + 255) & ~255u); d += 4 * kWave) {
+    const uint32_t c = d < a.width ? d : 0;
+    float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t z0 = 0; z0 < parts; z0 += 8) {  // eight loads in flight
+      float4_t y[8];
 #pragma unroll
-        for (uint32_t u = 0; u < 8; ++u) {
-          const uint32_t z = z0 + u < parts ? z0 + u : parts - 1;
-          x[u] = load_device4(from + (uint64_t)z * a.width);
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < 8; ++u)
-          if (z0 + u < parts) acc += x[u] * w[z0 + u];
+      for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t z = z0 + j < parts ? z0 + j : parts - 1;
+        y[j] = *reinterpret_cast<const float4_t*>(rows + (uint64_t)z * a.width + c);
       }
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const float w = __shfl(weight, z0 + j, kWave);
+        if (z0 + j < parts) x += y[j] * w;
+      }
+    }
+    if (d < a.width) {
       half4_t h;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) h[x] = (half_t)acc[x];
-      *reinterpret_cast<half4_t*>((half_t*)a.out + row * a.width + d) = h;
+      for (int e = 0; e < 4; ++e) h[e] = (half_t)x[e];
+      *reinterpret_cast<half4_t*>((half_t*)a.out + at * a.width + d) = h;
     }
   }
 }
@@ -534,15 +536,18 @@ int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2,
   }
   blocks *= a.key_heads;
   SplitKeys split = given;
-  if (!Shared && a.workspace.data && a.workspace.counter_count >= kFullChip) {
-    const uint64_t row_bytes = (uint64_t)a.rows * a.query_heads * (a.width + 2) * sizeof(float);
-    uint64_t parts = a.workspace.bytes / row_bytes;
+  // Parts where the blocks surely leave half of the chip's workgroups idle; how many,
+  // the kernel decides by the blocks that there are.
+  if (!Shared && a.workspace.data && blocks < kFullChip) {
+    const uint64_t rows = (uint64_t)a.rows * a.query_heads;
+    uint64_t parts = a.workspace.bytes / sizeof(float) / rows;  // floats per row, then parts
+    parts = parts > 0 ? (parts - 1) / (a.width + 2) : 0;
     if (parts > kMaxSplits) parts = kMaxSplits;
     if (parts > 1) {
       split.parts = (uint32_t)parts;
       split.rows = (float*)a.workspace.data;
-      split.sums = split.rows + (uint64_t)a.rows * a.query_heads * parts * a.width;
-      split.counters = a.workspace.counters;
+      split.sums = split.rows + rows * parts * a.width;
+      split.counts = (uint32_t*)(split.sums + rows * parts * 2);
     }
   }
   // Split blocks make at most kFullChip workgroups (Shared: the given parts of each).
@@ -551,6 +556,11 @@ int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2,
   if (grid > 0xffffffull) return IPUS_ERROR_UNAVAILABLE;  // a grid dimension holds less than 2^32 threads
   hipLaunchKernelGGL((attention_blocks_kernel<D, DC, QT, Shared>), dim3((uint32_t)grid), dim3(kThreads), 0, stream, a,
                      scale_log2, few, split);
+  if (int e = hip_status(hipGetLastError())) return e;
+  if (Shared || split.parts <= 1) return 0;
+  // Fewer than kFullChip blocks hold fewer than 2^16 rows.
+  hipLaunchKernelGGL(join_parts_kernel, dim3(a.rows, (a.query_heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, a,
+                     few, split);
   return hip_status(hipGetLastError());
 }
 template <bool Shared>

@@ -88,6 +88,7 @@ struct DecodeSplit {
   uint32_t* counters;  // by the workgroup that holds a segment's first part
 };
 constexpr uint32_t kMaxParts = 128;       // of one segment
+constexpr uint32_t kWhole = 4;
 constexpr uint32_t kMostChunks = 2048;    // workgroups of a launch at most
 
 template <int D, int DC, int MT>
@@ -109,10 +110,10 @@ struct Units {
 };
 template <uint32_t Keys, uint32_t Queries>
 __device__ __forceinline__ Units units_of(const BatchSequence& q, uint32_t group, uint32_t key_heads, uint32_t first_key,
-                                          uint64_t few) {
+                                          uint32_t few) {
   Units u;
-  const uint64_t queries = (uint64_t)q.rows * group;
-  u.segments = queries <= few ? (queries + Queries - 1) / Queries * key_heads : 0;
+  const uint32_t queries = q.rows * group;  // launch_attention_pages
+  u.segments = queries <= few ? (uint64_t)((queries + Queries - 1) / Queries) * key_heads : 0;
   const uint32_t keys = q.keys > first_key ? q.keys - first_key : 0;
   u.tiles = keys == 0 ? 1 : (uint32_t)(((uint64_t)keys + Keys - 1) / Keys);
   return u;
@@ -120,7 +121,7 @@ __device__ __forceinline__ Units units_of(const BatchSequence& q, uint32_t group
 
 template <int D, int DC, int MT>
 __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_decode_kernel(
-    PagedAttentionArgs a, float scale_log2, uint32_t first_key, uint64_t few, uint32_t most_chunks, DecodeSplit split,
+    PagedAttentionArgs a, float scale_log2, uint32_t first_key, uint32_t few, uint32_t most_chunks, DecodeSplit split,
     SharedParts shared) {
   using C = Decode<D, DC, MT>;
   constexpr uint32_t kKeys = C::kKeys, kKT = C::kKT, kKS = C::kKS, kDT = C::kDT, kHalves = C::kHalves;
@@ -130,10 +131,10 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
   __shared__ __attribute__((aligned(1024))) uint8_t stage0[kWaves * kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t stage1[kWaves * kTile];
   __shared__ float wave_sums[kWaves][kQueries][2];
-  // Weights of a query's parts: the waves' and the shared keys'.  Where a segment
-  // of several workgroups is merged, its parts' and the shared keys', in stage 0.
+  // Weights of a query's parts and their sums: the waves' and the shared keys'.  Where a
+  // segment of several workgroups is merged, its parts' and the shared keys', in the stages.
   constexpr uint32_t kFewParts = kWaves + kMaxSharedParts, kManyParts = kMaxParts + kMaxSharedParts;
-  __shared__ float few_weights[kQueries * kFewParts];
+  __shared__ float few_weights[kQueries * kFewParts], few_sums[kQueries * kFewParts];
   static_assert(kQueries * kManyParts * 4 <= kWaves * kTile, "the weights of a merge fit a stage");
   __shared__ uint32_t arrived;
 
@@ -141,41 +142,39 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint32_t group = a.query_heads / a.key_heads;
   const PagedBatch& b = a.batch;
-  const bool may_split = split.rows != nullptr;
 
   // ---- this workgroup's chunk of the line of units ----
-  uint64_t segments = 0;
-  uint32_t longest = 1;
+  uint32_t longest = 1;  // segment of a sequence that this lane has seen
   auto units_in = [&](uint32_t s) __attribute__((always_inline)) {
     const Units u = units_of<kKeys, kQueries>(sequence_at(b, s, a.rows), group, a.key_heads, first_key, few);
-    return u.segments * u.tiles;
-  };
-  const uint64_t total = count_units(b, [&](uint32_t s) __attribute__((always_inline)) {
-    const Units u = units_of<kKeys, kQueries>(sequence_at(b, s, a.rows), group, a.key_heads, first_key, few);
-    segments += u.segments;
     if (u.segments > 0 && u.tiles > longest) longest = u.tiles;
     return u.segments * u.tiles;
-  });
+  };
+  const UnitLine line = count_units(b, units_in);
+  const uint64_t total = line.total;
   if (total == 0) return;
-  segments = uniform(from_lane(scan(segments), kWave - 1));
-  for (uint32_t o = 32; o > 0; o >>= 1) {
-    const uint32_t other = __shfl_xor(longest, o, kWave);
-    longest = other > longest ? other : longest;
-  }
-  longest = uniform(longest);
-  // At least a tile per wave where segments are that long, and enough chunks to fill the
-  // chip; from 8 tiles per wave on one chunk per resident workgroup, so that the scan, a
-  // segment's start and its merge are paid once.
-  uint64_t chunk = (total + most_chunks - 1) / most_chunks;
-  const uint64_t usual = total / segments < kWaves ? total / segments : kWaves;
-  if (chunk < usual) chunk = usual;
+  // Segments of up to kWhole tiles per wave stay whole (a merge costs as much as walking
+  // them): a workgroup takes those that begin in its chunk.  Longer ones are cut.
+  const bool may_split = split.rows != nullptr && __any(longest > kWhole * kWaves);
+  // At least two tiles per wave of a cut segment, and enough chunks to fill the chip; from 8
+  // tiles per wave on one chunk per resident workgroup, so that the scan, a segment's start
+  // and its merge are paid once.
+  uint64_t chunk = quotient(total + most_chunks - 1, most_chunks);
+  if (chunk < 2 * kWaves && may_split) chunk = 2 * kWaves;
   const uint64_t resident = (total + kFullChip - 1) / kFullChip;
   if (resident >= 8 * kWaves && chunk < resident) chunk = resident;
-  if (chunk < (longest + kMaxParts - 2) / (kMaxParts - 1)) chunk = (longest + kMaxParts - 2) / (kMaxParts - 1);
+  if (total > chunk * (kMaxParts - 2)) {  // else no segment has so many parts
+    for (uint32_t o = 32; o > 0; o >>= 1) {
+      const uint32_t other = __shfl_xor(longest, o, kWave);
+      longest = other > longest ? other : longest;
+    }
+    const uint32_t least = (uniform(longest) + kMaxParts - 2) / (kMaxParts - 1);
+    if (chunk < least) chunk = least;
+  }
   const uint64_t begin = blockIdx.x * chunk;
   if (begin >= total) return;
   const uint64_t end = begin + chunk < total ? begin + chunk : total;
-  const UnitPlace place = find_unit(b, begin, units_in);
+  const UnitPlace place = find_unit(b, line, begin, units_in);
   uint32_t s = place.sequence;
   uint64_t sequence_begin = place.first;  // first unit of sequence s
 
@@ -201,10 +200,11 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
       continue;
     }
     const uint64_t within = unit - sequence_begin;
-    const uint32_t tile_first = (uint32_t)(within % u.tiles);
-    const uint64_t segment = within / u.tiles, segment_begin = unit - tile_first, segment_end = segment_begin + u.tiles;
-    const uint32_t key_head = (uint32_t)(segment % a.key_heads);
-    const uint64_t query0 = segment / a.key_heads * kQueries;  // of the sequence's rows x group
+    const uint64_t segment = quotient(within, u.tiles);
+    const uint32_t tile_first = (uint32_t)(within - segment * u.tiles);
+    const uint64_t segment_begin = unit - tile_first, segment_end = segment_begin + u.tiles;
+    const uint32_t query_tile = (uint32_t)segment / a.key_heads, key_head = (uint32_t)segment - query_tile * a.key_heads;
+    const uint32_t query0 = query_tile * kQueries;  // of the sequence's rows x group
     if (!may_split && tile_first != 0) {  // begun, and finished, by the workgroup before
       unit = segment_end;
       continue;
@@ -214,15 +214,15 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
 
     // The wave's queries: fragment (mt, ks) holds columns 32 ks + 8 (l / 16) .. + 7 of
     // query 16 mt + l % 16; padding queries repeat the last one, with no key allowed.
-    const uint64_t queries = (uint64_t)q.rows * group - query0;  // left, at least 1
+    const uint32_t queries = q.rows * group - query0;  // left, at least 1
     half8_t qf[MT][kKS];
     uint32_t limit[MT];  // keys that this lane's query may read
 #pragma unroll
     for (uint32_t mt = 0; mt < MT; ++mt) {
       uint32_t m = 16 * mt + r16;
       const bool real = m < queries;
-      m = real ? m : (uint32_t)queries - 1;
-      const uint32_t row = q.first + (uint32_t)((query0 + m) / group), head = (uint32_t)((query0 + m) % group);
+      m = real ? m : queries - 1;
+      const uint32_t row = q.first + (query0 + m) / group, head = (query0 + m) % group;
       const half_t* from = (const half_t*)a.query + (uint64_t)row * a.query_row_stride +
                            (uint64_t)(key_head * group + head) * a.width;
       const int position = row_position(q.length, (int)(q.first + q.rows), row);
@@ -418,12 +418,12 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
         *reinterpret_cast<float4_t*>(mine + ((dt * 4 + g4) ^ (r16 & 7)) * 4) = o[dt][mt];
     }
     __syncthreads();
-    const uint32_t real = queries < kQueries ? (uint32_t)queries : kQueries;
+    const uint32_t real = queries < kQueries ? queries : kQueries;
     const uint32_t quads = a.width / 4;
     // (row, head) of query m, for the shared keys' parts and the output.
     auto output_row = [&](uint32_t m) __attribute__((always_inline)) {
-      const uint64_t x = query0 + m;
-      return (uint64_t)(q.first + (uint32_t)(x / group)) * a.query_heads + key_head * group + (uint32_t)(x % group);
+      const uint32_t row = (query0 + m) / group;
+      return (uint64_t)(q.first + row) * a.query_heads + key_head * group + (query0 + m - row * group);
     };
     auto wave_quad = [&](uint32_t w, uint32_t m, uint32_t c) __attribute__((always_inline)) {
       const float* from = reinterpret_cast<const float*>((m < 16 ? stage0 : stage1) + w * kTile) + (m % 16) * D;
@@ -435,37 +435,49 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
       for (int e = 0; e < 4; ++e) h[e] = (half_t)x[e];
       *reinterpret_cast<half4_t*>((half_t*)a.out + output_row(m) * a.width + c * 4) = h;
     };
-    // Weights of `parts` results and of the shared keys' parts of each query, of
-    // which `load` gives the (reference point, sum) pairs: exp2(m - max m) / sum.
-    auto weigh = [&](float* weights, uint32_t most, uint32_t parts, auto load) __attribute__((always_inline)) {
+    // Weights of `parts` results and of the shared keys' parts of each query,
+    // exp2(m - max m) / sum, of which `load` gives the (reference point, sum) pairs: a
+    // thread loads a pair, a wave folds a query.
+    auto weigh = [&](float* weights, float* sums, uint32_t most, uint32_t parts, auto load) __attribute__((always_inline)) {
       const uint32_t all = parts + shared.parts;
-      for (uint32_t m = tid; m < real; m += kThreads) {
+      for (uint32_t i = tid; i < real * all; i += kThreads) {
+        const uint32_t m = i / all, z = i - m * all;
+        const float* pair = shared.sums + (output_row(m) * shared.parts + (z - parts)) * 2;
+        weights[m * most + z] = z < parts ? load(z, m, 0) : pair[0];
+        sums[m * most + z] = z < parts ? load(z, m, 1) : pair[1];
+      }
+      __syncthreads();
+      for (uint32_t m = wave; m < real; m += kWaves) {
         float* w = weights + m * most;
-        const float* pairs = shared.sums + output_row(m) * shared.parts * 2;
         float top = -INFINITY, sum = 0.0f;
-        for (uint32_t z = 0; z < all; ++z) {
-          w[z] = z < parts ? load(z, m, 0) : pairs[2 * (z - parts)];
-          top = fmaxf(top, w[z]);
-        }
+        for (uint32_t z = lane; z < all; z += kWave) top = fmaxf(top, w[z]);
+        for (uint32_t o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
         top = top == -INFINITY ? 0.0f : top;
-        for (uint32_t z = 0; z < all; ++z) {
-          w[z] = __builtin_amdgcn_exp2f(w[z] - top);
-          sum += w[z] * (z < parts ? load(z, m, 1) : pairs[2 * (z - parts) + 1]);
-        }
+        for (uint32_t z = lane; z < all; z += kWave) sum += __builtin_amdgcn_exp2f(w[z] - top) * sums[m * most + z];
+        sum = wave_sum(sum);
         const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-        for (uint32_t z = 0; z < all; ++z) w[z] *= inverse;
+        for (uint32_t z = lane; z < all; z += kWave) w[z] = __builtin_amdgcn_exp2f(w[z] - top) * inverse;
       }
       __syncthreads();
     };
     auto shared_quads = [&](const float* w, uint32_t m, uint32_t c, float4_t x) __attribute__((always_inline)) {
       const float* from = shared.rows + output_row(m) * shared.parts * a.width + c * 4;
-      for (uint32_t z = 0; z < shared.parts; ++z)
-        x += *reinterpret_cast<const float4_t*>(from + (uint64_t)z * a.width) * w[z];
+      for (uint32_t z0 = 0; z0 < shared.parts; z0 += 8) {  // eight loads in flight
+        float4_t y[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+          const uint32_t z = z0 + j < shared.parts ? z0 + j : shared.parts - 1;
+          y[j] = *reinterpret_cast<const float4_t*>(from + (uint64_t)z * a.width);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+          if (z0 + j < shared.parts) x += y[j] * w[z0 + j];
+      }
       return x;
     };
 
     if (stop - unit == u.tiles) {  // the whole segment
-      weigh(few_weights, kFewParts, kWaves, [&](uint32_t z, uint32_t m, uint32_t which) { return wave_sums[z][m][which]; });
+      weigh(few_weights, few_sums, kFewParts, kWaves, [&](uint32_t z, uint32_t m, uint32_t which) { return wave_sums[z][m][which]; });
       for (uint32_t i = tid; i < real * quads; i += kThreads) {
         const uint32_t m = i / quads, c = i % quads;
         float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -476,7 +488,7 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
     } else {
       // This part: slot 2 w of workgroup w for the segment it began in (or
       // before), 2 w + 1 for one begun later in its chunk.
-      const uint64_t first_part = segment_begin / chunk, last_part = (segment_end - 1) / chunk;
+      const uint64_t first_part = quotient(segment_begin, chunk), last_part = quotient(segment_end - 1, chunk);
       const uint32_t parts = (uint32_t)(last_part - first_part) + 1;
       auto slot_of = [&](uint64_t w) { return 2 * w + (segment_begin > w * chunk ? 1 : 0); };
       const uint64_t slot = slot_of(blockIdx.x);
@@ -504,7 +516,7 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
       }
       if (arrive(split.counters + first_part, parts, &arrived)) {
         float* weights = reinterpret_cast<float*>(stage0);
-        weigh(weights, kManyParts, parts, [&](uint32_t z, uint32_t m, uint32_t which) {
+        weigh(weights, reinterpret_cast<float*>(stage1), kManyParts, parts, [&](uint32_t z, uint32_t m, uint32_t which) {
           return load_device(split.sums + (slot_of(first_part + z) * kQueries + m) * 2 + which);
         });
         for (uint32_t i = tid; i < real * quads; i += kThreads) {
@@ -546,7 +558,7 @@ int launch_general(hipStream_t stream, const PagedAttentionArgs& a, float scale_
 // One launch over the sequences of at most `few` queries, keys from first_key on.
 struct DecodeLaunch {
   uint32_t first_key;
-  uint64_t few;
+  uint32_t few;
   SharedParts shared;
 };
 template <int D, int DC, int MT>
@@ -588,14 +600,18 @@ int launch_decode(hipStream_t stream, const PagedAttentionArgs& a, float scale_l
 
 // Queries of a key head (rows x query heads) up to which a sequence is the decode kernel's.
 constexpr uint32_t kFewQueries = 32;
+constexpr uint32_t kFewBeside = 16;  // beside sequences of more
 
 // The shared keys in a launch of their own: their parts in the workspace's lower
 // end, what is left to the launch that joins them.
 bool plan_shared(const PagedAttentionArgs& a, SharedParts* parts, Workspace* rest) {
   if (a.batch.shared_rows == 0 || a.batch.sequences < 2 || !a.workspace.data) return false;
   const uint64_t row_floats = (uint64_t)a.rows * a.query_heads * (a.width + 2);
-  // At least 4 MiB stay for the parts of the keys behind the shared ones.
-  const uint64_t room = a.workspace.bytes > (4u << 20) ? (a.workspace.bytes - (4u << 20)) / sizeof(float) : 0;
+  // What stays for the keys behind the shared ones: two slots of a chunk per resident workgroup.
+  const uint64_t queries = (uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16 && a.width <= 128 ? 32 : 16;
+  const uint64_t width = a.width > 128 ? 256 : a.width > 64 ? 128 : 64;
+  const uint64_t rest_bytes = 2 * kFullChip * queries * (width + 2) * sizeof(float);
+  const uint64_t room = a.workspace.bytes > rest_bytes ? (a.workspace.bytes - rest_bytes) / sizeof(float) : 0;
   const uint64_t most = room / row_floats < kMaxSharedParts ? room / row_floats : kMaxSharedParts;
   parts->parts = most == 0 ? 0 : shared_part_count(a, (uint32_t)most);
   if (parts->parts == 0) return false;
@@ -617,9 +633,12 @@ int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a) {
   const float scale_log2 = a.scale * kLog2e;
   const bool vectors = a.width % 8 == 0 && a.query_row_stride % 8 == 0 &&
                        ((uintptr_t)a.query | (uintptr_t)a.cache) % 16 == 0 && (uintptr_t)a.out % 8 == 0;
-  // A page's bytes fit 32 bits, for the tile loads' addresses.
-  if (!vectors || a.width > 256 || a.batch.page_elements * 2 > 0xffffffffull) return launch_general(stream, a, scale_log2);
+  // A page's bytes fit 32 bits, for the tile loads' addresses, and the batch's queries.
+  if (!vectors || a.width > 256 || a.batch.page_elements * 2 > 0xffffffffull ||
+      (uint64_t)a.rows * (a.query_heads / a.key_heads) > 0x7fffffffull)
+    return launch_general(stream, a, scale_log2);
   const uint64_t queries = (uint64_t)a.max_rows * (a.query_heads / a.key_heads);
+  const DecodeLaunch unshared{0, ~0u, {nullptr, nullptr, 0}};
   if (queries <= kFewQueries) {
     SharedParts parts;
     Workspace rest;
@@ -627,15 +646,17 @@ int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a) {
       if (int e = launch_shared_parts(stream, a, scale_log2, parts)) return e;
       PagedAttentionArgs behind = a;
       behind.workspace = rest;
-      return launch_decode(stream, behind, scale_log2, {a.batch.shared_rows, ~0ull, parts});
+      return launch_decode(stream, behind, scale_log2, {a.batch.shared_rows, ~0u, parts});
     }
-    return launch_decode(stream, a, scale_log2, {0, ~0ull, {nullptr, nullptr, 0}});
+    return launch_decode(stream, a, scale_log2, unshared);
   }
   // Sequences of many rows, and those of few beside them, of which there are none
   // where every sequence has max_rows.
-  const bool mixed = (uint64_t)a.batch.sequences * a.max_rows != a.rows;
-  if (int e = launch_attention_blocks(stream, a, scale_log2, mixed ? kFewQueries : 0)) return e;
-  return mixed ? launch_decode(stream, a, scale_log2, {0, kFewQueries, {nullptr, nullptr, 0}}) : 0;
+  if ((uint64_t)a.batch.sequences * a.max_rows == a.rows) return launch_attention_blocks(stream, a, scale_log2, 0);
+  if (int e = launch_attention_blocks(stream, a, scale_log2, kFewBeside)) return e;
+  PagedAttentionArgs beside = a;
+  beside.max_rows = 1;  // one tile of queries
+  return launch_decode(stream, beside, scale_log2, {0, kFewBeside, {nullptr, nullptr, 0}});
 }
 
 }  // namespace ipus
