@@ -40,8 +40,8 @@ struct Workspace;
 // after the other, whichever threads enqueue them, so they can share it.
 // Empty where the allocation failed, and while a caller records the stream
 // into a graph of its own (which it may launch on other streams, several at
-// once): the unsplit kernels run then.
-Workspace context_workspace(const ipus_context* ctx);
+// once): the unsplit kernels run then.  paged: all of it, for the paged attention.
+Workspace context_workspace(const ipus_context* ctx, bool paged = false);
 // The context's stream is being recorded into a graph (or cannot tell).
 bool stream_recorded(const ipus_context* ctx);
 

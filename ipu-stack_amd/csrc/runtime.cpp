@@ -48,8 +48,11 @@ int use_device(const ipus_context* ctx) {
 }
 
 // Partial results of one launch at most (a launch that would need more runs
-// unsplit), and a counter per group of workgroups that merges.
+// unsplit), and a counter per group of workgroups that merges.  Paged attention
+// may use all of it: rows over a shared prefix in 16 parts (128 sequences x 32 heads x
+// 128 columns: 34 MB) beside the parts of the keys behind it.
 constexpr size_t kWorkspaceBytes = 32u << 20;
+constexpr size_t kPagedWorkspaceBytes = 96u << 20;
 constexpr uint32_t kWorkspaceCounters = 16384;
 
 bool stream_recorded(const ipus_context* ctx) {
@@ -57,12 +60,12 @@ bool stream_recorded(const ipus_context* ctx) {
   return hipStreamIsCapturing(ctx->stream, &status) != hipSuccess || status != hipStreamCaptureStatusNone;
 }
 
-Workspace context_workspace(const ipus_context* ctx) {
+Workspace context_workspace(const ipus_context* ctx, bool paged) {
   Workspace w;
   if (!ctx->workspace) return w;
   if (!ctx->capturing_session.load(std::memory_order_relaxed) && stream_recorded(ctx)) return w;
   w.data = ctx->workspace;
-  w.bytes = kWorkspaceBytes;
+  w.bytes = paged ? kPagedWorkspaceBytes : kWorkspaceBytes;
   w.counters = ctx->workspace_counters;
   w.counter_count = kWorkspaceCounters;
   return w;
@@ -140,8 +143,8 @@ extern "C" int ipus_context_create(int device, ipus_context** out) {
   // The kernels' workspace, its counters at 0.  Without it (no memory left)
   // every launch still runs, unsplit.
   void* ws = nullptr;
-  if (hipMalloc(&ws, kWorkspaceBytes + kWorkspaceCounters * sizeof(uint32_t)) == hipSuccess) {
-    uint32_t* counters = (uint32_t*)((uint8_t*)ws + kWorkspaceBytes);
+  if (hipMalloc(&ws, kPagedWorkspaceBytes + kWorkspaceCounters * sizeof(uint32_t)) == hipSuccess) {
+    uint32_t* counters = (uint32_t*)((uint8_t*)ws + kPagedWorkspaceBytes);
     e = hipMemsetAsync(counters, 0, kWorkspaceCounters * sizeof(uint32_t), ctx->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     if (e == hipSuccess) {
@@ -612,7 +615,7 @@ int run_attention_pages(ipus_context* c, void* o, const void* const* i, const ui
   a.query_row_stride = s[6];
   a.causal = s[10] != 0;
   a.scale = s[11] == 0 ? 1.0f / std::sqrt((float)s[5]) : bits_to_float(s[11]);
-  a.workspace = context_workspace(c);
+  a.workspace = context_workspace(c, true);
   return launch_attention_pages(c->stream, a);
 }
 
