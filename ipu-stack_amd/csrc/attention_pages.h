@@ -52,14 +52,6 @@ __device__ __forceinline__ float sum_of_query(float x) {
   return x + __shfl_xor(x, 32, kWave);
 }
 
-__device__ __forceinline__ uint64_t shuffle_up(uint64_t x, uint32_t by) {
-  const uint32_t lo = __shfl_up((uint32_t)x, by, kWave), hi = __shfl_up((uint32_t)(x >> 32), by, kWave);
-  return lo | (uint64_t)hi << 32;
-}
-__device__ __forceinline__ uint64_t from_lane(uint64_t x, uint32_t lane) {
-  const uint32_t lo = __shfl((uint32_t)x, lane, kWave), hi = __shfl((uint32_t)(x >> 32), lane, kWave);
-  return lo | (uint64_t)hi << 32;
-}
 // Values that all lanes hold alike, into scalar registers.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ uint64_t uniform(uint64_t x) {
@@ -68,13 +60,43 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x) {
 __device__ __forceinline__ BatchSequence uniform(BatchSequence q) {
   return {uniform(q.first), uniform(q.rows), uniform(q.keys), (int)uniform((uint32_t)q.length)};
 }
-// Sum over the lanes up to this one.
+__device__ __forceinline__ uint64_t from_lane(uint64_t x, uint32_t lane) {  // lane: alike in all lanes
+  return (uint32_t)__builtin_amdgcn_readlane((uint32_t)x, lane) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(x >> 32), lane) << 32;
+}
+// x of the lane that the DPP control names, 0 where there is none.
+template <int Control, int RowMask>
+__device__ __forceinline__ uint32_t neighbour(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, Control, RowMask, 0xf, false);
+}
+template <int Control, int RowMask>
+__device__ __forceinline__ uint64_t neighbour(uint64_t x) {
+  return neighbour<Control, RowMask>((uint32_t)x) | (uint64_t)neighbour<Control, RowMask>((uint32_t)(x >> 32)) << 32;
+}
+// Sum over the lanes up to this one, and the largest of all lanes: four steps inside rows
+// of 16 lanes (row_shr), then the rows before (row_bcast:15 and :31).
 __device__ __forceinline__ uint64_t scan(uint64_t x) {
-  for (uint32_t o = 1; o < (uint32_t)kWave; o *= 2) {
-    const uint64_t y = shuffle_up(x, o);
-    if (threadIdx.x % kWave >= o) x += y;
-  }
+  x += neighbour<0x111, 0xf>(x);
+  x += neighbour<0x112, 0xf>(x);
+  x += neighbour<0x114, 0xf>(x);
+  x += neighbour<0x118, 0xf>(x);
+  x += neighbour<0x142, 0xa>(x);
+  x += neighbour<0x143, 0xc>(x);
   return x;
+}
+template <int Control, int RowMask>
+__device__ __forceinline__ uint32_t larger(uint32_t x) {
+  const uint32_t y = neighbour<Control, RowMask>(x);
+  return x > y ? x : y;
+}
+__device__ __forceinline__ uint32_t largest(uint32_t x) {
+  x = larger<0x111, 0xf>(x);
+  x = larger<0x112, 0xf>(x);
+  x = larger<0x114, 0xf>(x);
+  x = larger<0x118, 0xf>(x);
+  x = larger<0x142, 0xa>(x);
+  x = larger<0x143, 0xc>(x);
+  return (uint32_t)__builtin_amdgcn_readlane(x, kWave - 1);
 }
 
 // Quotient of values that mostly fit 32 bits (a 64-bit division takes about 100
@@ -94,11 +116,11 @@ __device__ __forceinline__ UnitLine count_units(const PagedBatch& b, F units) {
   const uint32_t lane = threadIdx.x % kWave;
   UnitLine l;
   l.upto = scan(lane < b.sequences ? units(lane) : 0);
-  l.total = uniform(from_lane(l.upto, kWave - 1));
+  l.total = from_lane(l.upto, kWave - 1);
   if (b.sequences > (uint32_t)kWave) {
     uint64_t more = 0;
     for (uint32_t s = kWave + lane; s < b.sequences; s += kWave) more += units(s);
-    l.total += uniform(from_lane(scan(more), kWave - 1));
+    l.total += from_lane(scan(more), kWave - 1);
   }
   return l;
 }
@@ -112,7 +134,7 @@ __device__ __forceinline__ UnitPlace find_unit(const PagedBatch& b, const UnitLi
   UnitPlace p{0, 0};
   uint64_t upto = line.upto;
   while (true) {
-    const uint64_t all = uniform(from_lane(upto, kWave - 1));
+    const uint64_t all = from_lane(upto, kWave - 1);
     if (at < p.first + all) break;
     p.first += all;
     p.sequence += kWave;
@@ -122,7 +144,7 @@ __device__ __forceinline__ UnitPlace find_unit(const PagedBatch& b, const UnitLi
   const uint64_t past = __ballot(p.first + upto > at);
   const uint32_t holder = past ? (uint32_t)__builtin_ctzll(past) : 0;
   p.sequence += holder;
-  if (holder > 0) p.first += uniform(from_lane(upto, holder - 1));
+  if (holder > 0) p.first += from_lane(upto, holder - 1);
   return p;
 }
 

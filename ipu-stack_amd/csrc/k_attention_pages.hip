@@ -79,17 +79,55 @@ __global__ __launch_bounds__(kWave) void attention_pages_general_kernel(PagedAtt
 // the second product as the sum of two fp16 values (22 bits): the matrix pipes have time for it here,
 // and the result is off by little more than its own rounding.
 
-// Partial results of a launch: slots of a workgroup's first and last segment, each
-// 16 * MT rows of D fp32 and their (reference point, sum) pairs; without
-// memory every segment is one workgroup's.
+// Partial results of a launch: two slots per workgroup, each 16 * MT rows of D fp32
+// and their (reference point, sum) pairs; without memory every segment is one
+// workgroup's.
 struct DecodeSplit {
   float* rows;
   float* sums;
-  uint32_t* counters;  // by the workgroup that holds a segment's first part
+  uint32_t* counters;  // by a segment's first part
 };
 constexpr uint32_t kMaxParts = 128;       // of one segment
-constexpr uint32_t kWhole = 4;
-constexpr uint32_t kMostChunks = 2048;    // workgroups of a launch at most
+constexpr uint32_t kMostGroups = 2048;    // workgroups of a launch at most
+
+// How a launch's segments (a sequence's query tile and key head, with its key tiles) are
+// dealt to the workgroups.  A segment's start and end cost about as much as four tiles per
+// wave, joining parts of it as much again:
+//  - no segment of more than 16 tiles: all whole;
+//  - at least 32 tiles per resident workgroup: the tiles of all segments are one line, cut
+//    into an equal chunk for each, wherever the cuts fall;
+//  - in between: every segment in parts of its own, of at least 8 tiles, one per
+//    workgroup (cut at any place, a workgroup would pay two segments' starts for a few tiles:
+//    2 x 8 segments of 34 tiles 18.1 us, of 48 tiles, where the cuts coincide, 13.0).
+// The line's units are tiles (part_tiles = 0) or parts of at most part_tiles tiles.
+struct Shares {
+  uint32_t part_tiles;
+  uint64_t chunk;  // units per workgroup
+  uint64_t parts;  // units of the line, or a bound on them
+  __device__ __forceinline__ uint32_t units(uint32_t tiles) const {
+    return part_tiles == 0 ? tiles : part_tiles >= tiles ? 1 : (tiles + part_tiles - 1) / part_tiles;
+  }
+  __device__ __forceinline__ uint64_t total(uint64_t tiles, uint64_t segments) const {
+    return part_tiles == 0 ? tiles : parts;
+  }
+};
+__device__ __forceinline__ Shares share_out(uint64_t tiles, uint64_t segments, uint32_t longest, uint32_t groups,
+                                            bool may_split) {
+  constexpr uint32_t kWholeTiles = 16, kLeastTiles = 8, kChunkTiles = 32;
+  if (!may_split || longest <= kWholeTiles)
+    return {0xffffffffu, quotient(segments + groups - 1, groups), segments};
+  const uint32_t resident = groups < kFullChip ? groups : kFullChip;
+  const uint64_t each = quotient(tiles + resident - 1, resident);
+  if (each < kChunkTiles) {
+    uint32_t part = each < kLeastTiles ? kLeastTiles : (uint32_t)each;
+    const uint32_t least = (longest + kMaxParts - 1) / kMaxParts;
+    if (part < least) part = least;
+    const uint64_t parts = quotient(tiles, part) + segments;  // at most
+    if (parts <= groups) return {part, 1, parts};
+  }
+  const uint64_t least = (longest + kMaxParts - 2) / (kMaxParts - 1);
+  return {0, each < least ? least : each, 0};
+}
 
 template <int D, int DC, int MT>
 struct Decode {
@@ -121,7 +159,7 @@ __device__ __forceinline__ Units units_of(const BatchSequence& q, uint32_t group
 
 template <int D, int DC, int MT>
 __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_decode_kernel(
-    PagedAttentionArgs a, float scale_log2, uint32_t first_key, uint32_t few, uint32_t most_chunks, DecodeSplit split,
+    PagedAttentionArgs a, float scale_log2, uint32_t first_key, uint32_t few, DecodeSplit split,
     SharedParts shared) {
   using C = Decode<D, DC, MT>;
   constexpr uint32_t kKeys = C::kKeys, kKT = C::kKT, kKS = C::kKS, kDT = C::kDT, kHalves = C::kHalves;
@@ -143,40 +181,33 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
   const uint32_t group = a.query_heads / a.key_heads;
   const PagedBatch& b = a.batch;
 
-  // ---- this workgroup's chunk of the line of units ----
-  uint32_t longest = 1;  // segment of a sequence that this lane has seen
-  auto units_in = [&](uint32_t s) __attribute__((always_inline)) {
-    const Units u = units_of<kKeys, kQueries>(sequence_at(b, s, a.rows), group, a.key_heads, first_key, few);
-    if (u.segments > 0 && u.tiles > longest) longest = u.tiles;
-    return u.segments * u.tiles;
+  // ---- this workgroup's share of the batch ----
+  auto units_at = [&](uint32_t s) __attribute__((always_inline)) {
+    return units_of<kKeys, kQueries>(sequence_at(b, s, a.rows), group, a.key_heads, first_key, few);
   };
-  const UnitLine line = count_units(b, units_in);
-  const uint64_t total = line.total;
-  if (total == 0) return;
-  // Segments of up to kWhole tiles per wave stay whole (a merge costs as much as walking
-  // them): a workgroup takes those that begin in its chunk.  Longer ones are cut.
-  const bool may_split = split.rows != nullptr && __any(longest > kWhole * kWaves);
-  // At least two tiles per wave of a cut segment, and enough chunks to fill the chip; from 8
-  // tiles per wave on one chunk per resident workgroup, so that the scan, a segment's start
-  // and its merge are paid once.
-  uint64_t chunk = quotient(total + most_chunks - 1, most_chunks);
-  if (chunk < 2 * kWaves && may_split) chunk = 2 * kWaves;
-  const uint64_t resident = (total + kFullChip - 1) / kFullChip;
-  if (resident >= 8 * kWaves && chunk < resident) chunk = resident;
-  if (total > chunk * (kMaxParts - 2)) {  // else no segment has so many parts
-    for (uint32_t o = 32; o > 0; o >>= 1) {
-      const uint32_t other = __shfl_xor(longest, o, kWave);
-      longest = other > longest ? other : longest;
-    }
-    const uint32_t least = (uniform(longest) + kMaxParts - 2) / (kMaxParts - 1);
-    if (chunk < least) chunk = least;
+  const Units held = lane < b.sequences ? units_at(lane) : Units{0, 1};  // of the first 64 sequences
+  uint64_t tiles = held.segments * held.tiles, segments = held.segments;
+  uint32_t longest = held.segments > 0 ? held.tiles : 0;
+  for (uint32_t s = kWave + lane; s < b.sequences; s += kWave) {
+    const Units u = units_at(s);
+    tiles += u.segments * u.tiles;
+    segments += u.segments;
+    if (u.segments > 0 && u.tiles > longest) longest = u.tiles;
   }
-  const uint64_t begin = blockIdx.x * chunk;
-  if (begin >= total) return;
-  const uint64_t end = begin + chunk < total ? begin + chunk : total;
+  tiles = from_lane(scan(tiles), kWave - 1);
+  segments = from_lane(scan(segments), kWave - 1);
+  longest = largest(longest);
+  if (segments == 0) return;
+  const Shares shares = share_out(tiles, segments, longest, gridDim.x, split.rows != nullptr);
+  auto line_units = [&](const Units& u) __attribute__((always_inline)) { return u.segments * shares.units(u.tiles); };
+  auto units_in = [&](uint32_t s) __attribute__((always_inline)) { return line_units(units_at(s)); };
+  UnitLine line{scan(line_units(held)), 0};
+  const uint64_t begin = (uint64_t)blockIdx.x * shares.chunk;
+  if (begin >= shares.total(tiles, segments)) return;
   const UnitPlace place = find_unit(b, line, begin, units_in);
   uint32_t s = place.sequence;
   uint64_t sequence_begin = place.first;  // first unit of sequence s
+  uint64_t end = begin + shares.chunk;
 
   // Per-lane offsets of the tile accesses.
   const uint64_t head_bytes = (uint64_t)b.page_rows * a.width * 2;
@@ -191,26 +222,34 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
 
   uint64_t unit = begin;
   while (unit < end) {
+    if (s >= b.sequences) break;  // the line's end
     const BatchSequence q = uniform(sequence_at(b, s, a.rows));
     const Units u = units_of<kKeys, kQueries>(q, group, a.key_heads, first_key, few);
-    const uint64_t units = u.segments * u.tiles;
+    const uint32_t per_segment = shares.units(u.tiles);
+    const uint64_t units = u.segments * per_segment;
     if (unit >= sequence_begin + units) {  // also a sequence without rows
       sequence_begin += units;
       ++s;
       continue;
     }
     const uint64_t within = unit - sequence_begin;
-    const uint64_t segment = quotient(within, u.tiles);
-    const uint32_t tile_first = (uint32_t)(within - segment * u.tiles);
-    const uint64_t segment_begin = unit - tile_first, segment_end = segment_begin + u.tiles;
+    const uint64_t segment = quotient(within, per_segment);
+    const uint32_t unit_first = (uint32_t)(within - segment * per_segment);
+    const uint64_t segment_begin = unit - unit_first, segment_end = segment_begin + per_segment;
     const uint32_t query_tile = (uint32_t)segment / a.key_heads, key_head = (uint32_t)segment - query_tile * a.key_heads;
     const uint32_t query0 = query_tile * kQueries;  // of the sequence's rows x group
-    if (!may_split && tile_first != 0) {  // begun, and finished, by the workgroup before
-      unit = segment_end;
-      continue;
+    // Its key tiles: those of one part, or (cut into chunks) up to the chunk's end.
+    uint32_t tile_first = unit_first, tile_last;
+    uint64_t stop;
+    if (shares.part_tiles) {
+      const uint32_t each = (u.tiles + per_segment - 1) / per_segment;  // every part has a tile
+      stop = unit + 1;
+      tile_first = unit_first * each;
+      tile_last = u.tiles - tile_first < each ? u.tiles : tile_first + each;
+    } else {
+      stop = segment_end < end ? segment_end : end;
+      tile_last = tile_first + (uint32_t)(stop - unit);
     }
-    const uint64_t stop = may_split && segment_end > end ? end : segment_end;
-    const uint32_t tile_last = tile_first + (uint32_t)(stop - unit);  // one past
 
     // The wave's queries: fragment (mt, ks) holds columns 32 ks + 8 (l / 16) .. + 7 of
     // query 16 mt + l % 16; padding queries repeat the last one, with no key allowed.
@@ -476,7 +515,7 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
       return x;
     };
 
-    if (stop - unit == u.tiles) {  // the whole segment
+    if (tile_last - tile_first == u.tiles) {  // the whole segment
       weigh(few_weights, few_sums, kFewParts, kWaves, [&](uint32_t z, uint32_t m, uint32_t which) { return wave_sums[z][m][which]; });
       for (uint32_t i = tid; i < real * quads; i += kThreads) {
         const uint32_t m = i / quads, c = i % quads;
@@ -486,12 +525,14 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
         store(m, c, shared_quads(few_weights + m * kFewParts + kWaves, m, c, x));
       }
     } else {
-      // This part: slot 2 w of workgroup w for the segment it began in (or
-      // before), 2 w + 1 for one begun later in its chunk.
-      const uint64_t first_part = quotient(segment_begin, chunk), last_part = quotient(segment_end - 1, chunk);
+      // This part's slot: by its unit; cut into chunks, 2 w of workgroup w for the segment
+      // in which its chunk begins, 2 w + 1 for one that begins later in it.
+      const bool chunks = shares.part_tiles == 0;
+      const uint64_t first_part = chunks ? quotient(segment_begin, shares.chunk) : segment_begin;
+      const uint64_t last_part = chunks ? quotient(segment_end - 1, shares.chunk) : segment_end - 1;
       const uint32_t parts = (uint32_t)(last_part - first_part) + 1;
-      auto slot_of = [&](uint64_t w) { return 2 * w + (segment_begin > w * chunk ? 1 : 0); };
-      const uint64_t slot = slot_of(blockIdx.x);
+      auto slot_of = [&](uint64_t w) { return chunks ? 2 * w + (segment_begin > w * shares.chunk ? 1 : 0) : w; };
+      const uint64_t slot = slot_of(chunks ? blockIdx.x : unit);
       float* rows = split.rows + slot * kQueries * D;
       float* sums = split.sums + slot * kQueries * 2;
       for (uint32_t i = tid; i < real * quads; i += kThreads) {
@@ -563,23 +604,26 @@ struct DecodeLaunch {
 };
 template <int D, int DC, int MT>
 int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
-  constexpr uint64_t kSlotFloats = Decode<D, DC, MT>::kQueries * (D + 2);
+  constexpr uint64_t kQueries = Decode<D, DC, MT>::kQueries, kSlotBytes = kQueries * (D + 2) * sizeof(float);
+  // A workgroup per segment (at most a partial query tile more per sequence) and one more per
+  // resident one, for segments in parts.
+  const uint64_t queries = (uint64_t)a.rows * (a.query_heads / a.key_heads);
+  const uint64_t sequences = a.batch.sequences < a.rows ? a.batch.sequences : a.rows;
+  uint64_t groups = ((queries + kQueries - 1) / kQueries + sequences) * a.key_heads + kFullChip;
+  if (groups > kMostGroups) groups = kMostGroups;
   DecodeSplit split{nullptr, nullptr, nullptr};
-  uint64_t chunks = kMostChunks;
   if (a.workspace.data) {
-    const uint64_t fit = a.workspace.bytes / (2 * kSlotFloats * sizeof(float));
-    if (chunks > fit) chunks = fit;
-    if (chunks > a.workspace.counter_count) chunks = a.workspace.counter_count;
+    const uint64_t fit = a.workspace.bytes / (2 * kSlotBytes);
+    const uint64_t most = fit < a.workspace.counter_count ? fit : a.workspace.counter_count;
+    if (most >= kFullChip) {
+      if (groups > most) groups = most;
+      split.rows = (float*)a.workspace.data;
+      split.sums = split.rows + 2 * groups * kQueries * D;
+      split.counters = a.workspace.counters;
+    }
   }
-  if (a.workspace.data && chunks >= kWaves) {
-    split.rows = (float*)a.workspace.data;
-    split.sums = split.rows + 2 * chunks * Decode<D, DC, MT>::kQueries * D;
-    split.counters = a.workspace.counters;
-  } else {
-    chunks = kMostChunks;
-  }
-  hipLaunchKernelGGL((attention_pages_decode_kernel<D, DC, MT>), dim3((uint32_t)chunks), dim3(kThreads), 0, stream,
-                     a, scale_log2, l.first_key, l.few, (uint32_t)chunks, split, l.shared);
+  hipLaunchKernelGGL((attention_pages_decode_kernel<D, DC, MT>), dim3((uint32_t)groups), dim3(kThreads), 0, stream,
+                     a, scale_log2, l.first_key, l.few, split, l.shared);
   return hip_status(hipGetLastError());
 }
 template <int D, int DC>
@@ -607,7 +651,7 @@ constexpr uint32_t kFewBeside = 16;  // beside sequences of more
 bool plan_shared(const PagedAttentionArgs& a, SharedParts* parts, Workspace* rest) {
   if (a.batch.shared_rows == 0 || a.batch.sequences < 2 || !a.workspace.data) return false;
   const uint64_t row_floats = (uint64_t)a.rows * a.query_heads * (a.width + 2);
-  // What stays for the keys behind the shared ones: two slots of a chunk per resident workgroup.
+  // What stays for the keys behind the shared ones: two slots per resident workgroup.
   const uint64_t queries = (uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16 && a.width <= 128 ? 32 : 16;
   const uint64_t width = a.width > 128 ? 256 : a.width > 64 ? 128 : 64;
   const uint64_t rest_bytes = 2 * kFullChip * queries * (width + 2) * sizeof(float);
