@@ -479,50 +479,49 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   }
 }
 
-// Joins the parts of the split blocks: a wave per row and query head.
+// Joins the parts of the split blocks: a wave per row and query head.  What it may need is
+// loaded at once, before it is known whether the row is one of them, and of how many parts.
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs a, uint32_t few, SplitKeys split) {
   const uint32_t row = blockIdx.x, lane = threadIdx.x % kWave;
   const uint32_t head = blockIdx.y * kWaves + threadIdx.x / kWave;
-  const uint32_t s = find_sequence(a.batch, row);
-  if (s >= a.batch.sequences || head >= a.query_heads) return;
-  const BatchSequence q = sequence_at(a.batch, s, a.rows);
-  if (row < q.first || q.rows * (a.query_heads / a.key_heads) <= few) return;
+  if (head >= a.query_heads) return;
   const uint64_t at = (uint64_t)row * a.query_heads + head;
   const uint32_t parts = split.counts[at];
-  if (parts < 2 || parts > split.parts) return;  // 1: its block has written the output
   // Lane z holds part z's weight, exp2(m - max m) / sum.
-  const float* pair = split.sums + (at * split.parts + (lane < parts ? lane : 0)) * 2;
-  const float m = lane < parts ? pair[0] : -INFINITY, l = lane < parts ? pair[1] : 0.0f;
-  float top = m;
-  for (uint32_t o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
-  const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
-  const float sum = wave_sum(lane < parts ? f * l : 0.0f);
-  const float weight = sum == 0.0f ? 0.0f : f / sum;
+  const float* pair = split.sums + (at * split.parts + (lane < split.parts ? lane : 0)) * 2;
+  const float m0 = pair[0], l0 = pair[1];
   const float* rows = split.rows + at * split.parts * a.width;
-  for (uint32_t d = lane * 4; d < ((a.width + 255) & ~255u); d += 4 * kWave) {
-    const uint32_t c = d < a.width ? d : 0;
-    float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t z0 = 0; z0 < parts; z0 += 8) {  // eight loads in flight
-      float4_t y[8];
+  const uint32_t c = lane * 4 < a.width ? lane * 4 : 0;
+  float4_t y[kMaxSplits];
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        const uint32_t z = z0 + j < parts ? z0 + j : parts - 1;
-        y[j] = *reinterpret_cast<const float4_t*>(rows + (uint64_t)z * a.width + c);
-      }
+  for (uint32_t z = 0; z < kMaxSplits; ++z)
+    y[z] = *reinterpret_cast<const float4_t*>(rows + (uint64_t)(z < split.parts ? z : 0) * a.width + c);
+  const uint32_t s = find_sequence(a.batch, row);
+  if (s >= a.batch.sequences) return;
+  const BatchSequence q = sequence_at(a.batch, s, a.rows);
+  if (row < q.first || q.rows * (a.query_heads / a.key_heads) <= few) return;
+  if (parts < 2 || parts > split.parts) return;  // 1: its block has written the output
+  const float m = lane < parts ? m0 : -INFINITY;
+  float top = m;
+  for (uint32_t o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+  top = __shfl(top, 0, kWave);  // of the first 16 lanes
+  const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+  const float sum = wave_sum(lane < parts ? f * l0 : 0.0f);
+  const float weight = sum == 0.0f ? 0.0f : f / sum;
+  float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        const float w = __shfl(weight, z0 + j, kWave);
-        if (z0 + j < parts) x += y[j] * w;
-      }
-    }
-    if (d < a.width) {
-      half4_t h;
+  for (uint32_t z = 0; z < kMaxSplits; ++z) {
+    const float w = __shfl(weight, z, kWave);
+    if (z < parts) x += y[z] * w;
+  }
+  if (lane * 4 < a.width) {
+    half4_t h;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = (half_t)x[e];
-      *reinterpret_cast<half4_t*>((half_t*)a.out + at * a.width + d) = h;
-    }
+    for (int e = 0; e < 4; ++e) h[e] = (half_t)x[e];
+    *reinterpret_cast<half4_t*>((half_t*)a.out + at * a.width + lane * 4) = h;
   }
 }
+static_assert(kMaxSplits == 16, "join_parts_kernel folds the parts over 16 lanes");
 
 template <int D, int DC, int QT, bool Shared>
 int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t few, const SplitKeys& given) {

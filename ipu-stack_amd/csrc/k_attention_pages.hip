@@ -87,8 +87,9 @@ struct DecodeSplit {
   float* sums;
   uint32_t* counters;  // by a segment's first part
 };
-constexpr uint32_t kMaxParts = 128;       // of one segment
-constexpr uint32_t kMostGroups = 2048;    // workgroups of a launch at most
+constexpr uint32_t kMaxParts = 96;       // of one segment
+constexpr uint32_t kMostGroups = 2048;   // workgroups of a launch at most
+constexpr uint32_t kMostResident = 512;  // workgroups on the chip at most (Decode::kResident)
 
 // How a launch's segments (a sequence's query tile and key head, with its key tiles) are
 // dealt to the workgroups.  A segment's start and end cost about as much as four tiles per
@@ -112,11 +113,11 @@ struct Shares {
   }
 };
 __device__ __forceinline__ Shares share_out(uint64_t tiles, uint64_t segments, uint32_t longest, uint32_t groups,
-                                            bool may_split) {
+                                            uint32_t resident, bool may_split) {
   constexpr uint32_t kWholeTiles = 16, kLeastTiles = 8, kChunkTiles = 32;
   if (!may_split || longest <= kWholeTiles)
     return {0xffffffffu, quotient(segments + groups - 1, groups), segments};
-  const uint32_t resident = groups < kFullChip ? groups : kFullChip;
+  if (resident > groups) resident = groups;
   const uint64_t each = quotient(tiles + resident - 1, resident);
   if (each < kChunkTiles) {
     uint32_t part = each < kLeastTiles ? kLeastTiles : (uint32_t)each;
@@ -129,15 +130,27 @@ __device__ __forceinline__ Shares share_out(uint64_t tiles, uint64_t segments, u
   return {0, each < least ? least : each, 0};
 }
 
-template <int D, int DC, int MT>
+// D: the width rounded up to 32, 64, 96, 128, 192 or 256 columns, which are computed and
+// are an LDS row.
+template <int D, int MT>
 struct Decode {
-  static constexpr uint32_t kKeys = D > 64 ? 32 : 64;  // keys per tile: 4 KiB of keys per wave at least
-  static constexpr uint32_t kTileBytes = kKeys * D * 2;
-  static constexpr uint32_t kKT = kKeys / 16, kKS = DC / 32, kDT = DC / 16, kHalves = kKeys / 32;
+  static constexpr uint32_t kKeys = D > 64 ? 32 : 64;  // per tile
+  static constexpr uint32_t kRowBytes = D * 2, kChunks = D / 8;
+  static constexpr uint32_t kTileBytes = kKeys * kRowBytes;
+  static constexpr uint32_t kKT = kKeys / 16, kKS = D / 32, kDT = D / 16, kHalves = kKeys / 32;
   static constexpr uint32_t kQueries = 16 * MT;
   static constexpr uint32_t kDma = kTileBytes / 1024;  // DMA instructions of a wave per tile
-  static constexpr uint32_t kDmaRows = 1024 / (D * 2);
+  // Workgroups per CU, by LDS (two stages of a tile per wave) and registers.
+  static constexpr uint32_t kPerCu = D > 128 ? 1 : 2;
+  static constexpr uint32_t kResident = 256 * kPerCu;
 };
+// 16-byte chunk c of a tile's row r lies at chunk c ^ swizzle(r): the 4 rows x 32 bytes that
+// 16 lanes of ds_read_b64_tr_b16 take then touch every bank once.  Rows of 64 and 192 bytes do
+// without; those of 384 bytes meet in pairs.
+template <int D>
+__device__ __forceinline__ uint32_t tile_swizzle(uint32_t row) {
+  return D == 64 || D == 128 || D == 256 ? value_swizzle<D>(row) : 0;
+}
 
 // Units of sequence q: query tiles x key heads, each of `tiles` key tiles (at
 // least one, so that rows without keys are written).  A sequence of more than `few`
@@ -157,13 +170,13 @@ __device__ __forceinline__ Units units_of(const BatchSequence& q, uint32_t group
   return u;
 }
 
-template <int D, int DC, int MT>
-__global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_decode_kernel(
+template <int D, int MT>
+__global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_pages_decode_kernel(
     PagedAttentionArgs a, float scale_log2, uint32_t first_key, uint32_t few, DecodeSplit split,
     SharedParts shared) {
-  using C = Decode<D, DC, MT>;
+  using C = Decode<D, MT>;
   constexpr uint32_t kKeys = C::kKeys, kKT = C::kKT, kKS = C::kKS, kDT = C::kDT, kHalves = C::kHalves;
-  constexpr uint32_t kQueries = C::kQueries, kTile = C::kTileBytes, kRowBytes = D * 2;
+  constexpr uint32_t kQueries = C::kQueries, kTile = C::kTileBytes, kRowBytes = C::kRowBytes;
   // Two stages, distinct objects, so that the compiler sees that the DMA into
   // one never meets the reads of the other; a wave's tile at wave * kTile.
   __shared__ __attribute__((aligned(1024))) uint8_t stage0[kWaves * kTile];
@@ -198,7 +211,7 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
   segments = from_lane(scan(segments), kWave - 1);
   longest = largest(longest);
   if (segments == 0) return;
-  const Shares shares = share_out(tiles, segments, longest, gridDim.x, split.rows != nullptr);
+  const Shares shares = share_out(tiles, segments, longest, gridDim.x, C::kResident, split.rows != nullptr);
   auto line_units = [&](const Units& u) __attribute__((always_inline)) { return u.segments * shares.units(u.tiles); };
   auto units_in = [&](uint32_t s) __attribute__((always_inline)) { return line_units(units_at(s)); };
   UnitLine line{scan(line_units(held)), 0};
@@ -215,7 +228,7 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
   uint32_t vbase;
   {
     const uint32_t row = 4 * g4 + r16 / 4, c1 = (r16 % 4) / 2;
-    vbase = row * kRowBytes + ((c1 ^ value_swizzle<D>(row)) << 4) + 8 * (r16 % 2);
+    vbase = row * kRowBytes + ((c1 ^ tile_swizzle<D>(row)) << 4) + 8 * (r16 % 2);
   }
   uint8_t* const my0 = stage0 + wave * kTile;
   uint8_t* const my1 = stage1 + wave * kTile;
@@ -329,8 +342,8 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
       const uint32_t lane_v = opaque(lane);
 #pragma unroll
       for (uint32_t i = 0; i < C::kDma; ++i) {
-        const uint32_t row = i * C::kDmaRows + lane_v / (D / 8);
-        const uint32_t column = ((lane_v % (D / 8)) ^ value_swizzle<D>(row)) * 8;
+        const uint32_t slot = i * kWave + lane_v, row = slot / C::kChunks;
+        const uint32_t column = ((slot % C::kChunks) ^ tile_swizzle<D>(row)) * 8;
         const int p = __shfl(page, row, kWave);
         dma16(pick((p >= 0) & (column < a.width), row_address(t, row, p) + value_bytes + column * 2, zeros), lv + i * 1024);
       }
@@ -392,7 +405,9 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
       for (uint32_t kk = 0; kk < kHalves; ++kk)
 #pragma unroll
         for (uint32_t dt = 0; dt < kDT; ++dt) {
-          const uint8_t* p = lv + (vbase_v ^ (dt << 5)) + 32 * kk * kRowBytes;
+          // The chunks of column tile dt: its number XORed in, or added where rows are not swizzled.
+          constexpr bool kSwizzled = D == 64 || D == 128 || D == 256;
+          const uint8_t* p = lv + (kSwizzled ? vbase_v ^ (dt << 5) : vbase_v + (dt << 5)) + 32 * kk * kRowBytes;
           const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS short4_t*)p);
           const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS short4_t*)(p + 16 * kRowBytes));
           const half8_t v = __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -443,7 +458,7 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : 2) void attention_pages_dec
     // Lane numbers made opaque, so that nothing of this is computed before the key loop.
     const uint32_t tid = opaque(threadIdx.x), r16 = tid % 16, g4 = tid % kWave / 16;
     // A wave's rows, fp32 [kQueries][D], fill its stage 0 and 1 (16 rows of each).
-    static_assert(16 * D * 4 <= kTile || D == 64, "a stage holds 16 rows");
+    static_assert(16 * D * 4 <= kTile, "a stage holds 16 rows");
 #pragma unroll
     for (uint32_t mt = 0; mt < MT; ++mt) {
       const float l = sum_of_query(l_run[mt]);
@@ -602,44 +617,45 @@ struct DecodeLaunch {
   uint32_t few;
   SharedParts shared;
 };
-template <int D, int DC, int MT>
+template <int D, int MT>
 int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
-  constexpr uint64_t kQueries = Decode<D, DC, MT>::kQueries, kSlotBytes = kQueries * (D + 2) * sizeof(float);
+  constexpr uint64_t kResident = Decode<D, MT>::kResident, kQueries = Decode<D, MT>::kQueries;
+  constexpr uint64_t kSlotBytes = kQueries * (D + 2) * sizeof(float);
   // A workgroup per segment (at most a partial query tile more per sequence) and one more per
   // resident one, for segments in parts.
   const uint64_t queries = (uint64_t)a.rows * (a.query_heads / a.key_heads);
   const uint64_t sequences = a.batch.sequences < a.rows ? a.batch.sequences : a.rows;
-  uint64_t groups = ((queries + kQueries - 1) / kQueries + sequences) * a.key_heads + kFullChip;
+  uint64_t groups = ((queries + kQueries - 1) / kQueries + sequences) * a.key_heads + kResident;
   if (groups > kMostGroups) groups = kMostGroups;
   DecodeSplit split{nullptr, nullptr, nullptr};
   if (a.workspace.data) {
     const uint64_t fit = a.workspace.bytes / (2 * kSlotBytes);
     const uint64_t most = fit < a.workspace.counter_count ? fit : a.workspace.counter_count;
-    if (most >= kFullChip) {
+    if (most >= kResident) {
       if (groups > most) groups = most;
       split.rows = (float*)a.workspace.data;
       split.sums = split.rows + 2 * groups * kQueries * D;
       split.counters = a.workspace.counters;
     }
   }
-  hipLaunchKernelGGL((attention_pages_decode_kernel<D, DC, MT>), dim3((uint32_t)groups), dim3(kThreads), 0, stream,
+  hipLaunchKernelGGL((attention_pages_decode_kernel<D, MT>), dim3((uint32_t)groups), dim3(kThreads), 0, stream,
                      a, scale_log2, l.first_key, l.few, split, l.shared);
   return hip_status(hipGetLastError());
 }
-template <int D, int DC>
+template <int D>
 int launch_decode_queries(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
   // Two tiles of queries at 256 columns do not fit the registers.
   if constexpr (D <= 128)
-    if ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16) return launch_decode_as<D, DC, 2>(stream, a, scale_log2, l);
-  return launch_decode_as<D, DC, 1>(stream, a, scale_log2, l);
+    if ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16) return launch_decode_as<D, 2>(stream, a, scale_log2, l);
+  return launch_decode_as<D, 1>(stream, a, scale_log2, l);
 }
 int launch_decode(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
-  if (a.width > 192) return launch_decode_queries<256, 256>(stream, a, scale_log2, l);
-  if (a.width > 128) return launch_decode_queries<256, 192>(stream, a, scale_log2, l);
-  if (a.width > 96) return launch_decode_queries<128, 128>(stream, a, scale_log2, l);
-  if (a.width > 64) return launch_decode_queries<128, 96>(stream, a, scale_log2, l);
-  if (a.width > 32) return launch_decode_queries<64, 64>(stream, a, scale_log2, l);
-  return launch_decode_queries<64, 32>(stream, a, scale_log2, l);
+  if (a.width > 192) return launch_decode_queries<256>(stream, a, scale_log2, l);
+  if (a.width > 128) return launch_decode_queries<192>(stream, a, scale_log2, l);
+  if (a.width > 96) return launch_decode_queries<128>(stream, a, scale_log2, l);
+  if (a.width > 64) return launch_decode_queries<96>(stream, a, scale_log2, l);
+  if (a.width > 32) return launch_decode_queries<64>(stream, a, scale_log2, l);
+  return launch_decode_queries<32>(stream, a, scale_log2, l);
 }
 
 // Queries of a key head (rows x query heads) up to which a sequence is the decode kernel's.
@@ -647,14 +663,23 @@ constexpr uint32_t kFewQueries = 32;
 constexpr uint32_t kFewBeside = 16;  // beside sequences of more
 
 // The shared keys in a launch of their own: their parts in the workspace's lower
-// end, what is left to the launch that joins them.
+// end, what is left to the launch that joins them.  That launch costs 8 us and more
+// (it writes the parts), reading the keys once per sequence what the caches give, about
+// 14 TB/s: worth it from some 160 MB saved.  Measured at width 128 with 64 keys of their own
+// each (us, shared / read per sequence): 8 sequences x 4096 keys x 8 heads (117 MB) 21.7 / 22.2,
+// 32 x 1024 x 16 (260 MB) 23.1 / 28.8, 8 x 4096 x 16 (235 MB) 25.6 / 50.4, 128 x 16384 x 8 (8.5 GB)
+// 70.9 / 598; not 2 x 16384 x 8 (67 MB) 35.8 / 26.1, 128 x 256 x 8 (134 MB) 34.0 / 29.8.
+constexpr uint64_t kSharedSaving = 160u << 20;
 bool plan_shared(const PagedAttentionArgs& a, SharedParts* parts, Workspace* rest) {
   if (a.batch.shared_rows == 0 || a.batch.sequences < 2 || !a.workspace.data) return false;
+  const uint64_t reach = (uint64_t)a.batch.table_columns * a.batch.page_rows;
+  const uint64_t keys = a.batch.shared_rows < reach ? a.batch.shared_rows : reach;
+  if ((a.batch.sequences - 1) * keys < kSharedSaving / ((uint64_t)a.key_heads * a.width * 4)) return false;
   const uint64_t row_floats = (uint64_t)a.rows * a.query_heads * (a.width + 2);
   // What stays for the keys behind the shared ones: two slots per resident workgroup.
   const uint64_t queries = (uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16 && a.width <= 128 ? 32 : 16;
-  const uint64_t width = a.width > 128 ? 256 : a.width > 64 ? 128 : 64;
-  const uint64_t rest_bytes = 2 * kFullChip * queries * (width + 2) * sizeof(float);
+  const uint64_t width = a.width > 128 ? 256 : a.width > 64 ? 128 : 64;  // at least the columns computed
+  const uint64_t rest_bytes = 2 * kMostResident * queries * (width + 2) * sizeof(float);
   const uint64_t room = a.workspace.bytes > rest_bytes ? (a.workspace.bytes - rest_bytes) / sizeof(float) : 0;
   const uint64_t most = room / row_floats < kMaxSharedParts ? room / row_floats : kMaxSharedParts;
   parts->parts = most == 0 ? 0 : shared_part_count(a, (uint32_t)most);

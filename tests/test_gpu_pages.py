@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 
 from decoder_forms import Batch, attention, norm_rotate, rotate, rounded
+from test_gpu_caller_capture import Recording
 
 pytestmark = pytest.mark.gpu
 
@@ -305,6 +306,166 @@ def test_attention_shared(ipus, ctx, rows, lengths, heads, key_heads, width, pag
     b.table[1:, :shared // page_rows] = -3
     for causal in (0, 1):
         check_attention(ipus, ctx, b, heads, key_heads, width, causal)
+
+
+ONCE = [
+    # As above, large enough that the shared keys get a launch of their own (160 MB saved).
+    (300, 1, 1003, 16, 4, 64, 16, 1000),
+    (180, 3, 700, 8, 8, 80, 32, 640),
+    (260, 1, 1500, 4, 1, 256, 64, 1455),
+    (100, 2, 3300, 12, 4, 128, 8, 3296),
+    (500, 1, 300, 64, 32, 32, 16, 288),
+]
+
+
+@pytest.mark.parametrize("sequences,rows,keys,heads,key_heads,width,page_rows,shared", ONCE)
+@pytest.mark.parametrize("causal", [0, 1])
+def test_attention_shared_read_once(ipus, ctx, sequences, rows, keys, heads, key_heads, width, page_rows,
+                                    shared, causal):
+    rng = np.random.default_rng(shared)
+    n = rng.integers(0, rows + 1, sequences)
+    k = rng.integers(shared - 20, keys + 40, sequences)  # some shorter than the prefix
+    k[0] = keys
+    n[0], k[3], n[3] = rows, 0, rows
+    b = Batch(rng, n, k, page_rows, 3, shared=shared)
+    b.table[1:, :shared // page_rows] = -3
+    if causal and width == 128:
+        b.table[0, 7] = b.pages  # shared keys without a page
+    check_attention(ipus, ctx, b, heads, key_heads, width, causal)
+
+
+def test_positions_past_32_bits(ipus, ctx):
+    """A cache and rows of more than 2^32 elements."""
+    heads, width, page_rows, pages = 8, 128, 256, 9000
+    page_bytes = 2 * heads * page_rows * width * 2
+    assert pages * page_bytes // 2 > 1 << 32
+    cache = ctx.alloc(pages * page_bytes)
+    ctx.memset(cache, 0)
+    b = Batch(np.random.default_rng(1), [300, 7], [300, 500], page_rows)
+    b.table[:] = np.where(b.table >= 0, b.table + 8990, -1)
+    b.pages = pages
+    keys, values = (halves(ipus, (b.rows, heads, width), t) for t in (2, 3))
+    f, _ = ipus.rotary_frequencies(width)
+    batch = upload_batch(ctx, b)
+    bufs = [ctx.upload(a) for a in (keys, values, f)] + batch
+    ctx.launch("ipu_stack_append_pages_f16", cache, bufs, append_scalars(b, heads, width, width, 0))
+    low, high = 8990, 9000
+    tail = ipus.DeviceBuffer(ctx, cache.ptr + low * page_bytes, (high - low) * page_bytes)
+    host = np.zeros((high - low, 2, heads, page_rows, width), np.float16)
+    got = tail.download(np.float16).reshape(host.shape)
+    shifted = Batch(np.random.default_rng(1), [300, 7], [300, 500], page_rows)
+    want, bound = append64(shifted, host, keys, values, f, 1.0, width, 0)
+    assert np.all(np.abs(got.astype(np.float64) - want) <= bound)
+    for rows, lengths in (([300, 7], [300, 500]), ([1, 1], [300, 500])):
+        a = Batch(np.random.default_rng(1), rows, lengths, page_rows)
+        view = Batch(np.random.default_rng(1), rows, lengths, page_rows)
+        a.table, a.pages = b.table, pages
+        q = halves(ipus, (a.rows, 16, width), 4)
+        ins = [ctx.upload(q), cache] + upload_batch(ctx, a)
+        out = ctx.alloc(q.nbytes)
+        ctx.launch("ipu_stack_attention_pages_f16", out, ins, attention_scalars(a, 16, heads, width, 1))
+        view.table = shifted.table
+        want, bound, _ = attention(view, q.astype(np.float64), got.astype(np.float64), heads, 1, width ** -0.5)
+        result = out.download(np.float16).reshape(q.shape).astype(np.float64)
+        assert np.all(np.abs(result - want) <= rounded(want, bound, np.float16))
+        for x in [ins[0], out] + ins[2:]:
+            x.free()
+    # Rotary rows 2^31 elements apart, in the same buffer: the third starts at 2^32.
+    stride, rows = 1 << 31, 3
+    x = halves(ipus, (rows, width), 5)
+    views = [ipus.DeviceBuffer(ctx, cache.ptr + r * stride * 2, width * 2) for r in range(rows)]
+    for r in range(rows):
+        ctx.write(views[r], x[r])
+    position = np.array([5, 6, 7], np.int32)
+    dp = ctx.upload(position)
+    ctx.launch("ipu_stack_rotary_f16", cache, [cache, dp, bufs[2]],
+               [rows, 1, width, width, 0, stride, width, stride, width, 0])
+    want, bound = rotate(x.astype(np.float64)[:, None], position, f, 1.0, width, False)
+    turned = np.stack([v.download(np.float16) for v in views]).astype(np.float64)[:, None]
+    assert np.all(np.abs(turned - want) <= rounded(want, bound, np.float16))
+    for x in bufs + [cache, dp]:
+        x.free()
+
+
+def test_recorded_launches(ipus, ctx):
+    """A caller's graph of a decoder step, replayed on a stream of its own beside the
+    context's launches: what it records uses no memory of the context."""
+    query, heads, width, page_rows = 8, 2, 128, 16
+    rows, lengths = [1] * 5 + [40], [3000, 17, 900, 1, 333, 700]
+    b = Batch(np.random.default_rng(21), rows, lengths, page_rows, 1)
+    start = halves(ipus, (b.pages, 2, heads, page_rows, width), 1)
+    q, keys, values = (halves(ipus, (b.rows, h, width), t) for h, t in ((query, 2), (heads, 3), (heads, 4)))
+    f, _ = ipus.rotary_frequencies(width)
+    position = np.zeros(b.rows, np.int32)
+    for s in range(b.sequences()):
+        position[b.offsets[s]:b.offsets[s + 1]] = b.k[s] - b.n[s] + np.arange(b.n[s])
+    dq, dk, dv, df, dp = (ctx.upload(a) for a in (q, keys, values, f, position))
+    batch = upload_batch(ctx, b)
+    sets = [(ctx.upload(start), ctx.alloc(q.nbytes), ctx.upload(np.full(q.shape, 7.0, np.float16)))
+            for _ in range(2)]
+    pitch = query * width
+
+    def launch(cache, turned, out):
+        ctx.launch("ipu_stack_rotary_f16", turned, [dq, dp, df],
+                   [b.rows, query, width, width, 0, pitch, width, pitch, width, 0])
+        ctx.launch("ipu_stack_append_pages_f16", cache, [dk, dv, df] + batch,
+                   append_scalars(b, heads, width, width, 0))
+        ctx.launch("ipu_stack_attention_pages_f16", out, [turned, cache] + batch,
+                   attention_scalars(b, query, heads, width, 1))
+
+    def check(cache, turned, out):
+        got_cache = cache.download(np.float16).reshape(start.shape)
+        want, bound = append64(b, start, keys, values, f, 1.0, width, 0)
+        assert np.all(np.abs(got_cache.astype(np.float64) - want) <= bound)
+        got_q = turned.download(np.float16).reshape(q.shape)
+        want, bound, inside = attention(b, got_q.astype(np.float64), got_cache.astype(np.float64), heads, 1,
+                                        width ** -0.5)
+        got = out.download(np.float16).reshape(q.shape).astype(np.float64)
+        assert np.all(np.abs(got - want)[inside] <= rounded(want, bound, np.float16)[inside])
+        assert np.all(got[~inside] == 7.0)
+
+    recording = Recording(ipus, ctx)
+    with recording:
+        launch(*sets[0])
+    for _ in range(4):
+        for cache, turned, out in sets:
+            ctx.write(cache, start)
+            ctx.memset(turned, 0xFF)
+            ctx.write(out, np.full(q.shape, 7.0, np.float16))
+        ctx.sync()
+        recording.replay()
+        launch(*sets[1])
+        recording.replay()
+        ctx.sync()
+        recording.sync()
+        check(*sets[0])
+        check(*sets[1])
+    recording.close()
+    for x in [dq, dk, dv, df, dp] + batch + [y for group in sets for y in group]:
+        x.free()
+
+
+def test_two_contexts_at_once(ipus, ctx):
+    """Launches of two contexts on one device run side by side, each with its own
+    workspace."""
+    other = ipus.Context(0)
+    b = Batch(np.random.default_rng(31), [1] * 3 + [50], [2500, 1300, 800, 600], 16)
+    cache = halves(ipus, (b.pages, 2, 2, 16, 128), 1)
+    runs = []
+    for c, t in ((ctx, 2), (other, 3)):
+        q = halves(ipus, (b.rows, 8, 128), t)
+        ins = [c.upload(q), c.upload(cache)] + upload_batch(c, b)
+        runs.append((c, q, ins, c.alloc(q.nbytes)))
+    for _ in range(20):
+        for c, q, ins, out in runs:
+            c.launch("ipu_stack_attention_pages_f16", out, ins, attention_scalars(b, 8, 2, 128, 1))
+    for c, q, ins, out in runs:
+        want, bound, _ = attention(b, q.astype(np.float64), cache.astype(np.float64), 2, 1, 128 ** -0.5)
+        got = out.download(np.float16).reshape(q.shape).astype(np.float64)
+        assert np.all(np.abs(got - want) <= rounded(want, bound, np.float16))
+        for x in ins + [out]:
+            x.free()
+    other.close()
 
 
 def test_decoder_steps(ipus, ctx):
