@@ -479,8 +479,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   }
 }
 
-// Joins the parts of the split blocks: a wave per row and query head.  What it may need is
-// loaded at once, before it is known whether the row is one of them, and of how many parts.
+// Joins the parts of the split blocks: a wave per row and query head.  The first eight parts
+// are loaded before it is known whether the row is one of them, and of how many.
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs a, uint32_t few, SplitKeys split) {
   const uint32_t row = blockIdx.x, lane = threadIdx.x % kWave;
   const uint32_t head = blockIdx.y * kWaves + threadIdx.x / kWave;
@@ -494,13 +494,16 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
   const uint32_t c = lane * 4 < a.width ? lane * 4 : 0;
   float4_t y[kMaxSplits];
 #pragma unroll
-  for (uint32_t z = 0; z < kMaxSplits; ++z)
+  for (uint32_t z = 0; z < 8; ++z)
     y[z] = *reinterpret_cast<const float4_t*>(rows + (uint64_t)(z < split.parts ? z : 0) * a.width + c);
   const uint32_t s = find_sequence(a.batch, row);
   if (s >= a.batch.sequences) return;
   const BatchSequence q = sequence_at(a.batch, s, a.rows);
   if (row < q.first || q.rows * (a.query_heads / a.key_heads) <= few) return;
   if (parts < 2 || parts > split.parts) return;  // 1: its block has written the output
+#pragma unroll
+  for (uint32_t z = 8; z < kMaxSplits; ++z)
+    if (z < parts) y[z] = *reinterpret_cast<const float4_t*>(rows + (uint64_t)z * a.width + c);
   const float m = lane < parts ? m0 : -INFINITY;
   float top = m;
   for (uint32_t o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));

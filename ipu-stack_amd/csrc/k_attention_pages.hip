@@ -87,7 +87,7 @@ struct DecodeSplit {
   float* sums;
   uint32_t* counters;  // by a segment's first part
 };
-constexpr uint32_t kMaxParts = 96;       // of one segment
+constexpr uint32_t kMaxParts = 64;       // of one segment
 constexpr uint32_t kMostGroups = 2048;   // workgroups of a launch at most
 constexpr uint32_t kMostResident = 512;  // workgroups on the chip at most (Decode::kResident)
 
@@ -99,7 +99,9 @@ constexpr uint32_t kMostResident = 512;  // workgroups on the chip at most (Deco
 //    into an equal chunk for each, wherever the cuts fall;
 //  - in between: every segment in parts of its own, of at least 8 tiles, one per
 //    workgroup (cut at any place, a workgroup would pay two segments' starts for a few tiles:
-//    2 x 8 segments of 34 tiles 18.1 us, of 48 tiles, where the cuts coincide, 13.0).
+//    2 x 8 segments of 34 tiles 18.1 us, of 48 tiles, where the cuts coincide, 13.0), and
+//    about one per CU (two make twice the parts to join: 8 segments of 500 tiles 24.5 us
+//    against 21.6, 32 of 66 18.2 against 16.1).
 // The line's units are tiles (part_tiles = 0) or parts of at most part_tiles tiles.
 struct Shares {
   uint32_t part_tiles;
@@ -114,13 +116,14 @@ struct Shares {
 };
 __device__ __forceinline__ Shares share_out(uint64_t tiles, uint64_t segments, uint32_t longest, uint32_t groups,
                                             uint32_t resident, bool may_split) {
-  constexpr uint32_t kWholeTiles = 16, kLeastTiles = 8, kChunkTiles = 32;
+  constexpr uint32_t kWholeTiles = 16, kLeastTiles = 8, kChunkTiles = 32, kCus = 256;
   if (!may_split || longest <= kWholeTiles)
     return {0xffffffffu, quotient(segments + groups - 1, groups), segments};
   if (resident > groups) resident = groups;
   const uint64_t each = quotient(tiles + resident - 1, resident);
   if (each < kChunkTiles) {
-    uint32_t part = each < kLeastTiles ? kLeastTiles : (uint32_t)each;
+    uint32_t part = (uint32_t)((tiles + kCus - 1) / kCus);
+    if (part < kLeastTiles) part = kLeastTiles;
     const uint32_t least = (longest + kMaxParts - 1) / kMaxParts;
     if (part < least) part = least;
     const uint64_t parts = quotient(tiles, part) + segments;  // at most
