@@ -58,7 +58,7 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x) {
   return uniform((uint32_t)x) | (uint64_t)uniform((uint32_t)(x >> 32)) << 32;
 }
 __device__ __forceinline__ BatchSequence uniform(BatchSequence q) {
-  return {uniform(q.first), uniform(q.rows), uniform(q.keys), (int)uniform((uint32_t)q.length)};
+  return {uniform(q.first), uniform(q.rows), uniform(q.keys), (int)uniform((uint32_t)q.length), (int)uniform((uint32_t)q.end)};
 }
 __device__ __forceinline__ uint64_t from_lane(uint64_t x, uint32_t lane) {  // lane: alike in all lanes
   return (uint32_t)__builtin_amdgcn_readlane((uint32_t)x, lane) |

@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   // ---- this workgroup's block: sequence s, key head, queries from query0 on ----
   uint32_t s = 0, key_head;
   uint32_t query0;
-  BatchSequence q{0, a.rows, 0, 0};  // Shared: all rows
+  BatchSequence q{0, a.rows, 0, 0, 0};  // Shared: all rows
   uint32_t queries;                   // of the sequence
   uint64_t block;                     // in the line of all blocks
   uint32_t part, splits = split.parts;
@@ -150,11 +150,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
         left = past ? left - half - 1 : half;
       }
       inside = real && low < b.sequences;
-      mine = inside ? sequence_at(b, low, a.rows) : BatchSequence{0, 0, 0, 0};
+      mine = inside ? sequence_at(b, low, a.rows) : BatchSequence{};
       inside = inside && row >= mine.first && row - mine.first < mine.rows;
       mine.keys = mine.keys < b.shared_rows ? mine.keys : b.shared_rows;
     }
-    const int position = row_position(mine.length, (int)(mine.first + mine.rows), row);
+    const int position = row_position(mine.length, mine.end, row);
     limit[qt] = inside ? readable_keys(mine, position, a.causal) : 0;
     if (limit[qt] < least) least = limit[qt];
 #pragma unroll
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   } else {
     const uint32_t last = query0 + kQueries < queries ? query0 + kQueries - 1 : queries - 1;
     const uint32_t row = q.first + last / group;
-    key_end = readable_keys(q, row_position(q.length, (int)(q.first + q.rows), row), a.causal);
+    key_end = readable_keys(q, row_position(q.length, q.end, row), a.causal);
   }
   // This part's: every part has a block of keys, but for the first of none at all.
   const uint32_t all_blocks = (key_end + kKeys - 1) / kKeys;

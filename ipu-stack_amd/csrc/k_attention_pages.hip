@@ -280,7 +280,7 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
       const uint32_t row = q.first + (query0 + m) / group, head = (query0 + m) % group;
       const half_t* from = (const half_t*)a.query + (uint64_t)row * a.query_row_stride +
                            (uint64_t)(key_head * group + head) * a.width;
-      const int position = row_position(q.length, (int)(q.first + q.rows), row);
+      const int position = row_position(q.length, q.end, row);
       limit[mt] = real ? readable_keys(q, position, a.causal) : 0;
 #pragma unroll
       for (uint32_t ks = 0; ks < kKS; ++ks) {

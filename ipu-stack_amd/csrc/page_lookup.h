@@ -36,10 +36,10 @@ IPUS_HD int page_of(const PagedBatch& b, uint32_t sequence, uint32_t position) {
 
 // Rows and keys of a sequence: rows first .. first + rows - 1 of the batch's
 // row_count (offsets outside it are cut off), keys [0, keys) that its table reaches,
-// and its length as given.
+// and its length and the end of its rows as given.
 struct BatchSequence {
   uint32_t first, rows, keys;
-  int length;
+  int length, end;
 };
 IPUS_HD BatchSequence sequence_at(const PagedBatch& b, uint32_t s, uint32_t row_count) {
   const int64_t from = b.row_offsets[s], to = b.row_offsets[s + 1];
@@ -49,6 +49,7 @@ IPUS_HD BatchSequence sequence_at(const PagedBatch& b, uint32_t s, uint32_t row_
   q.first = (uint32_t)first;
   q.rows = last > first ? (uint32_t)(last - first) : 0;
   q.length = b.lengths[s];
+  q.end = (int)to;
   const uint64_t reach = (uint64_t)b.table_columns * b.page_rows;
   q.keys = q.length <= 0 ? 0 : (uint64_t)q.length < reach ? (uint32_t)q.length : (uint32_t)reach;
   return q;

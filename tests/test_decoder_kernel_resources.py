@@ -1,0 +1,55 @@
+"""Register, scratch, occupancy and LDS budgets of the decoder kernels, from the
+compiler's resource remarks (no GPU needed)."""
+from __future__ import annotations
+
+import os
+import re
+
+import pytest
+
+from test_kernel_resources import BUILD, matching, parse
+
+SOURCES = ("k_rotary", "k_attention_pages", "k_attention_blocks")
+
+
+@pytest.fixture(scope="module")
+def kernels():
+    out = {}
+    for s in SOURCES:
+        path = os.path.join(BUILD, f"{s}.resources")
+        if not os.path.exists(path):
+            pytest.skip("library not built by the package Makefile (no resource remarks)")
+        got = parse(open(path).read())
+        assert got, f"{s}.resources holds no kernel"
+        out.update(got)
+    return out
+
+
+def test_no_scratch_memory(kernels):
+    # Two tiles of queries at 128 columns spill values that live across the key loop (stored
+    # before it, reloaded where the waves' results are joined).
+    for name, f in kernels.items():
+        limit = 64 if "attention_pages_decode_kernelILi128ELi2E" in name else 0
+        assert int(f["ScratchSize [bytes/lane]"]) <= limit, (name, f)
+        assert f.get("Dynamic Stack", "False") == "False", name
+
+
+def test_decode_kernels_fit_two_workgroups_per_cu(kernels):
+    for name, f in matching(kernels, "attention_pages_decode_kernel").items():
+        columns = int(re.search(r"decode_kernelILi(\d+)E", name).group(1))
+        per_cu = 1 if columns > 128 else 2
+        assert int(f["Occupancy [waves/SIMD]"]) >= per_cu, (name, f)
+        assert per_cu * int(f["LDS Size [bytes/block]"]) <= 163840, (name, f)
+
+
+def test_block_kernels_fit_two_workgroups_per_cu(kernels):
+    for name, f in matching(kernels, "attention_blocks_kernel").items():
+        assert int(f["Occupancy [waves/SIMD]"]) >= 2, (name, f)
+        assert 2 * int(f["LDS Size [bytes/block]"]) <= 163840, (name, f)
+
+
+def test_rotary_kernels_hide_their_loads(kernels):
+    for fragment in ("rotary_kernel", "append_kernel"):
+        for name, f in matching(kernels, fragment).items():
+            assert int(f["Occupancy [waves/SIMD]"]) >= 5, (name, f)
+            assert int(f["AGPRs"]) == 0 and int(f["VGPRs Spill"]) == 0, (name, f)

@@ -41,7 +41,9 @@ int main() {
   b.pages = 10;
   // Rows: offsets that decrease or pass the rows are cut off, keys end with the table.
   BatchSequence q = sequence_at(b, 0, 8);
-  CHECK(q.first == 0 && q.rows == 5 && q.keys == 7 && q.length == 7);
+  CHECK(q.first == 0 && q.rows == 5 && q.keys == 7 && q.length == 7 && q.end == 5);
+  q = sequence_at(b, 0, 3);                   // fewer rows than the offsets say: the first three
+  CHECK(q.first == 0 && q.rows == 3 && q.end == 5 && row_position(q.length, q.end, 2) == 4);
   q = sequence_at(b, 1, 8);
   CHECK(q.rows == 0 && q.first <= 8 && q.keys == 64);
   offsets = {kLow, kHigh, kHigh};
@@ -55,7 +57,7 @@ int main() {
   // Positions: the last row at length - 1, none below 0 or past an int.
   CHECK(row_position(7, 5, 4) == 6 && row_position(7, 5, 0) == 2 && row_position(2, 5, 2) == -1);
   CHECK(row_position(2, 5, 3) == 0 && row_position(kLow, kHigh, 0) == -1 && row_position(kHigh, kLow, 9) == -1);
-  BatchSequence keys{0, 1, 64, 100};
+  BatchSequence keys{0, 1, 64, 100, 1};
   CHECK(readable_keys(keys, -1, true) == 0 && readable_keys(keys, 0, true) == 1);
   CHECK(readable_keys(keys, 63, true) == 64 && readable_keys(keys, kHigh, true) == 64);
   CHECK(readable_keys(keys, -1, false) == 64);
