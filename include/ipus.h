@@ -220,9 +220,9 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        causal those up to its position lengths[s] - n + i.  Keys without a
  *        page carry no weight; a row whose weights are all zero (no key, or
  *        only scores of -inf) gives zeros; rows outside every sequence are
- *        left as they were.  What lies past a sequence's length is never read
- *        into a result; a non-finite value among its keys may also reach rows
- *        of the same call that stand before it.  max_rows, the most rows of a sequence (0 = rows),
+ *        left as they were.  Keys and values that a row may not read, past its
+ *        position or the sequence's length, may hold anything; non-finite
+ *        values that it reads make its output non-finite in their columns.  max_rows, the most rows of a sequence (0 = rows),
  *        only picks the kernel.  fp32 scores, maxima and sums; probabilities
  *        are rounded to fp16 for the second product.  width <= 1024; widths
  *        that are multiples of 8 up to 256 with 16-byte aligned pointers and

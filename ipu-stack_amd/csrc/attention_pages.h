@@ -148,6 +148,73 @@ __device__ __forceinline__ UnitPlace find_unit(const PagedBatch& b, const UnitLi
   return p;
 }
 
+// Non-finite values.  A key that a row may not read has probability 0 there, and 0 times a
+// non-finite value would be NaN, so that one bad value would spoil the rows of a tile that
+// stand before it.  Tiles with a key that some of a wave's queries may not read are
+// therefore looked through; where one holds such a value, its products are added one by one to the
+// rows that read it, and the value is cleared before the tile's MFMAs.
+__device__ __forceinline__ uint32_t non_finite_halves(uint32_t x) {  // the top bit of each such half
+  return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u;            // an exponent of all ones carries
+}
+template <uint32_t Bytes>
+__device__ __forceinline__ bool has_non_finite(const uint8_t* tile) {  // fp16, by one wave
+  uint32_t found = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < Bytes / (16 * kWave); ++i) {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(tile + (i * kWave + threadIdx.x % kWave) * 16);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) found |= non_finite_halves(x[w]);
+  }
+  return __any(found != 0);
+}
+// Clears them, `threads` threads together, this one `thread`.
+template <uint32_t Bytes>
+__device__ __forceinline__ void clear_non_finite(uint8_t* tile, uint32_t thread, uint32_t threads) {
+#pragma unroll 1
+  for (uint32_t i = thread; i < Bytes / 16; i += threads) {
+    u32x4 x = *reinterpret_cast<const u32x4*>(tile + i * 16);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t f = non_finite_halves(x[w]);
+      x[w] &= ~((f >> 15) * 0xffffu);
+    }
+    *reinterpret_cast<u32x4*>(tile + i * 16) = x;
+  }
+}
+// Adds the products of a tile's non-finite values, in the layout of the kernels' MFMAs: o[dt][qt][c]
+// is column 16 dt + 4 (l / 16) + c of query 16 qt + l % 16, and p(kk, qt, e) the probability of
+// key 32 kk + 4 (l / 16) + e % 4 + 16 (e / 4).  chunk(row, column): where 4 columns lie in the tile.
+template <uint32_t Halves, uint32_t DT, uint32_t QT, typename P, typename Chunk>
+__device__ __forceinline__ void add_non_finite(float4_t (&o)[DT][QT], P p, const uint8_t* tile, Chunk chunk,
+                                               const uint32_t (&limit)[QT], uint32_t key0) {
+#pragma unroll
+  for (uint32_t kk = 0; kk < Halves; ++kk)
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e)
+#pragma unroll 1
+      for (uint32_t g = 0; g < 4; ++g) {
+        uint32_t lane = threadIdx.x % kWave;
+        asm volatile("" : "+v"(lane));  // nothing of this is kept in registers
+        const uint32_t r16 = lane % 16, g4 = lane / 16;
+        const uint32_t row = 32 * kk + 4 * g + e % 4 + 16 * (e / 4);
+        float w[QT];
+#pragma unroll
+        for (uint32_t qt = 0; qt < QT; ++qt) w[qt] = __shfl(p(kk, qt, e), 16 * g + r16, kWave);
+#pragma unroll
+        for (uint32_t dt = 0; dt < DT; ++dt) {
+          __builtin_amdgcn_sched_barrier(0);
+          const half4_t x = *reinterpret_cast<const half4_t*>(tile + chunk(row, 16 * dt + 4 * g4));
+#pragma unroll
+          for (uint32_t c = 0; c < 4; ++c) {
+            const float v = (float)x[c];
+            const bool bad = !(fabsf(v) <= 65504.0f);
+#pragma unroll
+            for (uint32_t qt = 0; qt < QT; ++qt) o[dt][qt][c] += bad && key0 + row < limit[qt] ? w[qt] * v : 0.0f;
+          }
+        }
+      }
+}
+
 // Results over the shared keys, from a launch before the one that joins them: for
 // every (row, query head) `parts` unnormalised rows and (reference point, sum) pairs.
 struct SharedParts {

@@ -76,6 +76,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   __shared__ __attribute__((aligned(1024))) uint8_t lds_v0[kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t lds_k1[kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t lds_v1[kTile];
+  __shared__ uint32_t wave_word[kWaves];
 
   const uint32_t lane = threadIdx.x % kWave, r16 = lane % 16, g4 = lane / 16;
   const uint32_t wave = uniform(threadIdx.x / kWave);
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     }
     const int position = row_position(mine.length, mine.end, row);
     limit[qt] = inside ? readable_keys(mine, position, a.causal) : 0;
-    if (limit[qt] < least) least = limit[qt];
+    if (inside && limit[qt] < least) least = limit[qt];  // what the others compute is not used
 #pragma unroll
     for (uint32_t ks = 0; ks < kKS; ++ks) {
       const uint32_t d0 = ks * 32 + g4 * 8;
@@ -167,7 +168,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     const uint32_t x = __shfl_xor(least, o, kWave);
     least = x < least ? x : least;
   }
-  least = uniform(least);  // below it no query of the wave masks a key
+  least = uniform(least);  // every query of the wave reads the keys below it
+  if (lane == 0) wave_word[wave] = least;
+  __syncthreads();
+  uint32_t block_least = wave_word[0];  // every query of the workgroup
+#pragma unroll
+  for (uint32_t w = 1; w < kWaves; ++w) block_least = wave_word[w] < block_least ? wave_word[w] : block_least;
+  block_least = uniform(block_least);
 
   // Keys of the block: those of its last query (Shared: all of the shared ones; the host
   // has checked that the table reaches them).
@@ -378,6 +385,27 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
       for (uint32_t qt = 0; qt < QT; ++qt) pp[kk][qt] = pf[kk][qt];
   };
 
+  // Before the output products of block j with the values in lv: those that are not finite, where
+  // some query of the workgroup may not read all of its keys.  A wave looks through a quarter.
+  auto look_through = [&](uint32_t j, uint8_t* lv) __attribute__((always_inline)) {
+    const uint32_t upto = j * kKeys + kKeys < key_end ? j * kKeys + kKeys : key_end;
+    if (upto <= block_least) return;
+    const bool mine = has_non_finite<kTile / kWaves>(lv + wave * (kTile / kWaves));
+    if (lane == 0) wave_word[wave] = mine;
+    __syncthreads();
+    if (wave_word[0] | wave_word[1] | wave_word[2] | wave_word[3]) {
+      add_non_finite<kHalves, kDT, QT>(
+          o, [&](uint32_t kk, uint32_t qt, uint32_t e) __attribute__((always_inline)) { return (float)pp[kk][qt][e]; }, lv,
+          [&](uint32_t row, uint32_t column) __attribute__((always_inline)) {
+            return row * kRowBytes + (((column / 8) ^ value_swizzle<D>(row)) << 4) + column % 8 * 2;
+          },
+          limit, j * kKeys);
+      __syncthreads();
+      clear_non_finite<kTile>(lv, threadIdx.x, kThreads);
+      __syncthreads();
+    }
+  };
+
   // Block j of this part lives in stage j % 2.  Step j: every wave's DMA of K(j) and
   // V(j - 1) has landed, and every wave is done with K(j - 1) and V(j - 2), whose
   // stages this step's DMA overwrites.  Past the last block there is no page, and
@@ -385,9 +413,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   int page = page_at(block0, entry(block0)), e = entry(block0 + 1);
   uint64_t valid = __ballot(page >= 0);
   bases(block0, page, k_rows);
-  auto step = [&](const uint8_t* lk, const uint8_t* lv, uint8_t* nk, uint8_t* nv, uint32_t j)
+  auto step = [&](const uint8_t* lk, uint8_t* lv, uint8_t* nk, uint8_t* nv, uint32_t j)
       __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (j > block0) look_through(j - 1, lv);
     page = page_at(j + 1, e);
     e = entry(j + 2);
     const uint64_t now = valid;
@@ -425,7 +454,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     }
     if (j < nblocks) step(lds_k0, lds_v1, lds_k1, lds_v0, block0 + j);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    output((nblocks - 1) % 2 == 0 ? lds_v0 : lds_v1);
+    uint8_t* last = (nblocks - 1) % 2 == 0 ? lds_v0 : lds_v1;
+    look_through(block0 + nblocks - 1, last);
+    output(last);
   }
 
   // ---- results: o[dt][qt][e] = O^T[16 dt + 4 (l / 16) + e][query], unnormalised ----

@@ -75,9 +75,10 @@ __global__ __launch_bounds__(kWave) void attention_pages_general_kernel(PagedAtt
 // joined at the end of a segment.
 //
 // Scores are computed transposed, S^T = K Q^T, and the output as O^T += V^T P^T
-// (v_mfma_f32_16x16x32_f16, fp32 accumulation), as in k_attention.hip.  The probabilities enter
-// the second product as the sum of two fp16 values (22 bits): the matrix pipes have time for it here,
-// and the result is off by little more than its own rounding.
+// (v_mfma_f32_16x16x32_f16, fp32 accumulation), as in k_attention.hip.  The probabilities
+// enter the second product as the sum of two fp16 values (22 bits): the matrix pipes have
+// time for it here, and the result is off by little more than its own rounding.  With 32
+// queries per tile they are one fp16 value (2^-11), as in the kernel for many rows.
 
 // Partial results of a launch: two slots per workgroup, each 16 * MT rows of D fp32
 // and their (reference point, sum) pairs; without memory every segment is one
@@ -143,8 +144,12 @@ struct Decode {
   static constexpr uint32_t kKT = kKeys / 16, kKS = D / 32, kDT = D / 16, kHalves = kKeys / 32;
   static constexpr uint32_t kQueries = 16 * MT;
   static constexpr uint32_t kDma = kTileBytes / 1024;  // DMA instructions of a wave per tile
-  // Workgroups per CU, by LDS (two stages of a tile per wave) and registers.
-  static constexpr uint32_t kPerCu = D > 128 ? 1 : 2;
+  // Workgroups per CU, by LDS (two stages of a tile per wave) and registers.  One keeps
+  // nearly the bandwidth of two (64 sequences x 8 heads x 4096 keys x 128: 191 us against 185); three, where
+  // they fit, lose some (96 columns: 167 against 139).
+  static constexpr uint32_t kPerCu = D > 128 || (D == 128 && MT == 2) ? 1 : 2;
+  // Probabilities as two fp16 values; with two tiles of queries as one, for the registers.
+  static constexpr bool kTwoHalves = MT == 1;
   static constexpr uint32_t kResident = 256 * kPerCu;
 };
 // 16-byte chunk c of a tile's row r lies at chunk c ^ swizzle(r): the 4 rows x 32 bytes that
@@ -288,6 +293,9 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
         qf[mt][ks] = __builtin_bit_cast(half8_t, d0 < a.width ? load16(from + d0) : u32x4{0, 0, 0, 0});
       }
     }
+    // Every query of the tile reads the keys below `least`: causal rows stand in the order
+    // of their positions.
+    const uint32_t least = readable_keys(q, row_position(q.length, q.end, q.first + query0 / group), a.causal);
     float4_t o[kDT][MT];
     float m_run[MT], l_run[MT];
 #pragma unroll
@@ -365,7 +373,7 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
       __builtin_amdgcn_sched_barrier(0);
     };
     // Softmax of tile t's scores, rows of `valid`, and the output with the values in lv.
-    auto update = [&](uint32_t t, uint64_t valid, float4_t (&sc)[kKT][MT], const uint8_t* lv) __attribute__((always_inline)) {
+    auto update = [&](uint32_t t, uint64_t valid, float4_t (&sc)[kKT][MT], uint8_t* lv) __attribute__((always_inline)) {
       const uint32_t key0 = first_key + t * kKeys;
       half8_t high[kHalves][MT], low[kHalves][MT];
 #pragma unroll
@@ -395,13 +403,25 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
             const float p = __builtin_amdgcn_exp2f(sc[2 * kk + e / 4][mt][e % 4] - m_use);
             sum += p;
             high[kk][mt][e] = (half_t)p;
-            low[kk][mt][e] = (half_t)(p - (float)high[kk][mt][e]);
+            low[kk][mt][e] = C::kTwoHalves ? (half_t)(p - (float)high[kk][mt][e]) : (half_t)0.0f;
           }
         l_run[mt] = l_run[mt] * alpha + sum;
 #pragma unroll
         for (uint32_t dt = 0; dt < kDT; ++dt) o[dt][mt] *= alpha;
       }
       __builtin_amdgcn_sched_barrier(0);
+      const uint32_t upto = (t + 1) * kKeys < all_keys ? key0 + kKeys : q.keys;
+      if (upto > least && has_non_finite<kTile>(lv)) {
+        add_non_finite<kHalves, kDT, MT>(
+            o, [&](uint32_t kk, uint32_t mt, uint32_t e) __attribute__((always_inline)) {
+              return (float)high[kk][mt][e] + (float)low[kk][mt][e];
+            }, lv,
+            [&](uint32_t row, uint32_t column) __attribute__((always_inline)) {
+              return row * kRowBytes + (((column / 8) ^ tile_swizzle<D>(row)) << 4) + column % 8 * 2;
+            },
+            limit, key0);
+        clear_non_finite<kTile>(lv, lane, kWave);
+      }
       uint32_t vbase_v = vbase;
       asm volatile("" : "+v"(vbase_v));
 #pragma unroll
@@ -417,7 +437,8 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
 #pragma unroll
           for (uint32_t mt = 0; mt < MT; ++mt) {
             o[dt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, high[kk][mt], o[dt][mt], 0, 0, 0);
-            o[dt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, low[kk][mt], o[dt][mt], 0, 0, 0);
+            if constexpr (C::kTwoHalves)
+              o[dt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, low[kk][mt], o[dt][mt], 0, 0, 0);
           }
         }
     };
@@ -474,8 +495,8 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
       for (uint32_t dt = 0; dt < kDT; ++dt)
         *reinterpret_cast<float4_t*>(mine + ((dt * 4 + g4) ^ (r16 & 7)) * 4) = o[dt][mt];
     }
-    __syncthreads();
     const uint32_t real = queries < kQueries ? queries : kQueries;
+    __syncthreads();
     const uint32_t quads = a.width / 4;
     // (row, head) of query m, for the shared keys' parts and the output.
     auto output_row = [&](uint32_t m) __attribute__((always_inline)) {

@@ -123,9 +123,14 @@ def attention(batch, query, cache, key_heads, causal, scale, fp16_probabilities=
             w = np.where(ok, np.exp(x - np.where(np.isfinite(top), top, 0.0)), 0.0)
             total = w.sum(axis=1, keepdims=True)
             w = np.where(total > 0, w / np.where(total > 0, total, 1.0), 0.0)
-            v = np.where(np.isfinite(v), v, np.nan)
+            w = np.where(np.isnan(x).any(axis=1, keepdims=True), np.nan, w)  # a NaN score that the row reads
             at = slice(first, first + n)
-            out[at, h] = w @ v
+            if np.all(np.isfinite(v)):
+                out[at, h] = w @ v
+            else:  # a row's own keys alone: 0 times another's infinity is not there
+                for r in range(n):
+                    out[first + r, h] = w[r, ok[r]] @ v[ok[r]]
+                v = np.where(np.isfinite(v), v, 0.0)
             # Probabilities rounded to fp16, and their sum of unrounded ones;
             # probabilities below fp16's normal range lose 2^-25 each against
             # a largest of 2^-8 at least; fp32 accumulation.

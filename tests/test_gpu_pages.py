@@ -274,6 +274,48 @@ def test_attention_non_finite(ipus, ctx, rows, width):
         x.free()
 
 
+@pytest.mark.parametrize("rows,lengths,heads,key_heads,width,page_rows,shared", [
+    ([3, 5], [100, 40], 4, 2, 128, 16, 0),        # few rows, one and two query tiles
+    ([8, 1], [700, 900], 8, 2, 64, 16, 0),
+    ([5], [37], 4, 4, 96, 8, 0),
+    ([4], [90], 1, 1, 256, 64, 0),
+    ([70, 200], [300, 200], 4, 2, 128, 64, 0),    # blocks
+    ([90, 1], [1500, 30], 2, 2, 72, 16, 0),       # split keys
+    ([65], [80], 2, 1, 192, 16, 0),
+    ([40], [40], 8, 1, 32, 1, 0),
+    ([3, 4], [50, 60], 2, 1, 65, 16, 0),          # the general kernel
+    ([6, 3, 2], [40, 44, 100], 4, 1, 128, 16, 42),
+    ([2] * 300, [1003] * 150 + [1001] * 150, 16, 4, 64, 16, 1002),  # prefix in its own launch
+])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_values_that_rows_may_not_read(ipus, ctx, rows, lengths, heads, key_heads, width, page_rows, shared, bad):
+    """A non-finite value at a sequence's last position reaches the rows that read it,
+    in its column, and none before them."""
+    b = Batch(np.random.default_rng(14), rows, lengths, page_rows, shared=shared)
+    for c in range((shared + page_rows - 1) // page_rows):
+        if b.table[0, c] < 0:
+            b.table[0, c] = b.pages - 1
+    cache = halves(ipus, (b.pages, 2, key_heads, page_rows, width), 1)
+    for s in range(b.sequences()):
+        p, page, row = b.places(s)
+        cache[page[-1], 1, 0, row[-1], 5] = bad
+        cache[page[-1], 0, key_heads - 1, row[-1], 3] = np.nan
+    q = halves(ipus, (b.rows, heads, width), 2)
+    bufs = [ctx.upload(q), ctx.upload(cache)] + upload_batch(ctx, b)
+    out = ctx.alloc(q.nbytes)
+    ctx.launch(attention_symbol(b), out, bufs, attention_scalars(b, heads, key_heads, width, 1))
+    got = out.download(np.float16).reshape(q.shape).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        want, bound, _ = attention(b, q.astype(np.float64), cache.astype(np.float64), key_heads, 1, width ** -0.5)
+        bound = rounded(want, bound, np.float16)
+    fine = np.isfinite(want)
+    assert 0 < np.sum(fine) < fine.size
+    assert np.array_equal(np.isfinite(got), fine)
+    assert np.all(np.abs(got[fine] - want[fine]) <= bound[fine])
+    for x in bufs + [out]:
+        x.free()
+
+
 @pytest.mark.parametrize("q_scale", [0.0, 30.0])
 def test_attention_score_ranges(ipus, ctx, q_scale):
     """Equal scores, and scores whose softmax is nearly one key."""
