@@ -21,6 +21,7 @@ namespace ipus {
 namespace {
 
 constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMaxRows = 32;  // of a workgroup
 
 inline int hip_status(hipError_t e) { return e == hipSuccess ? 0 : IPUS_ERROR_HIP_BASE - (int)e; }
 
@@ -270,7 +271,6 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, uint32_t
 
 // Keys and values of rows_per_block new rows into the cache, both as heads of
 // one walk: heads [0, key_heads) are keys, turned, the rest values, copied.
-constexpr uint32_t kMaxRows = 8;
 template <int V, bool Interleaved, bool Loop>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, uint32_t first_row,
                                                           uint32_t rows_per_block,
@@ -362,14 +362,21 @@ inline uint32_t chunk_elements(uint32_t size, uint32_t width, uint32_t rotary_wi
   return 1;
 }
 
+// An append's rows at least: a wave finds a row's place (16 heads of 32000 rows, 32 groups:
+// 4 rows 37.7 us, 2 rows 38.3, 8 rows 39.7).
+constexpr uint32_t kAppendRows = kThreads / kWave;
 struct Plan {
   uint32_t rows, heads, lanes, blocks_y, lds;
   bool loop;
 };
-// Whole rows per workgroup, enough of them for about four units per thread (the
-// angles, computed once per row and workgroup, then cost little); where that would
-// make fewer than 1024 workgroups, one row and as many heads as it has lanes for.
-inline Plan plan_rows(uint32_t rows, uint32_t heads, uint32_t width, uint32_t rotary_width, uint32_t v) {
+// Whole rows per workgroup, the fewest (from `least` on) whose heads keep four fifths of
+// its lane groups' turns busy: an angle is computed once per row and workgroup in any
+// case, and small workgroups end together (16384 rows of 40 heads in 32 groups: 2 rows
+// 58.5 us, 1 row 65.0, 3 rows 62.9, 6 rows 73.1; of 16 heads in 16 groups, fp32: 1 row
+// 43.2, 4 rows 46.6, 8 rows 50.7).  Where that would make fewer than 1024 workgroups,
+// one row and as many heads as it has groups for.
+inline Plan plan_rows(uint32_t rows, uint32_t heads, uint32_t width, uint32_t rotary_width, uint32_t v,
+                      uint32_t least) {
   const uint32_t half = rotary_width / 2;
   const uint32_t units = half / v + (width - rotary_width + 2 * v - 1) / (2 * v);
   Plan p;
@@ -377,9 +384,11 @@ inline Plan plan_rows(uint32_t rows, uint32_t heads, uint32_t width, uint32_t ro
   while (p.lanes < units && p.lanes < (uint32_t)kWave) p.lanes *= 2;
   p.loop = units > p.lanes;
   const uint32_t slots = kThreads / p.lanes;
-  p.rows = (uint32_t)(4ull * slots / heads);
-  if (p.rows > kMaxRows) p.rows = kMaxRows;
-  if (half > 0 && p.rows > 2048 / half) p.rows = 2048 / half;
+  uint32_t most = half > 0 && kMaxRows > 2048 / half ? 2048 / half : kMaxRows;  // 16 KiB of angles
+  if (heads > 4 * slots) most = 1;
+  p.rows = least;
+  while (p.rows < most && 5ull * p.rows * heads < 4ull * slots * ((p.rows * heads + slots - 1) / slots)) ++p.rows;
+  if (p.rows > most) p.rows = most;
   if (p.rows < 1) p.rows = 1;
   p.heads = heads;
   if ((rows + p.rows - 1) / p.rows < 1024) {
@@ -410,7 +419,7 @@ int over_rows(uint32_t rows, uint32_t rows_per_block, const F& launch) {
 
 template <typename T, int V, bool Interleaved, bool Norm>
 int launch_rotary_as(hipStream_t stream, const RotaryArgs& a) {
-  const Plan p = plan_rows(a.rows, a.heads, a.width, a.rotary_width, V);
+  const Plan p = plan_rows(a.rows, a.heads, a.width, a.rotary_width, V, 1);
   return over_rows(a.rows, p.rows, [&](uint32_t first, uint32_t blocks) {
     const dim3 grid(blocks, p.blocks_y), block(kThreads);
     if (p.loop)
@@ -428,7 +437,7 @@ int launch_rotary_v(hipStream_t stream, const RotaryArgs& a) {
 
 template <int V, bool Interleaved>
 int launch_append_as(hipStream_t stream, const AppendArgs& a) {
-  const Plan p = plan_rows(a.rows, 2 * a.key_heads, a.width, a.rotary_width, V);
+  const Plan p = plan_rows(a.rows, 2 * a.key_heads, a.width, a.rotary_width, V, kAppendRows);
   return over_rows(a.rows, p.rows, [&](uint32_t first, uint32_t blocks) {
     const dim3 grid(blocks, p.blocks_y), block(kThreads);
     if (p.loop)
