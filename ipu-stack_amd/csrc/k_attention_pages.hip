@@ -95,9 +95,17 @@ constexpr uint32_t kMostResident = 512;  // workgroups on the chip at most (Deco
 // How a launch's segments (a sequence's query tile and key head, with its key tiles) are
 // dealt to the workgroups.  A segment's start and end cost about as much as four tiles per
 // wave, joining parts of it as much again:
+//  - none of more than 32 tiles, 600 times the longest in all, and no parts of shared keys
+//    to join: a wave takes a segment
+//    alone, so that the starts of four run at once and nothing is joined (us, alone / by
+//    a workgroup's waves together; 128 columns: 256 sequences x 8 heads x 300 keys
+//    66.7 / 82.2, 128 x 8 x 616 63.4 / 65.3, 300 x 8 of 37 to 600 keys 72 / 123; 64
+//    columns: 256 x 16 x 60 27 / 62, 40 x 16 x 200 (640 segments) 14.4 / 18.2; not 64 x 8 x 300
+//    at 128 columns (512 segments) 23.3 / 20.5, where a wave's own latency counts);
 //  - no segment of more than 16 tiles: all whole;
-//  - at least 32 tiles per resident workgroup: the tiles of all segments are one line, cut
-//    into an equal chunk for each, wherever the cuts fall;
+//  - at least 40 tiles per resident workgroup: the tiles of all segments are one line, cut
+//    into an equal chunk for each, wherever the cuts fall (128 segments of 125 tiles, 31 per
+//    workgroup, 61.6 us so, in parts 54.6);
 //  - in between: every segment in parts of its own, of at least 8 tiles, one per
 //    workgroup (cut at any place, a workgroup would pay two segments' starts for a few tiles:
 //    2 x 8 segments of 34 tiles 18.1 us, of 48 tiles, where the cuts coincide, 13.0), and
@@ -106,8 +114,9 @@ constexpr uint32_t kMostResident = 512;  // workgroups on the chip at most (Deco
 // The line's units are tiles (part_tiles = 0) or parts of at most part_tiles tiles.
 struct Shares {
   uint32_t part_tiles;
-  uint64_t chunk;  // units per workgroup
+  uint64_t chunk;  // units per workgroup, or per wave
   uint64_t parts;  // units of the line, or a bound on them
+  bool alone;      // every wave has segments of its own
   __device__ __forceinline__ uint32_t units(uint32_t tiles) const {
     return part_tiles == 0 ? tiles : part_tiles >= tiles ? 1 : (tiles + part_tiles - 1) / part_tiles;
   }
@@ -116,10 +125,15 @@ struct Shares {
   }
 };
 __device__ __forceinline__ Shares share_out(uint64_t tiles, uint64_t segments, uint32_t longest, uint32_t groups,
-                                            uint32_t resident, bool may_split) {
-  constexpr uint32_t kWholeTiles = 16, kLeastTiles = 8, kChunkTiles = 32, kCus = 256;
+                                            uint32_t resident, bool may_split, bool may_alone) {
+  constexpr uint32_t kAloneTiles = 32, kAloneSegments = 600;
+  constexpr uint32_t kWholeTiles = 16, kLeastTiles = 8, kChunkTiles = 40, kCus = 256;
+  if (may_alone && longest <= kAloneTiles && (uint64_t)longest * kAloneSegments <= tiles) {
+    const uint32_t waves = groups * kWaves;
+    return {0xffffffffu, quotient(segments + waves - 1, waves), segments, true};
+  }
   if (!may_split || longest <= kWholeTiles)
-    return {0xffffffffu, quotient(segments + groups - 1, groups), segments};
+    return {0xffffffffu, quotient(segments + groups - 1, groups), segments, false};
   if (resident > groups) resident = groups;
   const uint64_t each = quotient(tiles + resident - 1, resident);
   if (each < kChunkTiles) {
@@ -128,10 +142,10 @@ __device__ __forceinline__ Shares share_out(uint64_t tiles, uint64_t segments, u
     const uint32_t least = (longest + kMaxParts - 1) / kMaxParts;
     if (part < least) part = least;
     const uint64_t parts = quotient(tiles, part) + segments;  // at most
-    if (parts <= groups) return {part, 1, parts};
+    if (parts <= groups) return {part, 1, parts, false};
   }
   const uint64_t least = (longest + kMaxParts - 2) / (kMaxParts - 1);
-  return {0, each < least ? least : each, 0};
+  return {0, each < least ? least : each, 0, false};
 }
 
 // D: the width rounded up to 32, 64, 96, 128, 192 or 256 columns, which are computed and
@@ -219,11 +233,13 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
   segments = from_lane(scan(segments), kWave - 1);
   longest = largest(longest);
   if (segments == 0) return;
-  const Shares shares = share_out(tiles, segments, longest, gridDim.x, C::kResident, split.rows != nullptr);
+  const Shares shares = share_out(tiles, segments, longest, gridDim.x, C::kResident, split.rows != nullptr,
+                                  shared.parts == 0);
   auto line_units = [&](const Units& u) __attribute__((always_inline)) { return u.segments * shares.units(u.tiles); };
   auto units_in = [&](uint32_t s) __attribute__((always_inline)) { return line_units(units_at(s)); };
   UnitLine line{scan(line_units(held)), 0};
-  const uint64_t begin = (uint64_t)blockIdx.x * shares.chunk;
+  const bool alone = shares.alone;
+  const uint64_t begin = (alone ? (uint64_t)blockIdx.x * kWaves + wave : blockIdx.x) * shares.chunk;
   if (begin >= shares.total(tiles, segments)) return;
   const UnitPlace place = find_unit(b, line, begin, units_in);
   uint32_t s = place.sequence;
@@ -448,10 +464,11 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     };
 
-    uint32_t t = tile_first + wave;
+    const uint32_t stride = alone ? 1 : kWaves;
+    uint32_t t = tile_first + (alone ? 0 : wave);
     if (t < tile_last) {
       int page = page_at(t, entry(t));
-      int e = entry(t + kWaves);
+      int e = entry(t + stride);
       uint64_t valid = __ballot(page >= 0);
       fetch_values(t, page, my0);
       fetch_keys(t, page);
@@ -459,15 +476,15 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
       // their way into the registers just read, the rest.
       auto step = [&](uint8_t* lv, uint8_t* next) __attribute__((always_inline)) {
         settle();
-        page = page_at(t + kWaves, e);
-        e = entry(t + 2 * kWaves);
-        fetch_values(t + kWaves, page, next);
+        page = page_at(t + stride, e);
+        e = entry(t + 2 * stride);
+        fetch_values(t + stride, page, next);
         float4_t sc[kKT][MT];
         scores(sc);
-        fetch_keys(t + kWaves, page);
+        fetch_keys(t + stride, page);
         update(t, valid, sc, lv);
         valid = __ballot(page >= 0);
-        t += kWaves;
+        t += stride;
       };
       while (true) {
         step(my0, my1);
@@ -481,6 +498,30 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
     // ---- the waves' results joined ----
     // Lane numbers made opaque, so that nothing of this is computed before the key loop.
     const uint32_t tid = opaque(threadIdx.x), r16 = tid % 16, g4 = tid % kWave / 16;
+    // (row, head) of query m, for the shared keys' parts and the output.
+    auto output_row = [&](uint32_t m) __attribute__((always_inline)) {
+      const uint32_t row = (query0 + m) / group;
+      return (uint64_t)(q.first + row) * a.query_heads + key_head * group + (query0 + m - row * group);
+    };
+    if (alone) {  // nothing to join
+#pragma unroll
+      for (uint32_t mt = 0; mt < MT; ++mt) {
+        const uint32_t m = 16 * mt + r16;
+        const uint64_t at = output_row(m < queries ? m : queries - 1);
+        const float l = sum_of_query(l_run[mt]);
+        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (uint32_t dt = 0; dt < kDT; ++dt) {
+          const uint32_t d = 16 * dt + 4 * g4;
+          half4_t h;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h[e] = (half_t)(o[dt][mt][e] * inverse);
+          if (m < queries && d < a.width) *reinterpret_cast<half4_t*>((half_t*)a.out + at * a.width + d) = h;
+        }
+      }
+      unit = stop;
+      continue;
+    }
     // A wave's rows, fp32 [kQueries][D], fill its stage 0 and 1 (16 rows of each).
     static_assert(16 * D * 4 <= kTile, "a stage holds 16 rows");
 #pragma unroll
@@ -498,11 +539,6 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
     const uint32_t real = queries < kQueries ? queries : kQueries;
     __syncthreads();
     const uint32_t quads = a.width / 4;
-    // (row, head) of query m, for the shared keys' parts and the output.
-    auto output_row = [&](uint32_t m) __attribute__((always_inline)) {
-      const uint32_t row = (query0 + m) / group;
-      return (uint64_t)(q.first + row) * a.query_heads + key_head * group + (query0 + m - row * group);
-    };
     auto wave_quad = [&](uint32_t w, uint32_t m, uint32_t c) __attribute__((always_inline)) {
       const float* from = reinterpret_cast<const float*>((m < 16 ? stage0 : stage1) + w * kTile) + (m % 16) * D;
       return *reinterpret_cast<const float4_t*>(from + (c ^ (m & 7)) * 4);

@@ -209,6 +209,53 @@ def test_attention_chunks(ipus, ctx, rows, lengths, heads, key_heads, width, pag
     check_attention(ipus, ctx, b, heads, key_heads, width, causal)
 
 
+MANY = [
+    # sequences (their rows in turn), lengths from, to, query heads, key heads, width, page_rows
+    (220, [1], 65, 96, 16, 4, 128, 16),
+    (330, [1], 0, 64, 2, 2, 64, 8),
+    (160, [2], 40, 64, 64, 4, 96, 32),
+    (100, [1], 8, 30, 8, 8, 256, 16),
+    (100, [1, 0], 90, 90, 16, 16, 192, 64),
+    (1100, [1], 1, 6, 8, 8, 32, 2),
+    (260, [3, 2, 5], 33, 60, 8, 4, 72, 4),
+]
+
+
+@pytest.mark.parametrize("sequences,rows,low,high,heads,key_heads,width,page_rows", MANY)
+@pytest.mark.parametrize("causal", [0, 1])
+def test_attention_of_many_short_sequences(ipus, ctx, sequences, rows, low, high, heads, key_heads, width, page_rows,
+                                           causal):
+    rng = np.random.default_rng(sequences)
+    n = [rows[s % len(rows)] for s in range(sequences)]
+    lengths = [int(x) for x in rng.integers(low, high + 1, sequences)]
+    b = Batch(rng, n, lengths, page_rows, 3)
+    check_attention(ipus, ctx, b, heads, key_heads, width, causal)
+
+    def spoilt(cache, q):  # the last row's own value, which the rows before it may not read
+        for s in range(0, sequences, 7):
+            _, page, row = b.places(s)
+            if len(page) and b.n[s] > 1:
+                cache[page[-1], 1, 0, row[-1], 1] = np.nan
+
+    if causal and max(rows) > 1:
+        cache = halves(ipus, (b.pages, 2, key_heads, page_rows, width), 1)
+        q = halves(ipus, (b.rows, heads, width), 2)
+        spoilt(cache, q)
+        bufs = [ctx.upload(q), ctx.upload(cache)] + upload_batch(ctx, b)
+        out = ctx.upload(np.zeros(q.shape, np.float16))
+        ctx.launch("ipu_stack_attention_pages_f16", out, bufs, attention_scalars(b, heads, key_heads, width, 1))
+        got = out.download(np.float16).reshape(q.shape).astype(np.float64)
+        with np.errstate(invalid="ignore"):
+            want, bound, inside = attention(b, q.astype(np.float64), cache.astype(np.float64), key_heads, 1,
+                                            width ** -0.5)
+        bad = np.isnan(want)
+        assert np.any(bad) and np.array_equal(np.isnan(got)[inside], bad[inside])
+        good = inside[:, None, None] & ~bad
+        assert np.all(np.abs(got - want)[good] <= rounded(want, bound, np.float16)[good])
+        for x in bufs + [out]:
+            x.free()
+
+
 @pytest.mark.parametrize("max_rows", [0, 1, 7, 1000])
 def test_attention_is_whole_for_any_row_hint(ipus, ctx, max_rows):
     b = Batch(np.random.default_rng(2), [70, 1, 9], [300, 400, 9], 16)
