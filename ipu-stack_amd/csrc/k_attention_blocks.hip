@@ -37,6 +37,13 @@ struct SplitKeys {
   uint32_t parts;  // at most; 1: not split
 };
 constexpr uint32_t kMaxSplits = 16;
+// Key blocks from which they are split, and of a part at least.  The parts' rows and the
+// second launch cost what 8 to 16 key blocks take (128 columns, 32 query heads, us split /
+// whole: 512 rows against 1024 keys 37.2 / 28.9, against 2048 40.4 / 49.1, 128 against 4096
+// 36.9 / 88.8; 256 columns, 16 heads: 512 against 512 (16 blocks) 26.8 / 22.2, against 1024
+// 31.3 / 36.6).  Where the table cannot hold so many keys there is no second launch either
+// (512 rows against 512 keys 18.7, with both 28.8).
+constexpr uint32_t kLeastSplit = 17, kLeastPart = 4;
 
 template <int D, int QT>
 struct Block {
@@ -104,13 +111,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
       const uint32_t want = total < kFullChip / 2 ? kFullChip / (uint32_t)total : 1;
       splits = want < split.parts ? want : split.parts;
     }
+    // An XCD's range of the line, all blocks' first parts first: of blocks with fewer keys
+    // the other parts have nothing to do, and workgroups at a fixed distance meet on the same
+    // CUs (64 blocks of 8 possible parts, one in use: 41.5 us, so 29).
     const uint64_t items = total * splits, per_xcd = (items + 7) / 8;
-    const uint64_t item = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
+    uint64_t local = blockIdx.x / 8;
+    if (!Shared && splits > 1) {
+      const uint32_t across = (uint32_t)quotient(per_xcd + splits - 1, splits);
+      const uint32_t turn = (uint32_t)local / across;
+      local = turn < splits ? (uint64_t)((uint32_t)local - turn * across) * splits + turn : per_xcd;
+    }
+    const uint64_t item = blockIdx.x % 8 * per_xcd + local;
     block = quotient(item, splits);
     part = (uint32_t)(item - block * splits);
-    // Offsets that decrease can make more blocks than the host expects (and has
-    // counters for); what lies past the grid is not computed.
-    if (blockIdx.x / 8 >= per_xcd || item >= items || item >= gridDim.x) return;
+    // Offsets that decrease can make more blocks than the host expects (and has memory
+    // for the parts of); what lies past the grid is not computed.
+    if (local >= per_xcd || item >= items || item >= gridDim.x) return;
     uint64_t within = block;
     if (!Shared) {
       const UnitPlace place = find_unit(b, line, block, blocks_in);
@@ -190,7 +206,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   // This part's: every part has a block of keys, but for the first of none at all.
   const uint32_t all_blocks = (key_end + kKeys - 1) / kKeys;
   uint32_t per_part = (all_blocks + splits - 1) / splits;
-  if (!Shared && splits > 1 && per_part < 4) per_part = 4;  // a part's start and its join cost about as much
+  if (!Shared && splits > 1 && per_part < kLeastPart) per_part = kLeastPart;
+  if (!Shared && all_blocks < kLeastSplit) per_part = all_blocks;
   if (per_part == 0) per_part = 1;
   uint32_t parts = (all_blocks + per_part - 1) / per_part;
   if (parts == 0) parts = 1;
@@ -510,31 +527,33 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   }
 }
 
-// Joins the parts of the split blocks: a wave per row and query head.  The first eight parts
-// are loaded before it is known whether the row is one of them, and of how many.
+// Joins the parts of the split blocks: a wave per row and query head.
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs a, uint32_t few, SplitKeys split) {
   const uint32_t row = blockIdx.x, lane = threadIdx.x % kWave;
   const uint32_t head = blockIdx.y * kWaves + threadIdx.x / kWave;
   if (head >= a.query_heads) return;
   const uint64_t at = (uint64_t)row * a.query_heads + head;
-  const uint32_t parts = split.counts[at];
-  // Lane z holds part z's weight, exp2(m - max m) / sum.
-  const float* pair = split.sums + (at * split.parts + (lane < split.parts ? lane : 0)) * 2;
-  const float m0 = pair[0], l0 = pair[1];
-  const float* rows = split.rows + at * split.parts * a.width;
-  const uint32_t c = lane * 4 < a.width ? lane * 4 : 0;
-  float4_t y[kMaxSplits];
-#pragma unroll
-  for (uint32_t z = 0; z < 8; ++z)
-    y[z] = *reinterpret_cast<const float4_t*>(rows + (uint64_t)(z < split.parts ? z : 0) * a.width + c);
+  const uint32_t written = split.counts[at];
+  // Rows of no split block: what stands there is not theirs.
   const uint32_t s = find_sequence(a.batch, row);
   if (s >= a.batch.sequences) return;
   const BatchSequence q = sequence_at(a.batch, s, a.rows);
-  if (row < q.first || q.rows * (a.query_heads / a.key_heads) <= few) return;
+  const uint32_t parts = uniform(written);
   if (parts < 2 || parts > split.parts) return;  // 1: its block has written the output
+  // Lane z holds part z's weight, exp2(m - max m) / sum.
+  const float* pair = split.sums + (at * split.parts + (lane < parts ? lane : 0)) * 2;
+  const float m0 = pair[0], l0 = pair[1];
+  const float* rows = split.rows + at * split.parts * a.width;
+  const uint32_t c = lane * 4 < a.width ? lane * 4 : 0;
+  constexpr uint32_t kAtOnce = 8;  // loads in flight (past the last part: the last one again, not added)
+  float4_t y[kAtOnce];
+  auto load = [&](uint32_t z0) __attribute__((always_inline)) {
 #pragma unroll
-  for (uint32_t z = 8; z < kMaxSplits; ++z)
-    if (z < parts) y[z] = *reinterpret_cast<const float4_t*>(rows + (uint64_t)z * a.width + c);
+    for (uint32_t z = 0; z < kAtOnce; ++z)
+      y[z] = *reinterpret_cast<const float4_t*>(rows + (uint64_t)(z0 + z < parts ? z0 + z : parts - 1) * a.width + c);
+  };
+  load(0);
+  if (row < q.first || q.rows * (a.query_heads / a.key_heads) <= few) return;
   const float m = lane < parts ? m0 : -INFINITY;
   float top = m;
   for (uint32_t o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
@@ -543,10 +562,15 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
   const float sum = wave_sum(lane < parts ? f * l0 : 0.0f);
   const float weight = sum == 0.0f ? 0.0f : f / sum;
   float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t z0 = 0;;) {
 #pragma unroll
-  for (uint32_t z = 0; z < kMaxSplits; ++z) {
-    const float w = __shfl(weight, z, kWave);
-    if (z < parts) x += y[z] * w;
+    for (uint32_t z = 0; z < kAtOnce; ++z) {
+      const float w = __shfl(weight, z0 + z, kWave);
+      if (z0 + z < parts) x += y[z] * w;
+    }
+    z0 += kAtOnce;
+    if (z0 >= parts) break;
+    load(z0);
   }
   if (lane * 4 < a.width) {
     half4_t h;
@@ -569,9 +593,14 @@ int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2,
   }
   blocks *= a.key_heads;
   SplitKeys split = given;
-  // Parts where the blocks surely leave half of the chip's workgroups idle; how many,
-  // the kernel decides by the blocks that there are.
-  if (!Shared && a.workspace.data && blocks < kFullChip) {
+  // Parts where the blocks may leave half of the chip's workgroups idle and the table
+  // holds keys enough; how many, the kernel decides by the blocks that there are.
+  const uint64_t reach = (uint64_t)a.batch.table_columns * a.batch.page_rows;
+  // few = 0: sequences of max_rows each.
+  const uint64_t least = few > 0 ? 0 : ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) + kQueries - 1) / kQueries *
+                                           a.batch.sequences * a.key_heads;
+  const bool may_split = least < kFullChip / 2 && reach > (uint64_t)(kLeastSplit - 1) * Block<D, QT>::kKeys;
+  if (!Shared && a.workspace.data && blocks < kFullChip && may_split) {
     const uint64_t rows = (uint64_t)a.rows * a.query_heads;
     uint64_t parts = a.workspace.bytes / sizeof(float) / rows;  // floats per row, then parts
     parts = parts > 0 ? (parts - 1) / (a.width + 2) : 0;
@@ -583,8 +612,9 @@ int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2,
       split.counts = (uint32_t*)(split.sums + rows * parts * 2);
     }
   }
-  // Split blocks make at most kFullChip workgroups (Shared: the given parts of each).
-  uint64_t grid = Shared ? blocks * split.parts : blocks < kFullChip ? kFullChip : blocks;
+  // Split blocks make at most kFullChip workgroups, in ranges of whole blocks' parts (Shared: the
+  // given parts of each).
+  uint64_t grid = Shared ? blocks * split.parts : split.parts > 1 ? kFullChip + 8 * kMaxSplits : blocks;
   grid = (grid + 7) / 8 * 8;
   if (grid > 0xffffffull) return IPUS_ERROR_UNAVAILABLE;  // a grid dimension holds less than 2^32 threads
   hipLaunchKernelGGL((attention_blocks_kernel<D, DC, QT, Shared>), dim3((uint32_t)grid), dim3(kThreads), 0, stream, a,
