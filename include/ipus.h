@@ -222,8 +222,9 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        only scores of -inf) gives zeros; rows outside every sequence are
  *        left as they were.  Keys and values that a row may not read, past its
  *        position or the sequence's length, may hold anything; non-finite
- *        values that it reads make its output non-finite in their columns.  max_rows, the most rows of a sequence (0 = rows),
- *        only picks the kernel.  fp32 scores, maxima and sums; probabilities
+ *        values that it reads make its output non-finite in their columns.
+ *        max_rows, the most rows of a sequence (0 = rows), only picks the
+ *        kernel.  fp32 scores, maxima and sums; probabilities
  *        are rounded to fp16 for the second product.  width <= 1024; widths
  *        that are multiples of 8 up to 256 with 16-byte aligned pointers and
  *        strides run on the matrix units.

@@ -68,11 +68,16 @@ __global__ __launch_bounds__(kWave) void attention_pages_general_kernel(PagedAtt
 // its place by a scan over the sequences' lengths (two reads of a few words, in L2).
 //
 // Waves work alone: wave w takes the chunk's key tiles w, w + 4, ...  A tile's keys go
-// to registers in the layout of the first MFMA operand, its values by LDS DMA into the wave's own stage (the
-// transposing LDS read needs them there), the next tile's loads run
-// under this one's arithmetic, and the page numbers of the one after under both.  At 8 waves
-// per CU 128 KiB are in flight, without a barrier until the waves' results are
+// to registers in the layout of the first MFMA operand, its values by LDS DMA into the
+// wave's own stage (the transposing LDS read needs them there), the next tile's loads run
+// under this one's arithmetic, and the page numbers of the one after under both.  At 8
+// waves per CU 128 KiB are in flight, without a barrier until the waves' results are
 // joined at the end of a segment.
+//
+// Measured (width 128, 32 query heads on 8): 64 sequences of 2048 to 32768 keys, 2.8 GB,
+// 481 us, 5.9 TB/s of a copy's 6.3; 64 of 4000 181 us, 5.8; 256 of 300 67 us, 4.7; 64 of 300 20 us,
+// where a segment's start (five loads that wait for each other, about 6 us) and end (2 us)
+// are as long as its keys' loads.
 //
 // Scores are computed transposed, S^T = K Q^T, and the output as O^T += V^T P^T
 // (v_mfma_f32_16x16x32_f16, fp32 accumulation), as in k_attention.hip.  The probabilities
@@ -719,8 +724,14 @@ int launch_decode(hipStream_t stream, const PagedAttentionArgs& a, float scale_l
 }
 
 // Queries of a key head (rows x query heads) up to which a sequence is the decode kernel's.
+// Up to 16, one tile, it is ahead everywhere; of 17 to 32 it wins where there are few
+// segments and loses a little where there are many (us, decode / blocks at 32 queries: 16
+// sequences x 16 heads x 8000 keys x 128 190 / 220, x 64 118 / 150; 64 x 16 x 2000 x 128
+// 228 / 205, 64 x 8 x 2000 x 64 58 / 64); at 48, three tiles or two that read the keys
+// twice, it is behind (64 x 16 x 2000 x 128 372 / 206).
 constexpr uint32_t kFewQueries = 32;
-constexpr uint32_t kFewBeside = 16;  // beside sequences of more
+// Beside sequences of more the blocks' launch is there anyway: only sequences of one tile.
+constexpr uint32_t kFewBeside = 16;
 
 // The shared keys in a launch of their own: their parts in the workspace's lower
 // end, what is left to the launch that joins them.  That launch costs 8 us and more

@@ -13,6 +13,12 @@
 // of its row, so a workgroup takes whole rows, computes their sines and cosines
 // once (the angle in 64 bits: p f_i passes 2^20 rad in long contexts, where fp32
 // holds 2^-4) into LDS, with the first elements' loads already under way.
+//
+// Measured against a copy's 6.3 TB/s: 16384 rows x 16 heads x 128 fp32 43.5 us (6.2 TB/s);
+// 16384 rows x 40 heads x 128 fp16 with the norm 58.2 us (5.8: the sum over the head stands
+// between its loads and stores); 32000 rows x 8 key heads x 128 into pages 37.0 us (5.4 of the rows
+// in use: a row's keys and values go to 16 places).  A step of few rows takes 4.2 to 4.5 us,
+// 2.8 to 3.7 of them on the GPU: a launch and four loads that wait for each other.
 #include "../../include/ipus.h"
 #include "kernels.h"
 #include "pages.h"

@@ -209,6 +209,25 @@ def test_attention_chunks(ipus, ctx, rows, lengths, heads, key_heads, width, pag
     check_attention(ipus, ctx, b, heads, key_heads, width, causal)
 
 
+SPLIT = [
+    # blocks of queries whose keys are cut, up to 16 times, beside ones that are not
+    ([70], [4100], 4, 1, 64, 16, 0),
+    ([64, 64], [3000, 90], 4, 4, 128, 64, 0),
+    ([33, 1, 40, 1], [1100, 2500, 64, 9], 2, 2, 96, 8, 2),
+    ([60, 60], [1025, 1024], 2, 1, 128, 32, 0),
+    ([40], [513], 3, 3, 256, 16, 0),
+    ([129], [2200], 1, 1, 192, 128, 1),
+    ([200], [5000], 5, 1, 32, 16, 0),
+]
+
+
+@pytest.mark.parametrize("rows,lengths,heads,key_heads,width,page_rows,pad", SPLIT)
+@pytest.mark.parametrize("causal", [0, 1])
+def test_attention_with_split_keys(ipus, ctx, rows, lengths, heads, key_heads, width, page_rows, pad, causal):
+    b = Batch(np.random.default_rng(width), rows, lengths, page_rows, pad)
+    check_attention(ipus, ctx, b, heads, key_heads, width, causal)
+
+
 MANY = [
     # sequences (their rows in turn), lengths from, to, query heads, key heads, width, page_rows
     (220, [1], 65, 96, 16, 4, 128, 16),
