@@ -602,9 +602,10 @@ int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2,
   // Parts where the blocks may leave half of the chip's workgroups idle and the table
   // holds keys enough; how many, the kernel decides by the blocks that there are.
   const uint64_t reach = (uint64_t)a.batch.table_columns * a.batch.page_rows;
-  // few = 0: sequences of max_rows each.
-  const uint64_t least = few > 0 ? 0 : ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) + kQueries - 1) / kQueries *
-                                           a.batch.sequences * a.key_heads;
+  // Known exactly where every sequence has max_rows.
+  uint64_t least = 0;
+  if (few == 0 && (uint64_t)a.batch.sequences * a.max_rows == a.rows)
+    least = ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) + kQueries - 1) / kQueries * a.batch.sequences * a.key_heads;
   const bool may_split = least < kFullChip / 2 && reach > (uint64_t)(kLeastSplit - 1) * Block<D, QT>::kKeys;
   if (!Shared && a.workspace.data && blocks < kFullChip && may_split) {
     const uint64_t rows = (uint64_t)a.rows * a.query_heads;

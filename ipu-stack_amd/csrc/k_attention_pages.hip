@@ -795,6 +795,12 @@ int launch_decode(hipStream_t stream, const PagedAttentionArgs& a, float scale_l
 constexpr uint32_t kFewQueries = 32;
 // Beside sequences of more the blocks' launch is there anyway: only sequences of one tile.
 constexpr uint32_t kFewBeside = 16;
+// Where the table holds few keys and there are few segments, the blocks take those too: one
+// launch, and their time hardly counts (us, one launch / two; a prompt of 100 rows beside
+// single ones, 128 columns, 32 query heads on 8: 17 sequences x 256 keys 12.9 / 23.8, x 1000
+// 27.8 / 47.9, x 2000 32.1 / 48.2, 65 x 1000 54 / 71; not 17 x 4000 84 / 79, nor 257 x 128 (2056
+// segments) 53 / 43; of 64 columns, 16 heads: 65 x 1000 60 / 66, 120 x 1000 (1920) 102 / 98).
+constexpr uint32_t kShortReach = 2560, kShortSegments = 1280;
 
 // The shared keys in a launch of their own: their parts in the workspace's lower
 // end, what is left to the launch that joins them.  That launch costs 8 us and more
@@ -856,6 +862,9 @@ int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a) {
   // Sequences of many rows, and those of few beside them, of which there are none
   // where every sequence has max_rows.
   if ((uint64_t)a.batch.sequences * a.max_rows == a.rows) return launch_attention_blocks(stream, a, scale_log2, 0);
+  if ((uint64_t)a.batch.table_columns * a.batch.page_rows <= kShortReach &&
+      (uint64_t)a.batch.sequences * a.key_heads <= kShortSegments)
+    return launch_attention_blocks(stream, a, scale_log2, 0);
   if (int e = launch_attention_blocks(stream, a, scale_log2, kFewBeside)) return e;
   PagedAttentionArgs beside = a;
   beside.max_rows = 1;  // one tile of queries

@@ -376,11 +376,11 @@ struct Plan {
   bool loop;
 };
 // Whole rows per workgroup, the fewest (from `least` on) whose heads keep four fifths of
-// its lane groups' turns busy: an angle is computed once per row and workgroup in any
-// case, and small workgroups end together (16384 rows of 40 heads in 32 groups: 2 rows
-// 58.5 us, 1 row 65.0, 3 rows 62.9, 6 rows 73.1; of 16 heads in 16 groups, fp32: 1 row
-// 43.2, 4 rows 46.6, 8 rows 50.7).  Where that would make fewer than 1024 workgroups,
-// one row and as many heads as it has groups for.
+// its lane groups' turns busy, or as many as they can be: an angle is computed once per row
+// and workgroup in any case, and small workgroups end together (16384 rows of 40 heads in 32
+// groups: 2 rows 58.5 us, 1 row 65.0, 3 rows 62.9, 6 rows 73.1; of 16 heads in 16 groups,
+// fp32: 1 row 43.2, 4 rows 46.6, 8 rows 50.7).  Not so many that they make fewer than 1024
+// workgroups; where `least` does, one row and as many heads as it has groups for.
 inline Plan plan_rows(uint32_t rows, uint32_t heads, uint32_t width, uint32_t rotary_width, uint32_t v,
                       uint32_t least) {
   const uint32_t half = rotary_width / 2;
@@ -392,9 +392,14 @@ inline Plan plan_rows(uint32_t rows, uint32_t heads, uint32_t width, uint32_t ro
   const uint32_t slots = kThreads / p.lanes;
   uint32_t most = half > 0 && kMaxRows > 2048 / half ? 2048 / half : kMaxRows;  // 16 KiB of angles
   if (heads > 4 * slots) most = 1;
-  p.rows = least;
-  while (p.rows < most && 5ull * p.rows * heads < 4ull * slots * ((p.rows * heads + slots - 1) / slots)) ++p.rows;
-  if (p.rows > most) p.rows = most;
+  if (most > rows / 1024) most = rows / 1024 > least ? rows / 1024 : least;
+  // Busy parts of rows x heads on turns of slots, compared crosswise.
+  auto turns = [&](uint32_t r) { return (r * heads + slots - 1) / slots; };
+  p.rows = least < most ? least : most;
+  for (uint32_t r = p.rows; r <= most && heads <= 4 * slots; ++r) {
+    if ((uint64_t)r * turns(p.rows) > (uint64_t)p.rows * turns(r)) p.rows = r;
+    if (5ull * p.rows * heads >= 4ull * slots * turns(p.rows)) break;
+  }
   if (p.rows < 1) p.rows = 1;
   p.heads = heads;
   if ((rows + p.rows - 1) / p.rows < 1024) {

@@ -218,6 +218,9 @@ SPLIT = [
     ([40], [513], 3, 3, 256, 16, 0),
     ([129], [2200], 1, 1, 192, 128, 1),
     ([200], [5000], 5, 1, 32, 16, 0),
+    ([100, 1, 3, 1], [150, 2700, 40, 1], 8, 2, 128, 64, 0),
+    ([30, 1, 0, 2], [2600, 3000, 5, 2], 16, 16, 72, 16, 3),
+    ([1, 90, 17], [5000, 91, 2000], 8, 8, 256, 128, 0),
 ]
 
 
