@@ -163,13 +163,15 @@ constexpr uint32_t kMostResident = 512;  // workgroups on the chip at most (Deco
 // How a launch's segments (a sequence's query tile and key head, with its key tiles) are
 // dealt to the workgroups.  A segment's start and end cost about as much as four tiles per
 // wave, joining parts of it as much again:
-//  - none of more than 32 tiles, 600 times the longest in all, and no parts of shared keys
-//    to join: a wave takes a segment
+//  - none of more than 32 tiles (with shared keys' parts, which a wave alone joins slowly, 8;
+//    past 128 columns never), and 600 times the longest in all: a wave takes a segment
 //    alone, so that the starts of four run at once and nothing is joined (us, alone / by
 //    a workgroup's waves together; 128 columns: 256 sequences x 8 heads x 300 keys
 //    66.7 / 82.2, 128 x 8 x 616 63.4 / 65.3, 300 x 8 of 37 to 600 keys 72 / 123; 64
 //    columns: 256 x 16 x 60 27 / 62, 40 x 16 x 200 (640 segments) 14.4 / 18.2; not 64 x 8 x 300
-//    at 128 columns (512 segments) 23.3 / 20.5, where a wave's own latency counts);
+//    at 128 columns (512 segments) 23.3 / 20.5, where a wave's own latency counts; behind 2048
+//    shared keys, 256 x 16 x 52 of 64 columns 54 / 93, 256 x 8 x 52 of 128 55 / 71, but 113 x 12 x
+//    30 of 256 columns 151 / 92);
 //  - no segment of more than 16 tiles: all whole;
 //  - at least 40 tiles per resident workgroup: the tiles of all segments are one line, cut
 //    into an equal chunk for each, wherever the cuts fall (128 segments of 125 tiles, 31 per
@@ -180,6 +182,7 @@ constexpr uint32_t kMostResident = 512;  // workgroups on the chip at most (Deco
 //    about one per CU (two make twice the parts to join: 8 segments of 500 tiles 24.5 us
 //    against 21.6, 32 of 66 18.2 against 16.1).
 // The line's units are tiles (part_tiles = 0) or parts of at most part_tiles tiles.
+constexpr uint32_t kAloneTiles = 32, kAloneShared = 8;
 struct Shares {
   uint32_t part_tiles;
   uint64_t chunk;  // units per workgroup, or per wave
@@ -193,10 +196,10 @@ struct Shares {
   }
 };
 __device__ __forceinline__ Shares share_out(uint64_t tiles, uint64_t segments, uint32_t longest, uint32_t groups,
-                                            uint32_t resident, bool may_split, bool may_alone) {
-  constexpr uint32_t kAloneTiles = 32, kAloneSegments = 600;
+                                            uint32_t resident, bool may_split, uint32_t alone_tiles) {
+  constexpr uint32_t kAloneSegments = 600;
   constexpr uint32_t kWholeTiles = 16, kLeastTiles = 8, kChunkTiles = 40, kCus = 256;
-  if (may_alone && longest <= kAloneTiles && (uint64_t)longest * kAloneSegments <= tiles) {
+  if (longest <= alone_tiles && (uint64_t)longest * kAloneSegments <= tiles) {
     const uint32_t waves = groups * kWaves;
     return {0xffffffffu, quotient(segments + waves - 1, waves), segments, true};
   }
@@ -260,10 +263,13 @@ __device__ __forceinline__ Units units_of(const BatchSequence& q, uint32_t group
   return u;
 }
 
-template <int D, int MT>
+// Shared: the keys from first_key on, joined with the parts of those before it.
+template <int D, int MT, bool Shared>
 __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_pages_decode_kernel(
-    PagedAttentionArgs a, float scale_log2, uint32_t first_key, uint32_t few, DecodeSplit split,
-    SharedParts shared) {
+    PagedAttentionArgs a, float scale_log2, uint32_t keys_from, uint32_t few, DecodeSplit split,
+    SharedParts given) {
+  const uint32_t first_key = Shared ? keys_from : 0;
+  const SharedParts shared = Shared ? given : SharedParts{nullptr, nullptr, 0};
   using C = Decode<D, MT>;
   constexpr uint32_t kKeys = C::kKeys, kKT = C::kKT, kKS = C::kKS, kDT = C::kDT, kHalves = C::kHalves;
   constexpr uint32_t kQueries = C::kQueries, kTile = C::kTileBytes, kRowBytes = C::kRowBytes;
@@ -274,7 +280,8 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
   __shared__ float wave_sums[kWaves][kQueries][2];
   // Weights of a query's parts and their sums: the waves' and the shared keys'.  Where a
   // segment of several workgroups is merged, its parts' and the shared keys', in the stages.
-  constexpr uint32_t kFewParts = kWaves + kMaxSharedParts, kManyParts = kMaxParts + kMaxSharedParts;
+  constexpr uint32_t kShared = Shared ? kMaxSharedParts : 0;
+  constexpr uint32_t kFewParts = kWaves + kShared, kManyParts = kMaxParts + kShared;
   __shared__ float few_weights[kQueries * kFewParts], few_sums[kQueries * kFewParts];
   static_assert(kQueries * kManyParts * 4 <= kWaves * kTile, "the weights of a merge fit a stage");
   __shared__ uint32_t arrived;
@@ -302,7 +309,7 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
   longest = largest(longest);
   if (segments == 0) return;
   const Shares shares = share_out(tiles, segments, longest, gridDim.x, C::kResident, split.rows != nullptr,
-                                  shared.parts == 0);
+                                  !Shared ? kAloneTiles : D <= 128 ? kAloneShared : 0);
   auto line_units = [&](const Units& u) __attribute__((always_inline)) { return u.segments * shares.units(u.tiles); };
   auto units_in = [&](uint32_t s) __attribute__((always_inline)) { return line_units(units_at(s)); };
   UnitLine line{scan(line_units(held)), 0};
@@ -571,13 +578,67 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
       const uint32_t row = (query0 + m) / group;
       return (uint64_t)(q.first + row) * a.query_heads + key_head * group + (query0 + m - row * group);
     };
-    if (alone) {  // nothing to join
+    if (alone) {  // nothing to join but the shared keys' parts
 #pragma unroll
       for (uint32_t mt = 0; mt < MT; ++mt) {
         const uint32_t m = 16 * mt + r16;
         const uint64_t at = output_row(m < queries ? m : queries - 1);
         const float l = sum_of_query(l_run[mt]);
-        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+        float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+        if constexpr (Shared && D <= 128) {
+          // A query's four lanes hold every fourth part's weight.
+          constexpr uint32_t kHeld = kMaxSharedParts / 4, kAtOnce = MT == 1 ? 4 : 2;
+          float w[kHeld], sums[kHeld], top = m_run[mt], sum = 0.0f;
+#pragma unroll
+          for (uint32_t j = 0; j < kHeld; ++j) {
+            const uint32_t z = 4 * j + g4;
+            const float* pair = shared.sums + (at * shared.parts + (z < shared.parts ? z : 0)) * 2;
+            w[j] = pair[0];
+            sums[j] = pair[1];
+          }
+#pragma unroll
+          for (uint32_t j = 0; j < kHeld; ++j) {
+            w[j] = 4 * j + g4 < shared.parts ? w[j] : -INFINITY;
+            top = fmaxf(top, w[j]);
+          }
+          top = max_of_query(top);
+          top = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+          for (uint32_t j = 0; j < kHeld; ++j) {
+            w[j] = __builtin_amdgcn_exp2f(w[j] - top);
+            sum += 4 * j + g4 < shared.parts ? w[j] * sums[j] : 0.0f;
+          }
+          const float own = __builtin_amdgcn_exp2f(m_run[mt] - top);
+          sum = sum_of_query(sum) + own * l;
+          inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+          for (uint32_t dt = 0; dt < kDT; ++dt) o[dt][mt] *= own;
+          const float* from = shared.rows + at * shared.parts * a.width;
+#pragma unroll
+          for (uint32_t j = 0; j < kHeld; ++j)
+#pragma unroll
+            for (uint32_t z0 = 0; z0 < 4; z0 += kAtOnce) {  // parts, whose loads are in flight together
+              if (4 * j + z0 >= shared.parts) break;
+              float4_t y[kAtOnce][kDT];
+#pragma unroll
+              for (uint32_t k = 0; k < kAtOnce; ++k) {
+                const uint32_t z = 4 * j + z0 + k < shared.parts ? 4 * j + z0 + k : shared.parts - 1;
+#pragma unroll
+                for (uint32_t dt = 0; dt < kDT; ++dt) {
+                  const uint32_t d = 16 * dt + 4 * g4;
+                  y[k][dt] = *reinterpret_cast<const float4_t*>(from + z * a.width + (d < a.width ? d : 0));
+                }
+              }
+#pragma unroll
+              for (uint32_t k = 0; k < kAtOnce; ++k) {
+                const float weight = __shfl(w[j], 16 * (z0 + k) + r16, kWave);
+                if (4 * j + z0 + k < shared.parts) {
+#pragma unroll
+                  for (uint32_t dt = 0; dt < kDT; ++dt) o[dt][mt] += y[k][dt] * weight;
+                }
+              }
+            }
+        }
 #pragma unroll
         for (uint32_t dt = 0; dt < kDT; ++dt) {
           const uint32_t d = 16 * dt + 4 * g4;
@@ -745,7 +806,7 @@ struct DecodeLaunch {
   uint32_t few;
   SharedParts shared;
 };
-template <int D, int MT>
+template <int D, int MT, bool Shared>
 int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
   constexpr uint64_t kResident = Decode<D, MT>::kResident, kQueries = Decode<D, MT>::kQueries;
   constexpr uint64_t kSlotBytes = kQueries * (D + 2) * sizeof(float);
@@ -766,24 +827,29 @@ int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scal
       split.counters = a.workspace.counters;
     }
   }
-  hipLaunchKernelGGL((attention_pages_decode_kernel<D, MT>), dim3((uint32_t)groups), dim3(kThreads), 0, stream,
+  hipLaunchKernelGGL((attention_pages_decode_kernel<D, MT, Shared>), dim3((uint32_t)groups), dim3(kThreads), 0, stream,
                      a, scale_log2, l.first_key, l.few, split, l.shared);
   return hip_status(hipGetLastError());
 }
-template <int D>
+template <int D, bool Shared>
 int launch_decode_queries(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
   // Two tiles of queries at 256 columns do not fit the registers.
   if constexpr (D <= 128)
-    if ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16) return launch_decode_as<D, 2>(stream, a, scale_log2, l);
-  return launch_decode_as<D, 1>(stream, a, scale_log2, l);
+    if ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16) return launch_decode_as<D, 2, Shared>(stream, a, scale_log2, l);
+  return launch_decode_as<D, 1, Shared>(stream, a, scale_log2, l);
+}
+template <bool Shared>
+int launch_decode_width(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
+  if (a.width > 192) return launch_decode_queries<256, Shared>(stream, a, scale_log2, l);
+  if (a.width > 128) return launch_decode_queries<192, Shared>(stream, a, scale_log2, l);
+  if (a.width > 96) return launch_decode_queries<128, Shared>(stream, a, scale_log2, l);
+  if (a.width > 64) return launch_decode_queries<96, Shared>(stream, a, scale_log2, l);
+  if (a.width > 32) return launch_decode_queries<64, Shared>(stream, a, scale_log2, l);
+  return launch_decode_queries<32, Shared>(stream, a, scale_log2, l);
 }
 int launch_decode(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
-  if (a.width > 192) return launch_decode_queries<256>(stream, a, scale_log2, l);
-  if (a.width > 128) return launch_decode_queries<192>(stream, a, scale_log2, l);
-  if (a.width > 96) return launch_decode_queries<128>(stream, a, scale_log2, l);
-  if (a.width > 64) return launch_decode_queries<96>(stream, a, scale_log2, l);
-  if (a.width > 32) return launch_decode_queries<64>(stream, a, scale_log2, l);
-  return launch_decode_queries<32>(stream, a, scale_log2, l);
+  return l.shared.parts > 0 ? launch_decode_width<true>(stream, a, scale_log2, l)
+                            : launch_decode_width<false>(stream, a, scale_log2, l);
 }
 
 // Queries of a key head (rows x query heads) up to which a sequence is the decode kernel's.

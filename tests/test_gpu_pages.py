@@ -426,6 +426,11 @@ ONCE = [
     (260, 1, 1500, 4, 1, 256, 64, 1455),
     (100, 2, 3300, 12, 4, 128, 8, 3296),
     (500, 1, 300, 64, 32, 32, 16, 288),
+    # Many with few keys of their own: a wave takes a segment and joins its parts.
+    (600, 1, 1003, 16, 4, 64, 16, 1000),
+    (400, 2, 700, 64, 4, 96, 32, 690),
+    (400, 1, 900, 8, 8, 128, 16, 890),
+    (300, 1, 600, 12, 12, 72, 8, 590),
 ]
 
 
