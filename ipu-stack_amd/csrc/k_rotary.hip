@@ -392,7 +392,7 @@ inline Plan plan_rows(uint32_t rows, uint32_t heads, uint32_t width, uint32_t ro
   const uint32_t slots = kThreads / p.lanes;
   uint32_t most = half > 0 && kMaxRows > 2048 / half ? 2048 / half : kMaxRows;  // 16 KiB of angles
   if (heads > 4 * slots) most = 1;
-  if (most > rows / 1024) most = rows / 1024 > least ? rows / 1024 : least;
+  if (rows / 1024 >= least && most > rows / 1024) most = rows / 1024;
   // Busy parts of rows x heads on turns of slots, compared crosswise.
   auto turns = [&](uint32_t r) { return (r * heads + slots - 1) / slots; };
   p.rows = least < most ? least : most;

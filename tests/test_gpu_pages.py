@@ -73,6 +73,8 @@ def append64(b, cache, keys, values, f, magnitude, rotary_width, interleaved):
     ([9], [2000], 1, 2048, 2048, 0, 16, 0),
     ([1] * 70 + [0] * 5 + [2] * 60, [9] * 70 + [0] * 5 + [33] * 60, 2, 96, 24, 0, 16, 0),
     ([1] * 4200, [3] * 4200, 1, 32, 32, 1, 2, 2),
+    ([300] * 130, [311] * 130, 1, 8, 4, 0, 16, 5),
+    ([700] * 9, [900] * 9, 3, 40, 20, 0, 64, 1),
 ])
 def test_append(ipus, ctx, rows, lengths, heads, width, rotary_width, interleaved, page_rows, pad):
     b = Batch(np.random.default_rng(width), rows, lengths, page_rows, pad)

@@ -33,6 +33,11 @@ SHAPES = [
     (1, 1, 2, 2), (1, 16, 128, 128), (5, 3, 128, 64), (4100, 2, 64, 64), (1100, 12, 72, 72),
     (33, 5, 72, 18), (7, 40, 80, 40), (9, 2, 96, 24), (3, 2, 2048, 2048), (2, 3, 1000, 500),
     (6, 4, 65, 10), (6, 3, 67, 6), (3, 300, 32, 32), (2050, 17, 32, 16), (3, 2, 24, 0),
+    # Many rows per workgroup: up to 32, and the most that the rows leave.
+    (40000, 1, 16, 8),
+    (33000, 3, 32, 32),
+    (2600, 5, 72, 72),
+    (5003, 33, 64, 16),
 ]
 
 
