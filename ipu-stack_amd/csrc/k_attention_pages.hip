@@ -866,6 +866,9 @@ constexpr uint32_t kFewBeside = 16;
 // single ones, 128 columns, 32 query heads on 8: 17 sequences x 256 keys 12.9 / 23.8, x 1000
 // 27.8 / 47.9, x 2000 32.1 / 48.2, 65 x 1000 54 / 71; not 17 x 4000 84 / 79, nor 257 x 128 (2056
 // segments) 53 / 43; of 64 columns, 16 heads: 65 x 1000 60 / 66, 120 x 1000 (1920) 102 / 98).
+// So it is with sequences of 17 to 32 queries alone (24 queries, one launch of blocks / decode:
+// 64 x 8 segments x 128 keys x 128 13.2 / 30.9, x 500 27.7 / 44.4, x 1000 54 / 70, 16 x 8 x 2000
+// 32 / 36), but not of up to 16 (64 x 16 x 200 x 64 21.8 / 16.0).
 constexpr uint32_t kShortReach = 2560, kShortSegments = 1280;
 
 // The shared keys in a launch of their own: their parts in the workspace's lower
@@ -914,7 +917,9 @@ int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a) {
     return launch_general(stream, a, scale_log2);
   const uint64_t queries = (uint64_t)a.max_rows * (a.query_heads / a.key_heads);
   const DecodeLaunch unshared{0, ~0u, {nullptr, nullptr, 0}};
-  if (queries <= kFewQueries) {
+  const bool small = (uint64_t)a.batch.table_columns * a.batch.page_rows <= kShortReach &&
+                     (uint64_t)a.batch.sequences * a.key_heads <= kShortSegments;
+  if (queries <= (small && a.batch.shared_rows == 0 ? kFewBeside : kFewQueries)) {
     SharedParts parts;
     Workspace rest;
     if (plan_shared(a, &parts, &rest)) {
@@ -927,9 +932,7 @@ int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a) {
   }
   // Sequences of many rows, and those of few beside them, of which there are none
   // where every sequence has max_rows.
-  if ((uint64_t)a.batch.sequences * a.max_rows == a.rows) return launch_attention_blocks(stream, a, scale_log2, 0);
-  if ((uint64_t)a.batch.table_columns * a.batch.page_rows <= kShortReach &&
-      (uint64_t)a.batch.sequences * a.key_heads <= kShortSegments)
+  if (small || (uint64_t)a.batch.sequences * a.max_rows == a.rows)
     return launch_attention_blocks(stream, a, scale_log2, 0);
   if (int e = launch_attention_blocks(stream, a, scale_log2, kFewBeside)) return e;
   PagedAttentionArgs beside = a;

@@ -181,6 +181,12 @@ DECODE = [
     ([1] * 2, [90, 5], 3, 1, 65, 2, 0),
     ([2], [40], 2, 1, 1000, 16, 0),
     ([3, 4], [50, 10], 6, 3, 40, 16, 0),
+    # 17 to 32 queries of a key head: short tables, and long ones (two tiles).
+    ([3, 1, 0, 2], [300, 40, 0, 65], 16, 2, 128, 16, 1),
+    ([3, 1, 0, 2], [300, 4000, 0, 65], 16, 2, 128, 16, 1),
+    ([2, 2], [2700, 31], 14, 1, 96, 64, 0),
+    ([4], [5000], 6, 1, 64, 128, 0),
+    ([2] * 3, [2600, 1, 100], 28, 2, 32, 8, 2),
 ]
 
 
