@@ -23,6 +23,8 @@
  *     own for launches that merge partial results (allocated with it, outside
  *     ipus_context_live_buffers).
  *   - Launches are ordered on the context's stream (replacing BSP phases).
+ *     Threads may share a context: the launches of one call, of a session's run
+ *     and of a capture stand together, whatever other threads enqueue.
  *   - Every call returns 0 on success or a negative IPUS_ERROR_* code;
  *     ipus_last_error() returns the message of the calling thread's last
  *     failure.  HIP runtime failures map to IPUS_ERROR_HIP_BASE - hipError_t.

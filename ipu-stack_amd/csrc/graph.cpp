@@ -1484,6 +1484,7 @@ int launch_steps(ipus_session* s) {
 extern "C" int ipus_session_run(ipus_session* s) {
   if (!s) return fail(IPUS_ERROR_INVALID_ARGUMENT, "null session");
   if (int status = use_device(s->ctx)) return status;
+  std::lock_guard<std::recursive_mutex> lock(s->ctx->enqueue_mutex);
   // The captured graph splits reductions through the context's workspace, so it
   // only runs on the context's stream; a caller that records the stream gets
   // the steps themselves, which do without (context_workspace).
@@ -1496,8 +1497,11 @@ extern "C" int ipus_session_run(ipus_session* s) {
 
 extern "C" int ipus_session_capture(ipus_session* s) {
   if (!s) return fail(IPUS_ERROR_INVALID_ARGUMENT, "null session");
-  if (s->exec || s->pkg->steps.empty()) return 0;
+  if (s->pkg->steps.empty()) return 0;
   if (int status = use_device(s->ctx)) return status;
+  // Other threads' launches wait: on a stream that is being captured they would be recorded.
+  std::lock_guard<std::recursive_mutex> lock(s->ctx->enqueue_mutex);
+  if (s->exec) return 0;
   hipStream_t stream = s->ctx->stream;
   hipError_t e = hipStreamBeginCapture(stream, hipStreamCaptureModeThreadLocal);
   if (e != hipSuccess) return hip_fail(e, "hipStreamBeginCapture");

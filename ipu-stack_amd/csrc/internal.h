@@ -28,6 +28,11 @@ struct ipus_context {
   // buffers above.
   void* workspace = nullptr;
   uint32_t* workspace_counters = nullptr;
+  // Held while a call enqueues its launches on the stream: by ipus_launch (some
+  // operators are two launches with parts in the workspace between them), by a
+  // session's replay, and over the whole of ipus_session_capture, whose steps come
+  // through ipus_launch again.
+  std::recursive_mutex enqueue_mutex;
   // ipus_session_capture is recording this context's stream into a graph
   // that will only be launched on it.
   std::atomic<bool> capturing_session{false};
@@ -36,8 +41,9 @@ struct ipus_context {
 namespace ipus {
 
 struct Workspace;
-// The context's workspace, for a launch on its stream: launches there run one
-// after the other, whichever threads enqueue them, so they can share it.
+// The context's workspace, for the launches of one call on its stream.  Launches
+// there run one after the other, and enqueue_mutex, which the caller holds, keeps
+// other threads' launches from coming between those of one call: so all can share it.
 // Empty where the allocation failed, and while a caller records the stream
 // into a graph of its own (which it may launch on other streams, several at
 // once): the unsplit kernels run then.  paged: all of it, for the paged attention.

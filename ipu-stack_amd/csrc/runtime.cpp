@@ -1226,6 +1226,8 @@ extern "C" int ipus_launch(ipus_context* ctx, const char* symbol, void* output,
   for (int k = 0; k < input_count; ++k)
     if (!inputs || !inputs[k])
       return fail(IPUS_ERROR_INVALID_ARGUMENT, "kernel %s: null input %d", symbol, k);
+  // Another thread's launches come before or after all of this call's.
+  std::lock_guard<std::recursive_mutex> lock(ctx->enqueue_mutex);
   if (ctx->inject_status != 0) {
     if (ctx->inject_after == 0) {
       const int status = ctx->inject_status;
