@@ -398,10 +398,13 @@ def rotary_frequencies(rotary_width: int, base: float = 10000.0, scaling: int = 
     """(float32 [rotary_width / 2] rad per position, magnitude) for the rotary
     kernels; ROTARY_LINEAR, _BASE and _BANDED (by the turns over trained_rows)
     reach contexts `factor` times the trained one."""
-    out = np.empty(max(0, int(rotary_width)) // 2, dtype=np.float32)
+    rotary_width = int(rotary_width)
+    if not 0 <= rotary_width < 1 << 32:  # the library's width has 32 bits
+        raise IpusError(ERROR_INVALID_ARGUMENT, f"rotary_width {rotary_width} is not a positive even number")
+    out = np.empty(rotary_width // 2, dtype=np.float32)
     magnitude = ctypes.c_float(0)
     _check(_lib().ipus_rotary_frequencies(
-        out.ctypes.data, ctypes.addressof(magnitude), int(rotary_width), float(base),
+        out.ctypes.data, ctypes.addressof(magnitude), rotary_width, float(base),
         int(scaling), float(factor), float(trained_rows), float(slow_turns), float(fast_turns)))
     return out, magnitude.value
 

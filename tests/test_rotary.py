@@ -53,6 +53,14 @@ def test_frequencies_refuse(ipus, arguments):
     assert e.value.status == ipus.ERROR_INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("rotary_width", [-2, -1, -(2 ** 32) + 8, 2 ** 32, 2 ** 32 + 8])
+def test_frequencies_refuse_widths_past_32_bits(ipus, rotary_width):
+    """They would wrap to a width that the array was not made for."""
+    with pytest.raises(ipus.IpusError) as e:
+        ipus.rotary_frequencies(rotary_width)
+    assert e.value.status == ipus.ERROR_INVALID_ARGUMENT and str(rotary_width) in e.value.message
+
+
 def test_frequencies_null(ipus):
     assert ipus._lib().ipus_rotary_frequencies(None, None, 8, 10000.0, 0, 1.0, 0.0, 0.0, 0.0) == \
         ipus.ERROR_INVALID_ARGUMENT
