@@ -522,8 +522,9 @@ int run_norm_rotary(ipus_context* c, void* o, const void* const* i, const uint32
   RotaryArgs a;
   a.out = o;
   a.input = i[0];
-  a.query_weight = i[1];
-  a.key_weight = i[2];
+  // The weight of a group without heads is not read: the other's stands in for it.
+  a.query_weight = i[s[1] > 0 ? 1 : 2];
+  a.key_weight = i[s[2] > 0 ? 2 : 1];
   a.positions = (const int*)i[3];
   a.frequencies = (const float*)i[4];
   a.rows = s[0];

@@ -7,6 +7,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <atomic>
 #include <chrono>
 #include <mutex>
 #include <string>
@@ -20,6 +21,7 @@ struct Entry {
   std::string what;     // "launch", "replay", "begin", "end"
   std::thread::id by;
   dim3 grid;
+  const void* kernel;
   std::vector<char> first;  // bytes of a kernel's first argument
 };
 inline std::mutex log_mutex;
@@ -32,8 +34,8 @@ inline std::atomic<bool> stream_captured{false};
 inline int failures = 0;
 #define CHECK(x) do { if (!(x)) { printf("line %d: %s\n", __LINE__, #x); ++failures; } } while (0)
 
-inline void record(const char* what, dim3 grid = dim3(), const void* first = nullptr) {
-  Entry e{what, std::this_thread::get_id(), grid, {}};
+inline void record(const char* what, dim3 grid = dim3(), const void* kernel = nullptr, const void* first = nullptr) {
+  Entry e{what, std::this_thread::get_id(), grid, kernel, {}};
   if (first && first_bytes) e.first.assign((const char*)first, (const char*)first + first_bytes);
   {
     std::lock_guard<std::mutex> lock(log_mutex);
@@ -68,8 +70,8 @@ void** __hipRegisterFatBinary(const void*) {
 void __hipRegisterFunction(void**, const void*, char*, const char*, unsigned, void*, void*, dim3*, dim3*, int*) {}
 void __hipRegisterVar(void**, void*, char*, char*, int, size_t, int, int) {}
 void __hipUnregisterFatBinary(void**) {}
-hipError_t hipLaunchKernel(const void*, dim3 grid, dim3, void** args, size_t, hipStream_t) {
-  record("launch", grid, args ? args[0] : nullptr);
+hipError_t hipLaunchKernel(const void* kernel, dim3 grid, dim3, void** args, size_t, hipStream_t) {
+  record("launch", grid, kernel, args ? args[0] : nullptr);
   return hipSuccess;
 }
 hipError_t hipGetDeviceCount(int* n) { return *n = 1, hipSuccess; }

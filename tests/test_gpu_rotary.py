@@ -132,6 +132,34 @@ def test_norm_rotary(ipus, ctx, rows, heads, width, rotary_width, interleaved, d
         b.free()
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("width", [128, 2048, 65])
+@pytest.mark.parametrize("query,key", [(3, 0), (0, 3)])
+def test_norm_rotary_of_one_group(ipus, ctx, dtype, width, query, key):
+    """The weight of the group without heads is anything but null, at any address."""
+    rows, heads = 5, 3
+    x = values(ipus, rows * heads * width, 6, dtype)
+    w = (1 + 0.2 * values(ipus, width, 7, np.float32)).astype(dtype)
+    f, _ = ipus.rotary_frequencies(64)
+    bufs = [ctx.upload(a) for a in (x, w, np.arange(rows, dtype=np.int32), f)]
+    other = ctx.upload(np.full(2 * width + 8, np.nan, dtype))
+    got = []
+    for unused in (bufs[1].ptr, other.ptr + 1):
+        out = ctx.alloc(x.nbytes)
+        weights = [bufs[1], unused] if query else [unused, bufs[1]]
+        ctx.launch(symbol("norm_rotary", dtype), out, [bufs[0], *weights, *bufs[2:]],
+                   [rows, query, key, width, 64, 0, heads * width, heads * width, bits(1e-6), 0])
+        got.append(out.download(np.uint8))
+        out.free()
+    assert np.array_equal(got[0], got[1])
+    want, bound = norm_rotate(x.astype(np.float64).reshape(rows, heads, width), w.astype(np.float64),
+                              float(np.float32(1e-6)), np.arange(rows), f, 1.0, 64, False)
+    result = got[1].view(dtype).astype(np.float64).reshape(want.shape)
+    assert np.all(np.abs(result - want) <= rounded(want, bound, dtype))
+    for b in bufs + [other]:
+        b.free()
+
+
 def test_norm_of_zeros_and_large_values(ipus, ctx):
     """A head of zeros stays zero, one at fp16's end does not overflow."""
     width = 128

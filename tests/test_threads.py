@@ -5,7 +5,6 @@ from __future__ import annotations
 from host_programs import run_program
 
 SOURCE = r"""
-#include <atomic>
 #include "host_runtime.h"
 static char memory[1 << 16];
 static ipus_context* ctx;
