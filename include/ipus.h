@@ -20,8 +20,8 @@
  * Conventions (kernel.rs:14-16, crates/ipu-codegen/src/operator.rs:467-537):
  *   - The caller owns every buffer.  Kernels read inputs and write the output
  *     and allocate nothing.  A context holds 96 MiB of device memory of its
- *     own for launches that merge partial results (allocated with it, outside
- *     ipus_context_live_buffers).
+ *     own (32 MiB where there is no room for more) for launches that merge
+ *     partial results (allocated with it, outside ipus_context_live_buffers).
  *   - Launches are ordered on the context's stream (replacing BSP phases).
  *     Threads may share a context: the launches of one call, of a session's run
  *     and of a capture stand together, whatever other threads enqueue.

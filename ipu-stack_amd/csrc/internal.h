@@ -27,6 +27,7 @@ struct ipus_context {
   // (context_workspace): allocated with the context, not counted among the
   // buffers above.
   void* workspace = nullptr;
+  size_t workspace_bytes = 0;
   uint32_t* workspace_counters = nullptr;
   // Held while a call enqueues its launches on the stream: by ipus_launch (some
   // operators are two launches with parts in the workspace between them), by a

@@ -49,7 +49,7 @@ int use_device(const ipus_context* ctx) {
 
 // Partial results of one launch at most (a launch that would need more runs
 // unsplit), and a counter per group of workgroups that merges.  Paged attention
-// may use all of it: rows over a shared prefix in 16 parts (128 sequences x 32 heads x
+// may use all that the context has: rows over a shared prefix in 16 parts (128 sequences x 32 heads x
 // 128 columns: 34 MB) beside the parts of the keys behind it.
 constexpr size_t kWorkspaceBytes = 32u << 20;
 constexpr size_t kPagedWorkspaceBytes = 96u << 20;
@@ -65,7 +65,7 @@ Workspace context_workspace(const ipus_context* ctx, bool paged) {
   if (!ctx->workspace) return w;
   if (!ctx->capturing_session.load(std::memory_order_relaxed) && stream_recorded(ctx)) return w;
   w.data = ctx->workspace;
-  w.bytes = paged ? kPagedWorkspaceBytes : kWorkspaceBytes;
+  w.bytes = paged ? ctx->workspace_bytes : kWorkspaceBytes;
   w.counters = ctx->workspace_counters;
   w.counter_count = kWorkspaceCounters;
   return w;
@@ -140,19 +140,22 @@ extern "C" int ipus_context_create(int device, ipus_context** out) {
     return fail(status, "device %d: looking up the split-K scratch array failed (%d)", device,
                 status);
   }
-  // The kernels' workspace, its counters at 0.  Without it (no memory left)
-  // every launch still runs, unsplit.
-  void* ws = nullptr;
-  if (hipMalloc(&ws, kPagedWorkspaceBytes + kWorkspaceCounters * sizeof(uint32_t)) == hipSuccess) {
-    uint32_t* counters = (uint32_t*)((uint8_t*)ws + kPagedWorkspaceBytes);
+  // The kernels' workspace, its counters at 0: all of it, where there is no memory for
+  // that what the other kernels use, and without any every launch still runs, unsplit.
+  for (size_t bytes : {kPagedWorkspaceBytes, kWorkspaceBytes}) {
+    void* ws = nullptr;
+    if (hipMalloc(&ws, bytes + kWorkspaceCounters * sizeof(uint32_t)) != hipSuccess) continue;
+    uint32_t* counters = (uint32_t*)((uint8_t*)ws + bytes);
     e = hipMemsetAsync(counters, 0, kWorkspaceCounters * sizeof(uint32_t), ctx->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     if (e == hipSuccess) {
       ctx->workspace = ws;
+      ctx->workspace_bytes = bytes;
       ctx->workspace_counters = counters;
     } else {
       (void)hipFree(ws);
     }
+    break;
   }
   (void)hipGetLastError();
   *out = ctx;
