@@ -545,9 +545,11 @@ int run_norm_rotary(ipus_context* c, void* o, const void* const* i, const uint32
   return launch_rotary(c->stream, a);
 }
 
-// Rows of a page: a power of two, so that positions split by a shift.
-int check_pages(uint32_t rows, uint32_t key_heads, uint32_t page_rows) {
-  if (rows > 0x7fffffff || key_heads == 0 || key_heads > 32767) return IPUS_ERROR_INVALID_ARGUMENT;
+// Rows of a page: a power of two, so that positions split by a shift.  Sequences: the
+// kernels step over them by 64 in 32 bits, which must not wrap.
+int check_pages(uint32_t sequences, uint32_t rows, uint32_t key_heads, uint32_t page_rows) {
+  if (sequences > 0x7fffffff || rows > 0x7fffffff) return IPUS_ERROR_INVALID_ARGUMENT;
+  if (key_heads == 0 || key_heads > 32767) return IPUS_ERROR_INVALID_ARGUMENT;
   if (page_rows == 0 || page_rows > 65536 || (page_rows & (page_rows - 1)) != 0)
     return IPUS_ERROR_INVALID_ARGUMENT;
   return 0;
@@ -572,7 +574,7 @@ PagedBatch paged_batch(const void* table, const void* row_offsets, const void* l
 // interleaved, magnitude_bits, pages, page_rows, table_columns.
 int check_append(const uint32_t* s) {
   if (int e = check_rotation(s[3], s[6], s[7], s[8])) return e;
-  return check_pages(s[1], s[2], s[10]);
+  return check_pages(s[0], s[1], s[2], s[10]);
 }
 int run_append(ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
   AppendArgs a;
@@ -596,7 +598,7 @@ int run_append(ipus_context* c, void* o, const void* const* i, const uint32_t* s
 // pages, page_rows, table_columns, causal, scale_bits[, shared_rows].
 constexpr uint32_t kMaxPagedWidth = 1024;
 int check_attention_pages(const uint32_t* s) {
-  if (int e = check_pages(s[1], s[4], s[8])) return e;
+  if (int e = check_pages(s[0], s[1], s[4], s[8])) return e;
   if (s[3] == 0 || s[3] > 65535 || s[3] % s[4] != 0 || s[5] == 0 || s[10] > 1)
     return IPUS_ERROR_INVALID_ARGUMENT;
   const float scale = bits_or(s[11], 1.0f);

@@ -132,3 +132,18 @@ def test_head_major_outputs_are_accepted(ipus):
         ipus.validate_kernel_run("ipu_stack_rotary_f16", 3, scalars)
     with pytest.raises(ipus.IpusError):
         ipus.validate_kernel_run("ipu_stack_rotary_f16", 3, [4, 2, 64, 32, 0, 0, 0, 64, 255, 0])
+
+
+@pytest.mark.parametrize("symbol", ["ipu_stack_append_pages_f16", "ipu_stack_attention_pages_f16",
+                                    "ipu_stack_attention_shared_pages_f16"])
+def test_sequences_past_31_bits_are_refused(ipus, symbol):
+    """Sequence numbers that steps of 64 in 32 bits would pass without end."""
+    inputs, scalars = GOOD[symbol]
+    for sequences, good in ((0x7fffffff, True), (0x80000000, False), (0xffffffff, False)):
+        changed = [sequences] + scalars[1:]
+        if good:
+            ipus.validate_kernel_run(symbol, inputs, changed)
+            continue
+        with pytest.raises(ipus.IpusError) as e:
+            ipus.validate_kernel_run(symbol, inputs, changed)
+        assert e.value.status == ipus.ERROR_INVALID_ARGUMENT
