@@ -217,7 +217,8 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        the cache, page_table, row_offsets, lengths; sequences, rows,
  *        max_rows, query_heads, key_heads (a divisor: query head h reads key
  *        head h / (query_heads / key_heads)), width, query_row_stride, pages,
- *        page_rows, table_columns, causal, scale_bits (0 = 1 / sqrt(width)).
+ *        page_rows, table_columns, causal, scale_bits (0 = 1 / sqrt(width);
+ *        scales by which scores of finite values pass fp32 are refused).
  *        Row i of the n of sequence s reads the keys below lengths[s], when
  *        causal those up to its position lengths[s] - n + i.  Keys without a
  *        page carry no weight; a row whose weights are all zero (no key, or

@@ -602,7 +602,9 @@ int check_attention_pages(const uint32_t* s) {
   if (s[3] == 0 || s[3] > 65535 || s[3] % s[4] != 0 || s[5] == 0 || s[10] > 1)
     return IPUS_ERROR_INVALID_ARGUMENT;
   const float scale = bits_or(s[11], 1.0f);
-  if (!std::isfinite(scale) || scale <= 0.0f) return IPUS_ERROR_INVALID_ARGUMENT;
+  // The largest score of finite fp16 values, in the kernels' log2 units, must be finite.
+  const float most = 65504.0f * 65504.0f * (float)s[5] * (scale * 1.44269504f);
+  if (!std::isfinite(most) || scale <= 0.0f) return IPUS_ERROR_INVALID_ARGUMENT;
   return s[5] > kMaxPagedWidth ? IPUS_ERROR_UNAVAILABLE : 0;
 }
 int run_attention_pages(ipus_context* c, void* o, const void* const* i, const uint32_t* s,

@@ -147,3 +147,21 @@ def test_sequences_past_31_bits_are_refused(ipus, symbol):
         with pytest.raises(ipus.IpusError) as e:
             ipus.validate_kernel_run(symbol, inputs, changed)
         assert e.value.status == ipus.ERROR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("symbol", ["ipu_stack_attention_pages_f16", "ipu_stack_attention_shared_pages_f16"])
+def test_scales_past_fp32_are_refused(ipus, symbol):
+    """65504^2 * width * scale * log2(e), the largest score, is a finite fp32 value."""
+    inputs, scalars = GOOD[symbol]
+    names = ipus.kernel_abi(symbol).scalar_names
+    for width in (8, 64, 1024):
+        largest = np.finfo(np.float32).max / (65504.0 ** 2 * width * math.log2(math.e))
+        for scale, good in ((2.0 ** -149, True), (largest * 0.999, True), (largest * 1.001, False), (3e38, False)):
+            changed = list(scalars)
+            changed[names.index("width")], changed[names.index("scale_bits")] = width, bits(scale)
+            if good:
+                ipus.validate_kernel_run(symbol, inputs, changed)
+                continue
+            with pytest.raises(ipus.IpusError) as e:
+                ipus.validate_kernel_run(symbol, inputs, changed)
+            assert e.value.status == ipus.ERROR_INVALID_ARGUMENT
