@@ -1312,6 +1312,8 @@ extern "C" int ipus_rotary_frequencies(float* frequencies, float* magnitude, uin
                 "banded scaling needs trained_rows > 0 and 0 <= slow_turns < fast_turns");
   const double r = rotary_width;
   if (scaling == IPUS_ROTARY_BASE) base *= std::pow(factor, r / (r - 2.0));
+  if (!std::isfinite(base) || base <= 0.0)
+    return fail(IPUS_ERROR_INVALID_ARGUMENT, "the scaled base does not fit a double");
   for (uint32_t i = 0; i < rotary_width / 2; ++i) {
     double f = std::pow(base, -2.0 * i / r);
     if (scaling == IPUS_ROTARY_LINEAR) f /= factor;
@@ -1321,6 +1323,8 @@ extern "C" int ipus_rotary_frequencies(float* frequencies, float* magnitude, uin
       f *= keep + (1.0 - keep) / factor;
     }
     frequencies[i] = (float)f;
+    if (!std::isfinite(frequencies[i]))
+      return fail(IPUS_ERROR_INVALID_ARGUMENT, "frequency %u does not fit fp32", i);
   }
   *magnitude = scaling == IPUS_ROTARY_BANDED && factor > 1.0 ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
   return 0;

@@ -61,6 +61,18 @@ def test_frequencies_refuse_widths_past_32_bits(ipus, rotary_width):
     assert e.value.status == ipus.ERROR_INVALID_ARGUMENT and str(rotary_width) in e.value.message
 
 
+@pytest.mark.parametrize("arguments", [
+    dict(rotary_width=64, base=1e-300), dict(rotary_width=64, scaling=1, factor=1e-300),
+    dict(rotary_width=4, base=1e200, scaling=2, factor=1e200), dict(rotary_width=4, base=1e-200, scaling=2, factor=1e-200),
+    dict(rotary_width=64, scaling=3, factor=1e-300, trained_rows=4096.0),
+])
+def test_frequencies_that_are_not_finite_are_refused(ipus, arguments):
+    """Each turns some pair by an angle that is not a number."""
+    with pytest.raises(ipus.IpusError) as e:
+        ipus.rotary_frequencies(**arguments)
+    assert e.value.status == ipus.ERROR_INVALID_ARGUMENT
+
+
 def test_frequencies_null(ipus):
     assert ipus._lib().ipus_rotary_frequencies(None, None, 8, 10000.0, 0, 1.0, 0.0, 0.0, 0.0) == \
         ipus.ERROR_INVALID_ARGUMENT
