@@ -146,7 +146,8 @@ __global__ __launch_bounds__(kThreads) void attention_pages_general_kernel(Paged
 // (v_mfma_f32_16x16x32_f16, fp32 accumulation), as in k_attention.hip.  The probabilities
 // enter the second product as the sum of two fp16 values (22 bits): the matrix pipes have
 // time for it here, and the result is off by little more than its own rounding.  With 32
-// queries per tile they are one fp16 value (2^-11), as in the kernel for many rows.
+// queries per tile they are one fp16 value (2^-11), as in the kernel for many rows, and so
+// are the sums' terms.
 
 // Partial results of a launch: two slots per workgroup, each 16 * MT rows of D fp32
 // and their (reference point, sum) pairs; without memory every segment is one
@@ -492,8 +493,9 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
 #pragma unroll
           for (uint32_t e = 0; e < 8; ++e) {
             const float p = __builtin_amdgcn_exp2f(sc[2 * kk + e / 4][mt][e % 4] - m_use);
-            sum += p;
             high[kk][mt][e] = (half_t)p;
+            // What the second product sees: equal values come out as they are.
+            sum += C::kTwoHalves ? p : (float)high[kk][mt][e];
             low[kk][mt][e] = C::kTwoHalves ? (half_t)(p - (float)high[kk][mt][e]) : (half_t)0.0f;
           }
         l_run[mt] = l_run[mt] * alpha + sum;
