@@ -31,6 +31,11 @@ namespace ipus {
 namespace {
 
 constexpr float kSumLimit = 256.0f;  // as in k_attention.hip
+// A reference point is a score's product with scale_log2, rounded; the probabilities are
+// taken from the products unrounded, by one FMA.  From this point on (log2 units) the rounding
+// alone could make the largest of them overflow or vanish: there they are taken from
+// rounded products, block by block.
+constexpr float kFarPoint = 1 << 24;
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
@@ -223,11 +228,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
 
   float4_t o[kDT][QT];
   float m_run[QT], l_run[QT];  // reference points (log2 units), this lane's share of the row sums
+  float near[QT];              // -m_run, or infinity, with which no block is accepted
   half8_t pp[kHalves][QT];     // fp16 probabilities of the last softmax
 #pragma unroll
   for (uint32_t qt = 0; qt < QT; ++qt) {
     m_run[qt] = -INFINITY;
     l_run[qt] = 0.0f;
+    near[qt] = INFINITY;
 #pragma unroll
     for (uint32_t dt = 0; dt < kDT; ++dt) o[dt][qt] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -356,16 +363,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
           }
       }
     }
-    // Probabilities against the reference points, and this lane's share of their sums.
-    auto exps = [&](const float* neg_m, half8_t (&pf)[kHalves][QT], float* sum) __attribute__((always_inline)) {
+    // Probabilities against the reference points, and this lane's share of their sums, of
+    // scores or (Products) their products.
+    auto exps = [&]<bool Products>(const float* neg_m, half8_t (&pf)[kHalves][QT], float* sum) __attribute__((always_inline)) {
 #pragma unroll
       for (uint32_t qt = 0; qt < QT; ++qt) {
         sum[qt] = 0.0f;
 #pragma unroll
         for (uint32_t kk = 0; kk < kHalves; ++kk) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            pf[kk][qt][e] = (half_t)__builtin_amdgcn_exp2f(fmaf(sc[2 * kk + e / 4][qt][e % 4], scale_log2, neg_m[qt]));
+          for (int e = 0; e < 8; ++e) {
+            const float x = sc[2 * kk + e / 4][qt][e % 4];
+            pf[kk][qt][e] = (half_t)__builtin_amdgcn_exp2f(Products ? x + neg_m[qt] : fmaf(x, scale_log2, neg_m[qt]));
+          }
 #pragma unroll
           for (int e = 0; e < 8; e += 2)
             sum[qt] = __builtin_amdgcn_fdot2(half2_t{pf[kk][qt][e], pf[kk][qt][e + 1]}, half2_t{1, 1}, sum[qt], false);
@@ -374,31 +384,33 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     };
     half8_t pf[kHalves][QT];
     float sum[QT], neg_m[QT];
-#pragma unroll
-    for (uint32_t qt = 0; qt < QT; ++qt) neg_m[qt] = -m_run[qt];
-    exps(neg_m, pf, sum);
+    exps.template operator()<false>(near, pf, sum);
     bool over = false;
 #pragma unroll
     for (uint32_t qt = 0; qt < QT; ++qt) over = over || !(sum[qt] <= kSumLimit);
     if (__any(over)) {
 #pragma unroll
       for (uint32_t qt = 0; qt < QT; ++qt) {
-        float top = sc[0][qt][0];
+        float top = -INFINITY;
 #pragma unroll
-        for (uint32_t kt = 0; kt < kKT; ++kt)
+        for (uint32_t kt = 0; kt < kKT; ++kt) {
+#pragma clang fp contract(off)  // rounded, not one FMA with what follows
+          sc[kt][qt] *= scale_log2;
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[kt][qt][e]);
-        top = max_of_query(top * scale_log2);
+        }
+        top = max_of_query(top);
         const float m_new = fmaxf(m_run[qt], top);
         const float m_use = m_new == -INFINITY ? 0.0f : m_new;  // no NaN from (-inf) - (-inf)
         const float alpha = __builtin_amdgcn_exp2f(m_run[qt] - m_use);
         m_run[qt] = m_new;
+        near[qt] = fabsf(m_new) < kFarPoint ? -m_new : INFINITY;
         neg_m[qt] = -m_use;
         l_run[qt] *= alpha;
 #pragma unroll
         for (uint32_t dt = 0; dt < kDT; ++dt) o[dt][qt] *= alpha;
       }
-      exps(neg_m, pf, sum);
+      exps.template operator()<true>(neg_m, pf, sum);
     }
 #pragma unroll
     for (uint32_t qt = 0; qt < QT; ++qt) l_run[qt] += sum[qt];

@@ -1,5 +1,5 @@
-"""Paged attention at the ends of fp16's range: values whose mean must not pass the
-largest."""
+"""Paged attention at the ends of fp16's range: scores that fp32 holds in steps of
+more than one, and values whose mean must not pass the largest."""
 from __future__ import annotations
 
 import math
@@ -42,6 +42,36 @@ def run(ipus, ctx, b, q, cache, heads, key_heads, width, causal, scale):
     for x in bufs + [out]:
         x.free()
     return got
+
+
+@pytest.mark.parametrize("kernel", sorted(KERNELS))
+@pytest.mark.parametrize("size", [5000.0, 20000.0, -60000.0])
+def test_scores_past_fp32s_whole_steps(ipus, ctx, kernel, size):
+    """Every second key scores the same, up to 2^36 in log2 units, the others far less:
+    a row's output is the mean of the former's values."""
+    rows, lengths, heads, key_heads, width, page_rows, spare, shared = KERNELS[kernel]
+    b = Batch(np.random.default_rng(51), rows, lengths, page_rows, 0, spare, shared)
+    q = np.full((b.rows, heads, width), size, np.float16)
+    cache = np.full((b.pages, 2, key_heads, page_rows, width), np.nan, np.float16)
+    values = ipus.synth_f16(max(lengths) * width, 94, 1, ipus.NORMAL, 1.0).view(np.float16).reshape(-1, width)
+    low, high = (abs(size) * x for x in ((0.5, 1.0) if size > 0 else (1.0, 0.5)))
+    for s in range(b.sequences()):
+        p, page, row = b.places(s)
+        for h in range(key_heads):
+            cache[page, 0, h, row] = np.where(p % 2 == 0, high, low)[:, None]
+            cache[page, 1, h, row] = values[p]
+    got = run(ipus, ctx, b, q, cache, heads, key_heads, width, True, width ** -0.5)
+    sums = np.cumsum(values.astype(np.float64)[::2], axis=0)
+    sizes = np.cumsum(np.abs(values.astype(np.float64))[::2], axis=0)
+    for s in range(b.sequences()):
+        for i in range(b.n[s]):
+            n = (b.k[s] - b.n[s] + i) // 2 + 1  # even keys up to the row's position
+            want, weight = sums[n - 1] / n, sizes[n - 1] / n
+            # Equal weights: the sums over n keys in fp32, the division, the output's rounding.
+            bound = weight * (2 * n + 8) * 2.0 ** -24
+            bound += (np.abs(want) + bound) * 2.0 ** -11 + 2.0 ** -25
+            at = int(b.offsets[s]) + i
+            assert np.all(np.abs(got[at] - want) <= bound), (s, i)
 
 
 @pytest.mark.parametrize("kernel", sorted(KERNELS))
