@@ -140,3 +140,50 @@ def attention(batch, query, cache, key_heads, causal, scale, fp16_probabilities=
             bound[at, h] = ((step + delta + len(p) * 2.0 ** -23) * (w @ np.abs(v))
                             + tiny * (ok @ np.abs(v)) / np.maximum(total, 1.0))
     return out, bound, inside
+
+
+def close_weights(rng, batch, heads, key_heads, width):
+    """Query and cache whose outputs nearly cancel, fp16: keys of nearly equal weights by
+    twos whose values are each other's negatives, so that the output's rounding does
+    not hide what the weights lost.  Rows outside the sequences' keys are NaN."""
+    q = (0.05 * rng.standard_normal((batch.rows, heads, width))).astype(np.float16)
+    cache = np.full((batch.pages, 2, key_heads, batch.page_rows, width), np.nan, np.float16)
+    for s in range(batch.sequences()):
+        p, page, row = batch.places(s)
+        cache[page, 0, :, row] = rng.standard_normal((len(p), key_heads, width)).astype(np.float16)
+        v = (1 + rng.random(((len(p) + 1) // 2, key_heads, width))).astype(np.float16)
+        cache[page, 1, :, row] = np.stack([v, -v], axis=1).reshape(-1, key_heads, width)[:len(p)]
+    return q, cache
+
+
+def weighed(batch, query, cache, key_heads, scale, weights):
+    """Not causal: (output, bound before the last rounding) in float64, the weights as
+    `weights` leaves the probabilities: "exact", "two halves" or "one half".
+
+    The bound of exact and two halves: fp32 scores (`width` products, the scale, the
+    exponential) as in `attention`; the sums of n products and n probabilities in
+    fp32; two halves hold a probability, at most 1, within 2^-22 of itself and 2^-25
+    (the second's subnormal step)."""
+    rows, heads, width = query.shape
+    out, bound = np.zeros(query.shape), np.zeros(query.shape)
+    q64 = query.astype(np.float64)
+    for s in range(batch.sequences()):
+        at = slice(int(batch.offsets[s]), int(batch.offsets[s]) + batch.n[s])
+        _, page, row = batch.places(s)
+        for h in range(heads):
+            k, v = (cache[page, i, h // (heads // key_heads), row].astype(np.float64) for i in (0, 1))
+            x = (q64[at, h] @ k.T) * scale
+            dx = (np.abs(q64[at, h]) @ np.abs(k).T) * scale * (width + 4) * 2.0 ** -24 + np.abs(x) * 2.0 ** -21
+            p = np.exp(x - x.max(axis=1, keepdims=True))
+            total = p.sum(axis=1, keepdims=True)
+            if weights != "exact":
+                high = p.astype(np.float16).astype(np.float64)
+                low = (p - high).astype(np.float16).astype(np.float64) if weights == "two halves" else 0.0
+                out[at, h] = (high + low) @ v / total
+            else:
+                out[at, h] = p @ v / total
+            step, tiny = (2.0 ** -22, 2.0 ** -25) if weights != "exact" else (0.0, 0.0)
+            size = (p @ np.abs(v)) / total
+            bound[at, h] = ((step + 2.0 * dx.max(axis=1, keepdims=True) + len(page) * 2.0 ** -23) * size
+                            + tiny * np.abs(v).sum(axis=0) / total)
+    return out, bound
