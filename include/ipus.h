@@ -227,10 +227,14 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        position or the sequence's length, may hold anything; non-finite
  *        values that it reads make its output non-finite in their columns.
  *        max_rows, the most rows of a sequence (0 = rows), only picks the
- *        kernel.  fp32 scores, maxima and sums; probabilities
- *        are rounded to fp16 for the second product.  width <= 1024; widths
+ *        kernel.  fp32 scores, maxima and sums.  width <= 1024; widths
  *        that are multiples of 8 up to 256 with 16-byte aligned pointers and
- *        strides run on the matrix units.
+ *        strides run on the matrix units.  There the second product takes
+ *        probabilities to 22 bits where max_rows x the query heads of a key
+ *        head are at most 16 (at 97 to 128 columns and tables of more than
+ *        2560 positions 32); it may take them rounded to fp16 where they are
+ *        more, and over shared keys that are read once.  Other widths and
+ *        alignments: fp32.
  *   ipu_stack_attention_shared_pages_f16   the same with shared_rows behind
  *        the scalars: positions below it lie in the pages of the first
  *        sequence's table for every sequence (a shared prompt), and are read

@@ -9,8 +9,10 @@
 // block j - 1 as one MFMA cluster, the softmax of block j behind it, a reference point
 // that moves only when a block's probabilities pass 2^8 against it.  Keys and values lie
 // in pages: a lane holds the page of one of the block's rows, loaded two blocks
-// ahead, and every DMA takes its row's page from the lane that has it.  Row sums are
-// taken in fp32 of the fp16 probabilities that the second product sees.
+// ahead, and every DMA takes its row's page from the lane that has it.  Probabilities are
+// rounded to one fp16 value (2^-11) for the second product, and row sums taken in fp32 of what
+// it sees: a second value for what the first loses would be a half more MFMAs where those bound
+// (4 x 2048 rows against 8192 keys 1304 us against 955, 5 x 796 rows 39.9 against 31.6).
 //
 // A workgroup finds its block by a scan over the sequences; workgroups of one XCD
 // take a contiguous range of blocks, the query blocks of one (sequence, key head)

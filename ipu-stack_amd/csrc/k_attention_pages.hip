@@ -146,8 +146,8 @@ __global__ __launch_bounds__(kThreads) void attention_pages_general_kernel(Paged
 // (v_mfma_f32_16x16x32_f16, fp32 accumulation), as in k_attention.hip.  The probabilities
 // enter the second product as the sum of two fp16 values (22 bits): the matrix pipes have
 // time for it here, and the result is off by little more than its own rounding.  With 32
-// queries per tile they are one fp16 value (2^-11), as in the kernel for many rows, and so
-// are the sums' terms.
+// queries per tile, but for 128 columns, they are one fp16 value (2^-11), as in the kernel
+// for many rows, and so are the sums' terms.
 
 // Partial results of a launch: two slots per workgroup, each 16 * MT rows of D fp32
 // and their (reference point, sum) pairs; without memory every segment is one
@@ -234,8 +234,11 @@ struct Decode {
   // nearly the bandwidth of two (64 sequences x 8 heads x 4096 keys x 128: 191 us against 185); three, where
   // they fit, lose some (96 columns: 167 against 139).
   static constexpr uint32_t kPerCu = D > 128 || (D == 128 && MT == 2) ? 1 : 2;
-  // Probabilities as two fp16 values; with two tiles of queries as one, for the registers.
-  static constexpr bool kTwoHalves = MT == 1;
+  // Probabilities as two fp16 values; with two tiles of queries as one, for the registers,
+  // where a CU holds two workgroups: at 64 and 96 columns the second value spills, at 32 it
+  // costs 6% (64 sequences x 3 rows x 24 heads on 4 x 3000 keys, 30.9 us against 29.2); at 128
+  // nothing (16 x 3 x 64 on 8 x 8000 keys 107.3 against 106.4, 64 x 2000 101.5 against 101.3).
+  static constexpr bool kTwoHalves = MT == 1 || kPerCu == 1;
   static constexpr uint32_t kResident = 256 * kPerCu;
 };
 // 16-byte chunk c of a tile's row r lies at chunk c ^ swizzle(r): the 4 rows x 32 bytes that

@@ -1,5 +1,6 @@
 """How many bits of the probabilities reach the output of paged attention: two fp16 values
-(22 bits) with up to 16 queries of a key head on the matrix units, fp32 in the general kernel."""
+(22 bits) with up to 16 queries of a key head on the matrix units, and up to 32 at 97 to 128
+columns; fp32 in the general kernel."""
 from __future__ import annotations
 
 import struct
@@ -24,6 +25,9 @@ CASES = [
     ([1] * 4, [8, 6, 22, 4], 5, 1, 192, 32, "two halves"),
     ([1] * 4, [10, 4, 12, 28], 16, 2, 256, 16, "two halves"),
     ([1] * 320, [6, 8, 10, 12] * 80, 8, 4, 64, 8, "two halves"),  # a wave for each
+    # 17 to 32 queries, in pages of which few make a long table.
+    ([3, 1, 2], [14, 6, 30], 16, 2, 128, 4096, "two halves"),
+    ([2], [24], 28, 2, 104, 8192, "two halves"),
     ([1] * 5, [8, 2, 16, 30, 12], 4, 2, 65, 16, "exact"),
     ([2, 1], [10, 24], 4, 1, 500, 8, "exact"),
 ]
