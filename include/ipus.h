@@ -211,7 +211,8 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        of page page_table[s][p / page_rows], its key turned by p.  Rows past
  *        row_offsets[sequences], negative positions, positions past the table
  *        and entries outside [0, pages) write nothing.  The offsets do not
- *        decrease; a page that new rows go to belongs to one sequence.
+ *        decrease (nor for the attention below); a page that new rows go to
+ *        belongs to one sequence and stands once in its table.
  *   ipu_stack_attention_pages_f16   out f16 [rows][query_heads][width]; query
  *        f16 (heads side by side, query_row_stride elements from row to row),
  *        the cache, page_table, row_offsets, lengths; sequences, rows,
@@ -237,8 +238,10 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        alignments: fp32.
  *   ipu_stack_attention_shared_pages_f16   the same with shared_rows behind
  *        the scalars: positions below it lie in the pages of the first
- *        sequence's table for every sequence (a shared prompt), and are read
- *        once for many sequences where that pays.
+ *        sequence's table for every sequence (a shared prompt).  They are read
+ *        once for all where that pays, by launches that are not recorded into
+ *        a caller's graph and with max_rows x the query heads of a key head up
+ *        to 32; else by each sequence.
  *   ipu_stack_gelu_tanh_approx_f16     out f16; input f16; element_count
  *        (kernel.rs:1251-1263; count must be even, kernel.rs:1400-1413).
  *   ipu_stack_reduce_sum_f16           out f16; initial, packed remotes f16;

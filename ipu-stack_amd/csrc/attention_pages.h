@@ -22,7 +22,7 @@ inline int hip_status(hipError_t e) { return e == hipSuccess ? 0 : IPUS_ERROR_HI
 // 16 bytes of zeros: what a lane loads for keys that are not to be read and for columns
 // past the width, so that loads need no branch (with branches the compiler cannot count
 // them and waits for all) and nothing that is not the sequence's meets a product.
-__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
+alignas(16) __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // LDS rows of D fp16, 16-byte chunk c of row r at chunk c ^ value_swizzle(r): both the DMA's
 // 64 chunks and ds_read_b64_tr_b16's (4 rows x 32 bytes per 16 lanes) touch every bank once.

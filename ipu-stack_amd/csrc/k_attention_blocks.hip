@@ -24,7 +24,7 @@
 // for blocks and join, 28 in two launches).
 //
 // Measured, causal, 64-row pages (TFLOP/s of the products that the mask leaves): 32 query heads
-// on 8 x 128: 4 x 2048 rows against 8192 keys 930 to 960 us, 1000 to 1040; a prompt of 16384
+// on 8 x 128: 4 x 2048 rows against 8192 keys 945 to 960 us, 1000 to 1020; a prompt of 16384
 // 1030, of 4096 880, of 512 18.7 us; 64 columns 830, 96 910, 256 580 (one tile of queries
 // per wave: four accumulators of 256 columns do not fit beside two).
 #include "attention_pages.h"

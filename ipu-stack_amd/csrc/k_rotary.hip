@@ -16,7 +16,7 @@
 //
 // Measured against a copy's 6.3 TB/s: 16384 rows x 16 heads x 128 fp32 43.5 us (6.2 TB/s);
 // 16384 rows x 40 heads x 128 fp16 with the norm 58.2 us (5.8: the sum over the head stands
-// between its loads and stores); 32000 rows x 8 key heads x 128 into pages 37.0 us (5.4 of the rows
+// between its loads and stores); 32000 rows x 8 key heads x 128 into pages 37.8 us (5.3 of the rows
 // in use: a row's keys and values go to 16 places).  A step of few rows takes 4.2 to 4.5 us,
 // 2.8 to 3.7 of them on the GPU: a launch and four loads that wait for each other.
 #include "../../include/ipus.h"
