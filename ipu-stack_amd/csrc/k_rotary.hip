@@ -23,6 +23,8 @@
 #include "kernels.h"
 #include "pages.h"
 
+#include <type_traits>
+
 namespace ipus {
 namespace {
 
@@ -174,6 +176,14 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, uint32_t
                                                           uint32_t heads_per_block, uint32_t lanes) {
   extern __shared__ float trig[];
   using P = Pack<T, V>;
+  // The squares of fp32 elements and their sum pass fp32 from 2^64 / sqrt(width) on and
+  // vanish below 2^-75: they and their sum are taken in 64 bits, and the elements brought
+  // near 1 by a power of 2 before they meet its root.
+  using Sum = std::conditional_t<std::is_same_v<T, float>, double, float>;
+  struct Inverse {  // root x 2^shift
+    float root;
+    int shift;
+  };
   const uint32_t half = a.rotary_width / 2;
   const uint32_t units = half / V + (a.width - a.rotary_width + 2 * V - 1) / (2 * V);
   const uint32_t row0 = first_row + blockIdx.x * rows_per_block, head0 = blockIdx.y * heads_per_block;
@@ -185,6 +195,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, uint32_t
   T* out = (T*)a.out + (uint64_t)row0 * a.output_row_stride + (uint64_t)head0 * a.output_head_stride;
   const Unit own = unit_at<V, Interleaved>(lane, half, a.width);
   const bool on = lane < units;
+  const float per_element = 1.0f / (float)a.width;
   P xa, xb, wq[2], wk[2];
   auto load = [&](const T* x, const Unit& u, P* pa, P* pb) __attribute__((always_inline)) {
     *pa = *reinterpret_cast<const P*>(x + u.a);
@@ -207,24 +218,29 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, uint32_t
 
   // Squares of a unit's elements.
   auto squares = [&](const Unit& u, const P& pa, const P& pb) __attribute__((always_inline)) {
-    float sum = 0.0f;
+    Sum sum = 0;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      sum = fmaf((float)pa.e[e], (float)pa.e[e], sum);
-      if (u.second) sum = fmaf((float)pb.e[e], (float)pb.e[e], sum);
+      const Sum xa = (Sum)pa.e[e], xb = u.second ? (Sum)pb.e[e] : (Sum)0;
+      sum = __builtin_elementwise_fma(xa, xa, sum);
+      sum = __builtin_elementwise_fma(xb, xb, sum);
     }
     return sum;
   };
   auto finish = [&](const Unit& u, uint32_t index, const P& pa, const P& pb, const P& va, const P& vb,
-                    float inverse, T* y, uint32_t row) __attribute__((always_inline)) {
+                    Inverse inverse, T* y, uint32_t row) __attribute__((always_inline)) {
     float fa[V], fb[V] = {};
     widen(pa, fa);
     if (u.second) widen(pb, fb);
     if (Norm) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        fa[e] = fa[e] * inverse * (float)va.e[e];
-        if (u.second) fb[e] = fb[e] * inverse * (float)vb.e[e];
+        if constexpr (std::is_same_v<Sum, double>) {
+          fa[e] = __builtin_amdgcn_ldexpf(fa[e], inverse.shift);
+          fb[e] = __builtin_amdgcn_ldexpf(fb[e], inverse.shift);
+        }
+        fa[e] = fa[e] * inverse.root * (float)va.e[e];
+        if (u.second) fb[e] = fb[e] * inverse.root * (float)vb.e[e];
       }
     }
     if (u.turned) {
@@ -233,9 +249,15 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, uint32_t
     store_once(y + u.a, narrow<T, V>(fa));
     if (u.second) store_once(y + u.b, narrow<T, V>(fb));
   };
-  auto norm = [&](float sum) __attribute__((always_inline)) {
+  auto norm = [&](Sum sum) __attribute__((always_inline)) {
     for (uint32_t o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
-    return 1.0f / sqrtf(sum / (float)a.width + a.epsilon);
+    if constexpr (std::is_same_v<Sum, float>) {
+      return Inverse{1.0f / sqrtf(sum / (float)a.width + a.epsilon), 0};
+    } else {
+      const double mean = fma(sum, (double)per_element, (double)a.epsilon);
+      const int j = __builtin_amdgcn_frexp_exp(mean) >> 1;
+      return Inverse{1.0f / sqrtf((float)__builtin_amdgcn_ldexp(mean, -2 * j)), -j};
+    }
   };
 
   while (at.row < rows) {
@@ -245,9 +267,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, uint32_t
     const bool query = head0 + head < a.query_heads;
     at.next();
     if constexpr (Loop) {
-      float inverse = 1.0f;
+      Inverse inverse{1.0f, 0};
       if (Norm) {
-        float sum = 0.0f;
+        Sum sum = 0;
         for (uint32_t i = lane; i < units; i += lanes) {
           const Unit u = unit_at<V, Interleaved>(i, half, a.width);
           load(x, u, &xa, &xb);
@@ -267,7 +289,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, uint32_t
       P na, nb;
       if (on && at.row < rows)
         stream(in + (uint64_t)at.row * a.input_row_stride + (uint64_t)at.head * a.input_head_stride, own, &na, &nb);
-      const float inverse = Norm ? norm(on ? squares(own, xa, xb) : 0.0f) : 1.0f;
+      const Inverse inverse = Norm ? norm(on ? squares(own, xa, xb) : (Sum)0) : Inverse{1.0f, 0};
       if (on) finish(own, lane, xa, xb, query ? wq[0] : wk[0], query ? wq[1] : wk[1], inverse, y, row);
       xa = na;
       xb = nb;

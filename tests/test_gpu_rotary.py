@@ -160,6 +160,27 @@ def test_norm_rotary_of_one_group(ipus, ctx, dtype, width, query, key):
         b.free()
 
 
+@pytest.mark.parametrize("size", [1e37, 1e25, 2.0 ** 64, 1e-15, 1e-20, 1e-37])
+@pytest.mark.parametrize("heads,width,rotary_width", [(5, 128, 128), (3, 65, 10), (2, 2048, 64), (40, 64, 0)])
+@pytest.mark.parametrize("epsilon", [0.0, 1e-6])
+def test_norm_of_fp32_values_whose_squares_are_not_fp32(ipus, ctx, size, heads, width, rotary_width, epsilon):
+    rows = 4
+    x = (values(ipus, rows * heads * width, 8, np.float32).astype(np.float64) * size).astype(np.float32)
+    w = 1 + 0.2 * values(ipus, width, 9, np.float32)
+    positions = np.arange(rows, dtype=np.int32) * 1000
+    f, _ = ipus.rotary_frequencies(max(rotary_width, 2))
+    bufs = [ctx.upload(a) for a in (x, w, w, positions, f)]
+    out = ctx.alloc(x.nbytes)
+    ctx.launch("ipu_stack_norm_rotary_f32", out, bufs,
+               [rows, heads, 0, width, rotary_width, 0, heads * width, heads * width, bits(epsilon), 0])
+    got = out.download(np.float32).astype(np.float64).reshape(rows, heads, width)
+    want, bound = norm_rotate(x.astype(np.float64).reshape(rows, heads, width), w.astype(np.float64),
+                              float(np.float32(epsilon)), positions, f[:rotary_width // 2], 1.0, rotary_width, False)
+    assert np.all(np.abs(got - want) <= rounded(want, bound, np.float32))
+    for b in bufs + [out]:
+        b.free()
+
+
 def test_norm_of_zeros_and_large_values(ipus, ctx):
     """A head of zeros stays zero, one at fp16's end does not overflow."""
     width = 128
