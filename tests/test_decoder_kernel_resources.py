@@ -51,3 +51,13 @@ def test_rotary_kernels_hide_their_loads(kernels):
         for name, f in matching(kernels, fragment).items():
             assert int(f["Occupancy [waves/SIMD]"]) >= 5, (name, f)
             assert int(f["AGPRs"]) == 0 and int(f["VGPRs Spill"]) == 0, (name, f)
+
+
+def test_scalar_registers_parked_in_vector_lanes(kernels):
+    """They are moved around a segment's or a block's start, a lane each: as many as there are
+    now, some in reserve."""
+    for fragment, most in (("attention_pages_decode_kernel", None), ("attention_blocks_kernel", 80),
+                           ("attention_pages_general_kernel", 60), ("rotary_kernel", 0), ("append_kernel", 0)):
+        for name, f in matching(kernels, fragment).items():
+            budget = most if most is not None else 280 if "ELb1E" in name else 100
+            assert int(f["SGPRs Spill"]) <= budget, (name, f)
