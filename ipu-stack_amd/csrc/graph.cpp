@@ -1499,7 +1499,8 @@ extern "C" int ipus_session_capture(ipus_session* s) {
   if (!s) return fail(IPUS_ERROR_INVALID_ARGUMENT, "null session");
   if (s->pkg->steps.empty()) return 0;
   if (int status = use_device(s->ctx)) return status;
-  // Other threads' launches wait: on a stream that is being captured they would be recorded.
+  // Other threads wait: what they enqueue on a stream that is being captured would be recorded.
+  std::unique_lock<std::shared_mutex> capture(s->ctx->capture_mutex);
   std::lock_guard<std::recursive_mutex> lock(s->ctx->enqueue_mutex);
   if (s->exec) return 0;
   hipStream_t stream = s->ctx->stream;

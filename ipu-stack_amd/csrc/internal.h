@@ -10,6 +10,7 @@
 
 #include <atomic>
 #include <mutex>
+#include <shared_mutex>
 #include <unordered_map>
 
 struct ipus_context {
@@ -34,6 +35,9 @@ struct ipus_context {
   // session's replay, and over the whole of ipus_session_capture, whose steps come
   // through ipus_launch again.
   std::recursive_mutex enqueue_mutex;
+  // Held by ipus_session_capture, shared by copies, fills, events and waits: on a stream
+  // that is being captured those would be recorded, or end the capture.
+  std::shared_mutex capture_mutex;
   // ipus_session_capture is recording this context's stream into a graph
   // that will only be launched on it.
   std::atomic<bool> capturing_session{false};

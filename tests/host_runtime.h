@@ -18,7 +18,7 @@
 #include "ipus_graph.h"
 
 struct Entry {
-  std::string what;     // "launch", "replay", "begin", "end"
+  std::string what;     // "launch", "replay", "begin", "end", "copy", "fill", "wait", "event"
   std::thread::id by;
   dim3 grid;
   const void* kernel;
@@ -86,12 +86,19 @@ hipError_t hipMalloc(void** p, size_t bytes) {
 }
 hipError_t hipFree(void* p) { return free(p), hipSuccess; }
 hipError_t hipMemcpyAsync(void* to, const void* from, size_t n, hipMemcpyKind, hipStream_t) {
+  record("copy");
   return memcpy(to, from, n), hipSuccess;
 }
-hipError_t hipMemsetAsync(void* p, int v, size_t n, hipStream_t) { return memset(p, v, n), hipSuccess; }
+hipError_t hipMemsetAsync(void* p, int v, size_t n, hipStream_t) {
+  record("fill");
+  return memset(p, v, n), hipSuccess;
+}
 hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned) { return *s = (hipStream_t)malloc(1), hipSuccess; }
 hipError_t hipStreamDestroy(hipStream_t s) { return free(s), hipSuccess; }
-hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
+hipError_t hipStreamSynchronize(hipStream_t) { return record("wait"), hipSuccess; }
+hipError_t hipEventCreate(hipEvent_t* e) { return *e = (hipEvent_t)malloc(1), hipSuccess; }
+hipError_t hipEventDestroy(hipEvent_t e) { return free(e), hipSuccess; }
+hipError_t hipEventRecord(hipEvent_t, hipStream_t) { return record("event"), hipSuccess; }
 hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus* s) {
   return *s = stream_captured ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone, hipSuccess;
 }

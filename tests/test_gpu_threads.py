@@ -141,3 +141,37 @@ def test_a_session_beside_a_thread(ipus, ctx, kind):
     s.close()
     for buf in ins + outs:
         buf.free()
+
+
+def test_copies_beside_captures(ipus, ctx):
+    """Copies, fills and waits of one thread are in no other thread's graph, and end no capture."""
+    x = np.arange(4096, dtype=np.uint32)
+    a, b = ctx.alloc(x.nbytes), ctx.alloc(x.nbytes)
+    kept = []
+
+    def capture():
+        for _ in range(8):
+            s, name, bits = session(ipus, ctx)
+            s.capture()
+            s.run_sync()
+            kept.append((s, name, bits))
+
+    def copy():
+        for i in range(150):
+            ctx.write(a, x + np.uint32(i))
+            ctx.memset(b, i % 256)
+            ctx.sync()
+            assert np.array_equal(a.download(np.uint32), x + np.uint32(i))
+            assert np.all(b.download(np.uint8) == i % 256)
+
+    run_threads(capture, copy)
+    ctx.write(a, x)
+    ctx.memset(b, 0xFF)
+    for s, name, bits in kept:
+        s.run_sync()
+        assert np.array_equal(s.read(name), bits)
+    assert np.array_equal(a.download(np.uint32), x) and np.all(b.download(np.uint8) == 0xFF)
+    for s, _, _ in kept:
+        s.close()
+    a.free()
+    b.free()

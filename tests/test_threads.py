@@ -74,8 +74,30 @@ static void stands_together(std::thread::id by, size_t each) {
   CHECK(run % each == 0 && all > 0);
 }
 
+// Sessions captured, run and closed by one thread; another's entries stand outside of captures.
+static void captures(int n) {
+  for (int i = 0; i < n; ++i) {
+    ipus_session* t = two_products();
+    CHECK(ipus_session_capture(t) == 0 && ipus_session_capture(t) == 0);
+    CHECK(ipus_session_run(t) == 0 && ipus_session_destroy(t) == 0);
+  }
+}
+static void stands_outside(std::thread::id capturing, int n) {
+  bool recording = false;
+  int begun = 0, replayed = 0, beside = 0;
+  for (const Entry& e : entries) {
+    if (e.what == "begin") recording = true, ++begun;
+    if (e.what == "end") recording = false;
+    if (e.what == "replay") ++replayed;
+    if (e.by != capturing) ++beside;
+    CHECK(!recording || e.by == capturing);
+  }
+  CHECK(begun == n && replayed == n && beside > 0);
+}
+
 int main() {
   CHECK(ipus_context_create(0, &ctx) == 0);
+  entries.clear();
   CHECK(split_keys() == 0 && entries.size() == 2);
   entries.clear();
   CHECK(shared_keys() == 0 && entries.size() == 2);
@@ -97,23 +119,22 @@ int main() {
   together(loop(split_keys, 30), loop(run, 30), &a, &b);
   stands_together(a, 2);
   stands_together(b, 2);
-  together(loop(split_keys, 20), [=] {
-    for (int i = 0; i < 10; ++i) {
-      ipus_session* t = two_products();
-      CHECK(ipus_session_capture(t) == 0 && ipus_session_capture(t) == 0);
-      CHECK(ipus_session_run(t) == 0 && ipus_session_destroy(t) == 0);
-    }
-  }, &a, &b);
+  together(loop(split_keys, 20), [] { captures(10); }, &a, &b);
   stands_together(a, 2);
-  bool recording = false;
-  int begun = 0, replayed = 0;
-  for (const Entry& e : entries) {
-    if (e.what == "begin") recording = true, ++begun;
-    if (e.what == "end") recording = false;
-    if (e.what == "replay") ++replayed;
-    CHECK(!recording || e.by == b);
-  }
-  CHECK(begun == 10 && replayed == 10);
+  stands_outside(b, 10);
+  // Copies, fills, waits and events beside captures.
+  ipus_event* event;
+  CHECK(ipus_event_create(ctx, &event) == 0);
+  static char host[64];
+  auto others = [=] {
+    const int done[] = {ipus_buffer_upload(ctx, memory, host, 64), ipus_buffer_download(ctx, host, memory, 64),
+                        ipus_buffer_copy(ctx, memory, memory + 64, 64), ipus_buffer_memset(ctx, memory, 0, 64),
+                        ipus_stream_sync(ctx), ipus_event_record(ctx, event)};
+    for (int e : done) if (e) return e;
+    return 0;
+  };
+  together(loop(others, 15), [] { captures(10); }, &a, &b);
+  stands_outside(b, 10);
   printf("%d failures\n", failures);
   return failures != 0;
 }
