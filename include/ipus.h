@@ -373,7 +373,8 @@ int ipus_launch(ipus_context *context, const char *symbol, void *output,
  * split tiles of 256 x 256, all fit), else IPUS_ERROR_UNSUPPORTED_COUNT.
  * The call enqueues on the context's stream and calls no allocator.  Every
  * call on one device shares that device's array: calls that overlap on one
- * device (from different streams or threads) race. */
+ * device (from other contexts, or recorded and replayed on other streams) race;
+ * those of one context stand one after the other on its stream. */
 #define IPUS_SPLIT_SCRATCH_BYTES (16ull << 20)
 int ipus_gemm_f16_split_noalloc(ipus_context *context, void *output, const void *left,
                                 const void *right, uint32_t batches, uint32_t rows,

@@ -31,8 +31,8 @@ struct ipus_context {
   size_t workspace_bytes = 0;
   uint32_t* workspace_counters = nullptr;
   // Held while a call enqueues its launches on the stream: by ipus_launch (some
-  // operators are two launches with parts in the workspace between them), by a
-  // session's replay, and over the whole of ipus_session_capture, whose steps come
+  // operators are two launches with parts in the workspace between them), by
+  // ipus_gemm_f16_split_noalloc, by a session's replay, and over the whole of ipus_session_capture, whose steps come
   // through ipus_launch again.
   std::recursive_mutex enqueue_mutex;
   // Held by ipus_session_capture, shared by copies, fills, events and waits: on a stream

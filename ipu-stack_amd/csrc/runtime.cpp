@@ -1290,6 +1290,7 @@ extern "C" int ipus_gemm_f16_split_noalloc(ipus_context* ctx, void* output, cons
   a.left_batch_stride = left_batch_stride;
   a.right_batch_stride = right_batch_stride;
   a.gelu = gelu != 0;
+  std::lock_guard<std::recursive_mutex> lock(ctx->enqueue_mutex);
   return check_launch(launch_gemm_f16_split_noalloc(ctx->stream, ctx->device, a, splits),
                       "ipus_gemm_f16_split_noalloc");
 }

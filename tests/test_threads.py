@@ -26,6 +26,9 @@ static int product() {  // splits its sum in the same workspace
   const void* in[] = {memory, memory};
   return ipus_launch(ctx, "ipu_stack_gemm_f16", memory, in, 2, s, 8);
 }
+static int split_product() {  // partial products in the library's own array, then their sum
+  return ipus_gemm_f16_split_noalloc(ctx, memory, memory, memory, 1, 8, 512, 4096, 0, 0, 0, 0, 4, 0);
+}
 static ipus_session* two_products() {
   ipus_graph* g;
   ipus_value x, w, y, out;
@@ -103,6 +106,8 @@ int main() {
   CHECK(shared_keys() == 0 && entries.size() == 2);
   entries.clear();
   CHECK(product() == 0 && entries.size() == 1);
+  entries.clear();
+  CHECK(split_product() == 0 && entries.size() == 2);
   pause_us = 300;
   auto loop = [](auto f, int n) { return [=] { for (int i = 0; i < n; ++i) CHECK(f() == 0); }; };
   std::thread::id a, b;
@@ -113,6 +118,9 @@ int main() {
   together(loop(split_keys, 30), loop(shared_keys, 30), &a, &b);
   stands_together(a, 2);
   stands_together(b, 2);
+  together(loop(split_product, 30), loop(split_product, 30), &a, &b);
+  stands_together(a, 2);
+  stands_together(b, 2);
   // A session's run, its replays and its capture.
   ipus_session* s = two_products();
   auto run = [=] { return ipus_session_run(s); };
@@ -121,6 +129,8 @@ int main() {
   stands_together(b, 2);
   together(loop(split_keys, 20), [] { captures(10); }, &a, &b);
   stands_together(a, 2);
+  stands_outside(b, 10);
+  together(loop(split_product, 20), [] { captures(10); }, &a, &b);
   stands_outside(b, 10);
   // Copies, fills, waits and events beside captures.
   ipus_event* event;
