@@ -23,19 +23,23 @@ struct Entry {
   dim3 grid;
   const void* kernel;
   std::vector<char> first;  // bytes of a kernel's first argument
+  dim3 block;
+  size_t shared;
+  std::vector<uint32_t> words;  // its arguments behind the first, of 32 bits each
 };
 inline std::mutex log_mutex;
 inline std::vector<Entry> entries;
 inline int pause_us = 0;                 // how long an entry takes
 inline size_t first_bytes = 0;           // of each launch's first argument, to be logged
+inline size_t first_words = 0;           // how many arguments of 32 bits behind it
 inline size_t largest_allocation = ~0ull;
 inline std::vector<size_t> allocations;  // that succeeded
 inline std::atomic<bool> stream_captured{false};
 inline int failures = 0;
 #define CHECK(x) do { if (!(x)) { printf("line %d: %s\n", __LINE__, #x); ++failures; } } while (0)
 
-inline void record(const char* what, dim3 grid = dim3(), const void* kernel = nullptr, const void* first = nullptr) {
-  Entry e{what, std::this_thread::get_id(), grid, kernel, {}};
+inline void record(Entry e, const void* first = nullptr) {
+  e.by = std::this_thread::get_id();
   if (first && first_bytes) e.first.assign((const char*)first, (const char*)first + first_bytes);
   {
     std::lock_guard<std::mutex> lock(log_mutex);
@@ -43,6 +47,8 @@ inline void record(const char* what, dim3 grid = dim3(), const void* kernel = nu
   }
   if (pause_us) std::this_thread::sleep_for(std::chrono::microseconds(pause_us));
 }
+
+inline void record(const char* what) { record(Entry{what}); }
 
 struct Configuration {
   dim3 grid, block;
@@ -70,8 +76,10 @@ void** __hipRegisterFatBinary(const void*) {
 void __hipRegisterFunction(void**, const void*, char*, const char*, unsigned, void*, void*, dim3*, dim3*, int*) {}
 void __hipRegisterVar(void**, void*, char*, char*, int, size_t, int, int) {}
 void __hipUnregisterFatBinary(void**) {}
-hipError_t hipLaunchKernel(const void* kernel, dim3 grid, dim3, void** args, size_t, hipStream_t) {
-  record("launch", grid, kernel, args ? args[0] : nullptr);
+hipError_t hipLaunchKernel(const void* kernel, dim3 grid, dim3 block, void** args, size_t shared, hipStream_t) {
+  Entry e{"launch", {}, grid, kernel, {}, block, shared, {}};
+  for (size_t i = 0; i < first_words; ++i) e.words.push_back(*(const uint32_t*)args[1 + i]);
+  record(std::move(e), args ? args[0] : nullptr);
   return hipSuccess;
 }
 hipError_t hipGetDeviceCount(int* n) { return *n = 1, hipSuccess; }
