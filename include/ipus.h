@@ -196,8 +196,9 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        magnitude_bits.  A row's heads lie side by side, queries before keys
  *        (the value heads of a fused projection may follow in the row): each
  *        becomes x * weight / sqrt(mean(x^2) + epsilon), then is turned as
- *        above, with one rounding.  key_heads or query_heads may be 0 (its
- *        weight pointer is then not read, but not null either).
+ *        above, with one rounding, in place or not as there.  key_heads or
+ *        query_heads may be 0 (its weight pointer is then not read, but not
+ *        null either).
  *   ipu_stack_append_pages_f16   out the cache, fp16 [pages][2][key_heads]
  *        [page_rows][width] (keys, then values); new keys and values
  *        [rows][key_heads][width] (row strides in elements), frequencies,
@@ -213,7 +214,8 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        and entries outside [0, pages) write nothing.  The offsets do not
  *        decrease (nor for the attention below); a page that new rows go to
  *        belongs to one sequence and stands once in its table.
- *   ipu_stack_attention_pages_f16   out f16 [rows][query_heads][width]; query
+ *   ipu_stack_attention_pages_f16   out f16 [rows][query_heads][width], apart
+ *        from the inputs; query
  *        f16 (heads side by side, query_row_stride elements from row to row),
  *        the cache, page_table, row_offsets, lengths; sequences, rows,
  *        max_rows, query_heads, key_heads (a divisor: query head h reads key
