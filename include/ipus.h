@@ -244,6 +244,69 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        once for all where that pays, by launches that are not recorded into
  *        a caller's graph and with max_rows x the query heads of a key head up
  *        to 32; else by each sequence.
+ *   A step with drafted tokens (no reference counterpart; the batch as above).
+ *   A tree's mask is u32 [rows][mask_words]: bit j % 32 of word j / 32 says that
+ *   the row reads the j-th row of its sequence (its ancestors and itself); bits
+ *   past the sequence's rows or the words are not read.
+ *   ipu_stack_page_tables   out an int32 state: free, missing, free pages
+ *        [pages] (-1 from `free` on), held [sequences], page_table [sequences]
+ *        [table_columns] (-1 from held[s] on); the previous state, with
+ *        previous_sequences rows, source [sequences], lengths [sequences];
+ *        sequences, previous_sequences, pages, page_rows, table_columns.
+ *        Sequence s goes on with row source[s] of the previous table (the first
+ *        that names it; one that names none of it begins) and has pages for
+ *        lengths[s] positions, at most table_columns.  Pages past that and those
+ *        of rows that nobody goes on with go behind the free ones, in the order
+ *        of the previous rows; what sequences need is taken from the end, the
+ *        sequences in order.  missing: how many there were too few; the sequences
+ *        then hold fewer (their table ends earlier).  A first state: all pages
+ *        free, previous_sequences 0.  Up to 4096 sequences; the states must not
+ *        overlap.  A page is held once: no prefix is shared.
+ *   ipu_stack_slot_maps   out int32 row_offsets [sequences + 1], positions [rows],
+ *        slots [rows], one after the other; counts [sequences] (new rows, below 0
+ *        as 0), lengths [sequences] (with them), page_table, the tree's mask;
+ *        sequences, rows, pages, page_rows, table_columns, mask_words (0: none,
+ *        and not read).  Offsets are cut off at `rows`.  Row i of the n of
+ *        sequence s is stored at place lengths[s] - n + i: its slot is page *
+ *        page_rows + row in the page, -1 where the place has no page.  Its
+ *        position is the place, in a tree lengths[s] - n + how many other rows it
+ *        reads (its depth), -1 below 0.  Rows behind the last sequence: position
+ *        0, slot -1.  pages x page_rows <= 2^31.
+ *   ipu_stack_attention_tree_pages_f16   as ipu_stack_attention_pages_f16 with the
+ *        tree's mask behind the inputs and mask_words (at least 1) in the place of
+ *        causal: row i of sequence s reads the keys before its sequence's rows,
+ *        below lengths[s] - n, and those of the rows that its mask names (row j's
+ *        stands at lengths[s] - n + j).  A row that reads no key gives zeros.
+ *        Recorded launches do not split their keys, as there.
+ *   ipu_stack_adjust_logits_f16, ipu_stack_adjust_logits_f32   out [rows] of
+ *        columns logits; logits, row_offsets, tokens [rows], the tree's mask,
+ *        history [sequences][history_columns], history_counts [sequences][2] (the
+ *        prompt's tokens, all), penalties fp32 [sequences][3] (repetition r,
+ *        frequency f, presence p), bias_offsets [sequences + 1], biases
+ *        [bias_entries][2] (token, fp32 bits), allowed u32 [rows][allowed_words]
+ *        (bit t % 32 of word t / 32: token t); sequences, rows, columns,
+ *        input_row_stride, output_row_stride (elements, at least columns),
+ *        mask_words, history_columns, bias_entries, allowed_words.  A scalar of 0
+ *        says that there is no such list, which is then not read; without a mask
+ *        a row's path is its sequence's rows up to itself, else those that its
+ *        mask names.  With g how often a token stands in the path and the history
+ *        behind the prompt: a token of prompt, history or path has its logit x
+ *        divided by r (x > 0) or multiplied by it, and if g > 0 lessened by f g +
+ *        p; then its bias is added (of several entries the last); a token that is
+ *        not allowed gets -inf, whatever it was.  fp32 arithmetic, one rounding.
+ *        Tokens outside [0, columns) count for nothing (-1: a prompt's rows, whose
+ *        tokens stand in the history).  Rows outside every sequence are left as
+ *        they were.  The output is the input (with its stride) or does not overlap
+ *        it.
+ *   ipu_stack_keep_pages_f16   out the caches of all layers, fp16 [layers][pages][2]
+ *        [key_heads][page_rows][width]; page_table, row_offsets, lengths, path
+ *        [sequences][path_columns], path_counts [sequences]; sequences, rows, layers
+ *        (up to 65535), key_heads, width, pages, page_rows, table_columns,
+ *        path_columns.  Row path[s][i] of the new rows of sequence s moves to row i,
+ *        keys and values, for i < path_counts[s]: after it the accepted drafts stand
+ *        behind one another, from place lengths[s] - n on.  The path increases; it
+ *        ends at an entry that does not, or is no row of the sequence.  A place
+ *        without a page is neither read nor written.
  *   ipu_stack_gelu_tanh_approx_f16     out f16; input f16; element_count
  *        (kernel.rs:1251-1263; count must be even, kernel.rs:1400-1413).
  *   ipu_stack_reduce_sum_f16           out f16; initial, packed remotes f16;

@@ -148,7 +148,7 @@ _LAUNCH = None
 _LAUNCH_TYPE = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p,
                                 ctypes.c_char_p, ctypes.c_int, ctypes.c_char_p, ctypes.c_int)
 # Packers by count; a count beyond them takes the ctypes arrays.
-_PACK_POINTERS = tuple(struct.Struct(f"={n}Q").pack for n in range(8))
+_PACK_POINTERS = tuple(struct.Struct(f"={n}Q").pack for n in range(13))
 _PACK_SCALARS = tuple(struct.Struct(f"={n}I").pack for n in range(MAX_SCALARS + 1))
 
 _P = ctypes.c_void_p

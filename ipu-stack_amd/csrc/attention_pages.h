@@ -5,6 +5,7 @@
 #include "../../include/ipus.h"
 #include "kernels.h"
 #include "pages.h"
+#include "wave_scan.h"
 
 #define LDS_AS __attribute__((address_space(3)))
 #define GLOBAL_AS __attribute__((address_space(1)))
@@ -52,51 +53,8 @@ __device__ __forceinline__ float sum_of_query(float x) {
   return x + __shfl_xor(x, 32, kWave);
 }
 
-// Values that all lanes hold alike, into scalar registers.
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ uint64_t uniform(uint64_t x) {
-  return uniform((uint32_t)x) | (uint64_t)uniform((uint32_t)(x >> 32)) << 32;
-}
 __device__ __forceinline__ BatchSequence uniform(BatchSequence q) {
   return {uniform(q.first), uniform(q.rows), uniform(q.keys), (int)uniform((uint32_t)q.length), (int)uniform((uint32_t)q.end)};
-}
-__device__ __forceinline__ uint64_t from_lane(uint64_t x, uint32_t lane) {  // lane: alike in all lanes
-  return (uint32_t)__builtin_amdgcn_readlane((uint32_t)x, lane) |
-         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(x >> 32), lane) << 32;
-}
-// x of the lane that the DPP control names, 0 where there is none.
-template <int Control, int RowMask>
-__device__ __forceinline__ uint32_t neighbour(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, Control, RowMask, 0xf, false);
-}
-template <int Control, int RowMask>
-__device__ __forceinline__ uint64_t neighbour(uint64_t x) {
-  return neighbour<Control, RowMask>((uint32_t)x) | (uint64_t)neighbour<Control, RowMask>((uint32_t)(x >> 32)) << 32;
-}
-// Sum over the lanes up to this one, and the largest of all lanes: four steps inside rows
-// of 16 lanes (row_shr), then the rows before (row_bcast:15 and :31).
-__device__ __forceinline__ uint64_t scan(uint64_t x) {
-  x += neighbour<0x111, 0xf>(x);
-  x += neighbour<0x112, 0xf>(x);
-  x += neighbour<0x114, 0xf>(x);
-  x += neighbour<0x118, 0xf>(x);
-  x += neighbour<0x142, 0xa>(x);
-  x += neighbour<0x143, 0xc>(x);
-  return x;
-}
-template <int Control, int RowMask>
-__device__ __forceinline__ uint32_t larger(uint32_t x) {
-  const uint32_t y = neighbour<Control, RowMask>(x);
-  return x > y ? x : y;
-}
-__device__ __forceinline__ uint32_t largest(uint32_t x) {
-  x = larger<0x111, 0xf>(x);
-  x = larger<0x112, 0xf>(x);
-  x = larger<0x114, 0xf>(x);
-  x = larger<0x118, 0xf>(x);
-  x = larger<0x142, 0xa>(x);
-  x = larger<0x143, 0xc>(x);
-  return (uint32_t)__builtin_amdgcn_readlane(x, kWave - 1);
 }
 
 // Quotient of values that mostly fit 32 bits (a 64-bit division takes about 100
@@ -183,10 +141,11 @@ __device__ __forceinline__ void clear_non_finite(uint8_t* tile, uint32_t thread,
 }
 // Adds the products of a tile's non-finite values, in the layout of the kernels' MFMAs: o[dt][qt][c]
 // is column 16 dt + 4 (l / 16) + c of query 16 qt + l % 16, and p(kk, qt, e) the probability of
-// key 32 kk + 4 (l / 16) + e % 4 + 16 (e / 4).  chunk(row, column): where 4 columns lie in the tile.
-template <uint32_t Halves, uint32_t DT, uint32_t QT, typename P, typename Chunk>
+// key 32 kk + 4 (l / 16) + e % 4 + 16 (e / 4).  chunk(row, column): where 4 columns lie in the tile;
+// reads(qt, row): whether this lane's query reads the tile's key `row`.
+template <uint32_t Halves, uint32_t DT, uint32_t QT, typename P, typename Chunk, typename Reads>
 __device__ __forceinline__ void add_non_finite(float4_t (&o)[DT][QT], P p, const uint8_t* tile, Chunk chunk,
-                                               const uint32_t (&limit)[QT], uint32_t key0) {
+                                               Reads reads) {
 #pragma unroll
   for (uint32_t kk = 0; kk < Halves; ++kk)
 #pragma unroll
@@ -209,7 +168,7 @@ __device__ __forceinline__ void add_non_finite(float4_t (&o)[DT][QT], P p, const
             const float v = (float)x[c];
             const bool bad = !(fabsf(v) <= 65504.0f);
 #pragma unroll
-            for (uint32_t qt = 0; qt < QT; ++qt) o[dt][qt][c] += bad && key0 + row < limit[qt] ? w[qt] * v : 0.0f;
+            for (uint32_t qt = 0; qt < QT; ++qt) o[dt][qt][c] += bad && reads(qt, row) ? w[qt] * v : 0.0f;
           }
         }
       }

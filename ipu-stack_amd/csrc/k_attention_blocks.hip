@@ -82,8 +82,9 @@ __device__ __forceinline__ uint64_t blocks_of(const BatchSequence& q, uint32_t g
 }
 
 // Shared: the rows of the whole batch over the keys below shared_rows, as parts for
-// another launch.
-template <int D, int DC, int QT, bool Shared>
+// another launch.  Tree: the masks of a sequence's rows, looked up for the key blocks that hold
+// their keys.
+template <int D, int DC, int QT, bool Shared, bool Tree>
 __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAttentionArgs a, float scale_log2,
                                                                        uint32_t few, SplitKeys split) {
   using F = Block<D, QT>;
@@ -197,6 +198,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     const uint32_t x = __shfl_xor(least, o, kWave);
     least = x < least ? x : least;
   }
+  const TreeRows tree = Tree ? tree_rows(b, s, a.rows, a.mask_words) : TreeRows{0, 0};
+  if (Tree) least = tree.base <= 0 ? 0 : tree.base < (int64_t)q.keys ? (uint32_t)tree.base : q.keys;
   least = uniform(least);  // every query of the wave reads the keys below it
   if (lane == 0) wave_word[wave] = least;
   __syncthreads();
@@ -345,15 +348,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     }
     __builtin_amdgcn_s_setprio(0);
   };
+  // Of the 64 keys from key0 on, those that the mask of query 16 qt + l % 16 names.
+  auto seen = [&](uint32_t qt, uint32_t key0) __attribute__((always_inline)) {
+    uint32_t m = wave0 + 16 * qt + r16;
+    m = m < queries ? m : queries - 1;
+    return tree_window(a.tree_mask + (uint64_t)(q.first + m / group) * a.mask_words, tree, key0);
+  };
   // Softmax of block j (of all), whose rows with a page are `valid`; result in pp.
   auto softmax = [&](float4_t (&sc)[kKT][QT], uint32_t j, uint64_t valid) __attribute__((always_inline)) {
     constexpr uint64_t kAll = ~0ull >> (64 - kKeys);
     const uint32_t key0 = j * kKeys;
     if (valid != kAll || key0 + kKeys > least) {
       // sc[kt][qt][e]: key 16 kt + 4 (l / 16) + e of query 16 qt + l % 16.
-      const uint64_t mine = valid >> (4 * g4);
+      const uint64_t here = valid >> (4 * g4);
 #pragma unroll
       for (uint32_t qt = 0; qt < QT; ++qt) {
+        const uint64_t mine = Tree ? here & seen(qt, key0) >> (4 * g4) : here;
         const uint32_t left = limit[qt] > key0 + 4 * g4 ? limit[qt] - (key0 + 4 * g4) : 0;
 #pragma unroll
         for (uint32_t kt = 0; kt < kKT; ++kt)
@@ -431,12 +441,17 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     if (lane == 0) wave_word[wave] = mine;
     __syncthreads();
     if (wave_word[0] | wave_word[1] | wave_word[2] | wave_word[3]) {
+      uint64_t bits[QT];
+#pragma unroll
+      for (uint32_t qt = 0; qt < QT; ++qt) bits[qt] = Tree ? seen(qt, j * kKeys) : ~0ull;
       add_non_finite<kHalves, kDT, QT>(
           o, [&](uint32_t kk, uint32_t qt, uint32_t e) __attribute__((always_inline)) { return (float)pp[kk][qt][e]; }, lv,
           [&](uint32_t row, uint32_t column) __attribute__((always_inline)) {
             return row * kRowBytes + (((column / 8) ^ value_swizzle<D>(row)) << 4) + column % 8 * 2;
           },
-          limit, j * kKeys);
+          [&](uint32_t qt, uint32_t row) __attribute__((always_inline)) {
+            return j * kKeys + row < limit[qt] && (!Tree || (bits[qt] >> row & 1));
+          });
       __syncthreads();
       clear_non_finite<kTile>(lv, threadIdx.x, kThreads);
       __syncthreads();
@@ -601,7 +616,7 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
 }
 static_assert(kMaxSplits == 16, "join_parts_kernel folds the parts over 16 lanes");
 
-template <int D, int DC, int QT, bool Shared>
+template <int D, int DC, int QT, bool Shared, bool Tree>
 int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t few, const SplitKeys& given) {
   const uint64_t queries = (uint64_t)a.rows * (a.query_heads / a.key_heads);
   constexpr uint64_t kQueries = Block<D, QT>::kQueries;
@@ -638,7 +653,7 @@ int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2,
   uint64_t grid = Shared ? blocks * split.parts : split.parts > 1 ? kFullChip + 8 * kMaxSplits : blocks;
   grid = (grid + 7) / 8 * 8;
   if (grid > 0xffffffull) return IPUS_ERROR_UNAVAILABLE;  // a grid dimension holds less than 2^32 threads
-  hipLaunchKernelGGL((attention_blocks_kernel<D, DC, QT, Shared>), dim3((uint32_t)grid), dim3(kThreads), 0, stream, a,
+  hipLaunchKernelGGL((attention_blocks_kernel<D, DC, QT, Shared, Tree>), dim3((uint32_t)grid), dim3(kThreads), 0, stream, a,
                      scale_log2, few, split);
   if (int e = hip_status(hipGetLastError())) return e;
   if (Shared || split.parts <= 1) return 0;
@@ -647,23 +662,25 @@ int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2,
                      few, split);
   return hip_status(hipGetLastError());
 }
-template <bool Shared>
+template <bool Shared, bool Tree>
 int launch(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t few, const SplitKeys& split) {
-  if (a.width > 192) return launch_as<256, 256, 1, Shared>(stream, a, scale_log2, few, split);
-  if (a.width > 128) return launch_as<256, 192, 1, Shared>(stream, a, scale_log2, few, split);
-  if (a.width > 96) return launch_as<128, 128, 2, Shared>(stream, a, scale_log2, few, split);
-  if (a.width > 64) return launch_as<128, 96, 2, Shared>(stream, a, scale_log2, few, split);
-  if (a.width > 32) return launch_as<64, 64, 2, Shared>(stream, a, scale_log2, few, split);
-  return launch_as<64, 32, 2, Shared>(stream, a, scale_log2, few, split);
+  if (a.width > 192) return launch_as<256, 256, 1, Shared, Tree>(stream, a, scale_log2, few, split);
+  if (a.width > 128) return launch_as<256, 192, 1, Shared, Tree>(stream, a, scale_log2, few, split);
+  if (a.width > 96) return launch_as<128, 128, 2, Shared, Tree>(stream, a, scale_log2, few, split);
+  if (a.width > 64) return launch_as<128, 96, 2, Shared, Tree>(stream, a, scale_log2, few, split);
+  if (a.width > 32) return launch_as<64, 64, 2, Shared, Tree>(stream, a, scale_log2, few, split);
+  return launch_as<64, 32, 2, Shared, Tree>(stream, a, scale_log2, few, split);
 }
 
 }  // namespace
 
 int launch_attention_blocks(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, uint32_t few) {
-  return launch<false>(stream, a, scale_log2, few, SplitKeys{nullptr, nullptr, nullptr, 1});
+  const SplitKeys whole{nullptr, nullptr, nullptr, 1};
+  return a.tree_mask ? launch<false, true>(stream, a, scale_log2, few, whole)
+                     : launch<false, false>(stream, a, scale_log2, few, whole);
 }
 int launch_shared_parts(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const SharedParts& parts) {
-  return launch<true>(stream, a, scale_log2, 0, SplitKeys{parts.rows, parts.sums, nullptr, parts.parts});
+  return launch<true, false>(stream, a, scale_log2, 0, SplitKeys{parts.rows, parts.sums, nullptr, parts.parts});
 }
 uint32_t shared_part_count(const PagedAttentionArgs& a, uint32_t most) {
   const uint32_t block_queries = a.width > 128 ? 64 : 128, block_keys = a.width > 128 ? 32 : 64;

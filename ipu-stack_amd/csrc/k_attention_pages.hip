@@ -3,9 +3,12 @@
 // for every row of every sequence, query head h reading key head
 // h / (query_heads / key_heads).  Row i of the n rows of sequence s stands at
 // position lengths[s] - n + i; it reads the keys below lengths[s], when causal
-// those up to its own position.  Keys without a page carry no weight, and a row
+// those up to its own position, of a tree all before the sequence's rows and those of
+// the rows that its mask names.  Keys without a page carry no weight, and a row
 // whose weights are all zero (no key, or only scores of -inf) gives zeros.
 #include "attention_pages.h"
+
+#include <type_traits>
 
 namespace ipus {
 namespace {
@@ -15,6 +18,7 @@ namespace {
 // 16 heads x 1000 keys of 65 columns 69 us, of 2000 of 500 columns 434; one key after the
 // other by one wave 859 and 8,530).
 constexpr uint32_t kGeneralWidth = 1024, kGeneralPerLane = kGeneralWidth / kWave, kGeneralKeys = 8;
+template <bool Tree>
 __global__ __launch_bounds__(kThreads) void attention_pages_general_kernel(PagedAttentionArgs a, uint32_t first_row,
                                                                            float scale_log2) {
   __shared__ float wave_rows[kWaves][kGeneralWidth], wave_sums[kWaves][2];
@@ -27,6 +31,8 @@ __global__ __launch_bounds__(kThreads) void attention_pages_general_kernel(Paged
   const half_t* from = (const half_t*)a.query + (uint64_t)row * a.query_row_stride + (uint64_t)head * a.width;
   const uint32_t key_head = head / (a.query_heads / a.key_heads);
   const uint64_t head_elements = (uint64_t)a.batch.page_rows * a.width;
+  TreeRows tree = Tree ? tree_rows(a.batch, s, a.rows, a.mask_words) : TreeRows{0, 0};
+  if (Tree) asm volatile("" : "+v"(tree.base), "+v"(tree.bits));  // not in scalar registers
   float q[kGeneralPerLane], acc[kGeneralPerLane];
 #pragma unroll
   for (uint32_t i = 0; i < kGeneralPerLane; ++i) {
@@ -40,7 +46,9 @@ __global__ __launch_bounds__(kThreads) void attention_pages_general_kernel(Paged
     const half_t *key[kGeneralKeys], *value[kGeneralKeys];
     bool has[kGeneralKeys];
     float dot[kGeneralKeys];
-    const int mine = lane < kGeneralKeys && j0 + lane < count ? page_of(a.batch, s, j0 + lane) : -1;
+    int mine = lane < kGeneralKeys && j0 + lane < count ? page_of(a.batch, s, j0 + lane) : -1;
+    if (Tree && (int64_t)j0 + kGeneralKeys > tree.base)
+      mine = tree_window(a.tree_mask + (uint64_t)row * a.mask_words, tree, j0) >> lane & 1 ? mine : -1;
 #pragma unroll
     for (uint32_t u = 0; u < kGeneralKeys; ++u) {
       const int page = __builtin_amdgcn_readlane(mine, u);
@@ -267,8 +275,9 @@ __device__ __forceinline__ Units units_of(const BatchSequence& q, uint32_t group
   return u;
 }
 
-// Shared: the keys from first_key on, joined with the parts of those before it.
-template <int D, int MT, bool Shared>
+// Shared: the keys from first_key on, joined with the parts of those before it.  Tree: the
+// masks of a sequence's rows, looked up for the tiles that hold their keys.
+template <int D, int MT, bool Shared, bool Tree>
 __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_pages_decode_kernel(
     PagedAttentionArgs a, float scale_log2, uint32_t keys_from, uint32_t few, DecodeSplit split,
     SharedParts given) {
@@ -390,7 +399,9 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
     }
     // Every query of the tile reads the keys below `least`: causal rows stand in the order
     // of their positions.
-    const uint32_t least = readable_keys(q, row_position(q.length, q.end, q.first + query0 / group), a.causal);
+    const TreeRows tree = Tree ? tree_rows(b, s, a.rows, a.mask_words) : TreeRows{0, 0};
+    const uint32_t least = !Tree ? readable_keys(q, row_position(q.length, q.end, q.first + query0 / group), a.causal)
+                           : tree.base <= 0 ? 0 : tree.base < (int64_t)q.keys ? (uint32_t)tree.base : q.keys;
     float4_t o[kDT][MT];
     float m_run[MT], l_run[MT];
 #pragma unroll
@@ -470,11 +481,21 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
     // Softmax of tile t's scores, rows of `valid`, and the output with the values in lv.
     auto update = [&](uint32_t t, uint64_t valid, float4_t (&sc)[kKT][MT], uint8_t* lv) __attribute__((always_inline)) {
       const uint32_t key0 = first_key + t * kKeys;
+      const uint32_t upto = (t + 1) * kKeys < all_keys ? key0 + kKeys : q.keys;
       half8_t high[kHalves][MT], low[kHalves][MT];
+      // Of the tile's keys, those that the query's mask names.
+      auto seen = [&](uint32_t mt) __attribute__((always_inline)) {
+        uint32_t m = 16 * mt + opaque(lane) % 16;
+        m = m < queries ? m : queries - 1;
+        const uint32_t row = q.first + (query0 + m) / group;
+        return tree_window(a.tree_mask + (uint64_t)row * a.mask_words, tree, key0);
+      };
 #pragma unroll
       for (uint32_t mt = 0; mt < MT; ++mt) {
         // sc[kt][mt][e]: key 16 kt + 4 (l / 16) + e of query 16 mt + l % 16.
-        const uint64_t mine = valid >> (4 * g4);
+        uint64_t here = valid;
+        if (Tree && upto > least) here &= seen(mt);
+        const uint64_t mine = here >> (4 * g4);
         const uint32_t left = limit[mt] > key0 + 4 * g4 ? limit[mt] - (key0 + 4 * g4) : 0;
         float top = -INFINITY;
 #pragma unroll
@@ -506,8 +527,10 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
         for (uint32_t dt = 0; dt < kDT; ++dt) o[dt][mt] *= alpha;
       }
       __builtin_amdgcn_sched_barrier(0);
-      const uint32_t upto = (t + 1) * kKeys < all_keys ? key0 + kKeys : q.keys;
       if (upto > least && has_non_finite<kTile>(lv)) {
+        std::conditional_t<kKeys == 64, uint64_t, uint32_t> bits[MT];
+#pragma unroll
+        for (uint32_t mt = 0; mt < MT; ++mt) if (Tree) bits[mt] = seen(mt);
         add_non_finite<kHalves, kDT, MT>(
             o, [&](uint32_t kk, uint32_t mt, uint32_t e) __attribute__((always_inline)) {
               return (float)high[kk][mt][e] + (float)low[kk][mt][e];
@@ -515,7 +538,9 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
             [&](uint32_t row, uint32_t column) __attribute__((always_inline)) {
               return row * kRowBytes + (((column / 8) ^ tile_swizzle<D>(row)) << 4) + column % 8 * 2;
             },
-            limit, key0);
+            [&](uint32_t mt, uint32_t row) __attribute__((always_inline)) {
+              return key0 + row < limit[mt] && (!Tree || (bits[mt] >> row & 1));
+            });
         clear_non_finite<kTile>(lv, lane, kWave);
       }
       uint32_t vbase_v = vbase;
@@ -798,8 +823,12 @@ int launch_general(hipStream_t stream, const PagedAttentionArgs& a, float scale_
   constexpr uint32_t kMostRows = 1u << 23;  // a grid dimension holds less than 2^32 threads
   for (uint64_t done = 0; done < a.rows; done += kMostRows) {
     const uint32_t rows = a.rows - done < kMostRows ? (uint32_t)(a.rows - done) : kMostRows;
-    hipLaunchKernelGGL(attention_pages_general_kernel, dim3(rows, a.query_heads), dim3(kThreads), 0, stream, a,
-                       (uint32_t)done, scale_log2);
+    if (a.tree_mask)
+      hipLaunchKernelGGL(attention_pages_general_kernel<true>, dim3(rows, a.query_heads), dim3(kThreads), 0, stream, a,
+                         (uint32_t)done, scale_log2);
+    else
+      hipLaunchKernelGGL(attention_pages_general_kernel<false>, dim3(rows, a.query_heads), dim3(kThreads), 0, stream, a,
+                         (uint32_t)done, scale_log2);
     if (int e = hip_status(hipGetLastError())) return e;
   }
   return 0;
@@ -811,7 +840,7 @@ struct DecodeLaunch {
   uint32_t few;
   SharedParts shared;
 };
-template <int D, int MT, bool Shared>
+template <int D, int MT, bool Shared, bool Tree>
 int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
   constexpr uint64_t kResident = Decode<D, MT>::kResident, kQueries = Decode<D, MT>::kQueries;
   constexpr uint64_t kSlotBytes = kQueries * (D + 2) * sizeof(float);
@@ -832,29 +861,30 @@ int launch_decode_as(hipStream_t stream, const PagedAttentionArgs& a, float scal
       split.counters = a.workspace.counters;
     }
   }
-  hipLaunchKernelGGL((attention_pages_decode_kernel<D, MT, Shared>), dim3((uint32_t)groups), dim3(kThreads), 0, stream,
+  hipLaunchKernelGGL((attention_pages_decode_kernel<D, MT, Shared, Tree>), dim3((uint32_t)groups), dim3(kThreads), 0, stream,
                      a, scale_log2, l.first_key, l.few, split, l.shared);
   return hip_status(hipGetLastError());
 }
-template <int D, bool Shared>
+template <int D, bool Shared, bool Tree>
 int launch_decode_queries(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
   // Two tiles of queries at 256 columns do not fit the registers.
   if constexpr (D <= 128)
-    if ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16) return launch_decode_as<D, 2, Shared>(stream, a, scale_log2, l);
-  return launch_decode_as<D, 1, Shared>(stream, a, scale_log2, l);
+    if ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) > 16) return launch_decode_as<D, 2, Shared, Tree>(stream, a, scale_log2, l);
+  return launch_decode_as<D, 1, Shared, Tree>(stream, a, scale_log2, l);
 }
-template <bool Shared>
+template <bool Shared, bool Tree>
 int launch_decode_width(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
-  if (a.width > 192) return launch_decode_queries<256, Shared>(stream, a, scale_log2, l);
-  if (a.width > 128) return launch_decode_queries<192, Shared>(stream, a, scale_log2, l);
-  if (a.width > 96) return launch_decode_queries<128, Shared>(stream, a, scale_log2, l);
-  if (a.width > 64) return launch_decode_queries<96, Shared>(stream, a, scale_log2, l);
-  if (a.width > 32) return launch_decode_queries<64, Shared>(stream, a, scale_log2, l);
-  return launch_decode_queries<32, Shared>(stream, a, scale_log2, l);
+  if (a.width > 192) return launch_decode_queries<256, Shared, Tree>(stream, a, scale_log2, l);
+  if (a.width > 128) return launch_decode_queries<192, Shared, Tree>(stream, a, scale_log2, l);
+  if (a.width > 96) return launch_decode_queries<128, Shared, Tree>(stream, a, scale_log2, l);
+  if (a.width > 64) return launch_decode_queries<96, Shared, Tree>(stream, a, scale_log2, l);
+  if (a.width > 32) return launch_decode_queries<64, Shared, Tree>(stream, a, scale_log2, l);
+  return launch_decode_queries<32, Shared, Tree>(stream, a, scale_log2, l);
 }
 int launch_decode(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2, const DecodeLaunch& l) {
-  return l.shared.parts > 0 ? launch_decode_width<true>(stream, a, scale_log2, l)
-                            : launch_decode_width<false>(stream, a, scale_log2, l);
+  if (a.tree_mask) return launch_decode_width<false, true>(stream, a, scale_log2, l);
+  return l.shared.parts > 0 ? launch_decode_width<true, false>(stream, a, scale_log2, l)
+                            : launch_decode_width<false, false>(stream, a, scale_log2, l);
 }
 
 // Queries of a key head (rows x query heads) up to which a sequence is the decode kernel's.
@@ -911,7 +941,8 @@ bool plan_shared(const PagedAttentionArgs& a, SharedParts* parts, Workspace* res
 
 int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a) {
   if (a.rows == 0 || a.batch.sequences == 0) return 0;
-  if (((uintptr_t)a.query | (uintptr_t)a.cache | (uintptr_t)a.out) % 2 != 0 || batch_addresses(a.batch) % 4 != 0)
+  if (((uintptr_t)a.query | (uintptr_t)a.cache | (uintptr_t)a.out) % 2 != 0 ||
+      (batch_addresses(a.batch) | (uintptr_t)a.tree_mask) % 4 != 0)
     return IPUS_ERROR_INVALID_ARGUMENT;
   const float scale_log2 = a.scale * kLog2e;
   const bool vectors = a.width % 8 == 0 && a.query_row_stride % 8 == 0 &&

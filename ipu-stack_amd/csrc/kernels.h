@@ -145,9 +145,66 @@ struct PagedAttentionArgs {
   uint32_t rows, max_rows, query_heads, key_heads, width, query_row_stride;
   float scale;
   bool causal;
+  // Not null: which of its sequence's rows a row reads, [rows][mask_words], and all
+  // keys before them (causal is false then, and nothing is shared).
+  const uint32_t* tree_mask = nullptr;
+  uint32_t mask_words = 0;
   Workspace workspace;
 };
 int launch_attention_pages(hipStream_t stream, const PagedAttentionArgs& a);
+
+// Page tables fitted to the sequences' lengths (k_page_maps.hip): int32 states
+// [free][missing][free pages: pages][held: sequences][table: sequences x columns].
+constexpr uint32_t kMostTableSequences = 4096;  // of a state; running sums in LDS
+struct PageTableArgs {
+  int* out;
+  const int* previous;
+  const int* source;   // [sequences] row of the previous state, none outside it
+  const int* lengths;  // [sequences]
+  uint32_t sequences, previous_sequences, pages, page_shift, columns;
+};
+int launch_page_tables(hipStream_t stream, const PageTableArgs& a);
+
+// Row offsets, positions and cache slots of a step's rows: int32 [sequences + 1],
+// [rows], [rows].  batch.row_offsets is not read.
+struct SlotMapArgs {
+  int* out;
+  const int* counts;     // [sequences] new rows
+  const uint32_t* mask;  // [rows][mask_words], none of 0 words
+  PagedBatch batch;
+  uint32_t rows, mask_words;
+};
+int launch_slot_maps(hipStream_t stream, const SlotMapArgs& a);
+
+// Accepted rows of every sequence's new ones moved together, in the caches of all
+// layers, each of batch.pages pages.
+struct KeepArgs {
+  void* caches;
+  const int* path;         // [sequences][path_columns]
+  const int* path_counts;  // [sequences]
+  PagedBatch batch;
+  uint32_t rows, layers, key_heads, width, path_columns;
+};
+int launch_keep_pages(hipStream_t stream, const KeepArgs& a);
+
+// Penalties, biases and masks on logits (k_logits.hip).
+struct LogitArgs {
+  void* out;
+  const void* logits;
+  const int* row_offsets;     // [sequences + 1]
+  const int* tokens;          // [rows]
+  const uint32_t* mask;       // [rows][mask_words], none of 0 words: rows in order
+  const int* history;         // [sequences][history_columns]
+  const int* history_counts;  // [sequences][2]: the prompt's, all
+  const float* penalties;     // [sequences][3]: repetition, frequency, presence
+  const int* bias_offsets;    // [sequences + 1]
+  const int* biases;          // [bias_entries][2]: token, fp32 bits
+  const uint32_t* allowed;    // [rows][allowed_words], none of 0 words
+  uint32_t sequences, rows, columns, input_row_stride, output_row_stride;
+  uint32_t mask_words, history_columns, bias_entries, allowed_words;
+  bool f32;
+};
+int launch_adjust_logits(hipStream_t stream, const LogitArgs& a);
 
 // Bandwidth kernels (k_memory.hip).
 int launch_transpose_f16(hipStream_t stream, void* dst, const void* src, uint32_t matrices,

@@ -69,4 +69,36 @@ IPUS_HD uint32_t readable_keys(const BatchSequence& q, int position, bool causal
   return upto < q.keys ? upto : q.keys;
 }
 
+// A tree of drafted tokens: the sequence's rows, and which of them each reads.  A row's
+// mask says so by bit j for the j-th of them, whose key stands at position base + j;
+// the keys before `base` are every row's.
+struct TreeRows {
+  int64_t base;   // of the first row, negative where the sequence has more rows than keys
+  uint32_t bits;  // of a mask that are read: one per row, as far as the mask reaches
+};
+IPUS_HD TreeRows tree_rows(const PagedBatch& b, uint32_t s, uint32_t row_count, uint32_t mask_words) {
+  const int64_t from = b.row_offsets[s], to = b.row_offsets[s + 1];
+  const int64_t rows = to > from ? to - from : 0;
+  const uint64_t most = rows < (int64_t)row_count ? (uint64_t)rows : row_count, reach = 32ull * mask_words;
+  return {(int64_t)b.lengths[s] - rows, (uint32_t)(most < reach ? most : reach)};
+}
+// Which of the 64 keys from position `key` on a row with this mask reads: bit i for key + i.
+IPUS_HD uint64_t tree_window(const uint32_t* mask, const TreeRows& t, uint32_t key) {
+  const int64_t first = (int64_t)key - t.base;  // bit of the mask, negative before the rows
+  if (first >= (int64_t)t.bits) return 0;
+  if (first <= -64) return ~0ull;
+  const uint32_t at = first > 0 ? (uint32_t)first : 0, word = at / 32, shift = at % 32;
+  uint64_t x = 0;
+  if (t.bits > at) {
+    const uint32_t last = (t.bits - 1) / 32;
+    x = mask[word];
+    if (word < last) x |= (uint64_t)mask[word + 1] << 32;
+    x >>= shift;
+    if (shift > 0 && word + 1 < last) x |= (uint64_t)mask[word + 2] << (64 - shift);
+    const uint32_t left = t.bits - at;
+    if (left < 64) x &= (1ull << left) - 1;
+  }
+  return first >= 0 ? x : x << -first | ((1ull << -first) - 1);
+}
+
 }  // namespace ipus

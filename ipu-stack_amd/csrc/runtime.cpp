@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cctype>
 #include <cmath>
@@ -613,8 +614,16 @@ int check_attention_pages(const uint32_t* s) {
   if (!std::isfinite(most) || scale <= 0.0f) return IPUS_ERROR_INVALID_ARGUMENT;
   return s[5] > kMaxPagedWidth ? IPUS_ERROR_UNAVAILABLE : 0;
 }
+// As above with mask_words in the place of causal.
+int check_attention_tree(const uint32_t* s) {
+  uint32_t same[12];
+  std::copy(s, s + 12, same);
+  same[10] = 0;
+  if (s[10] == 0) return IPUS_ERROR_INVALID_ARGUMENT;
+  return check_attention_pages(same);
+}
 int run_attention_pages(ipus_context* c, void* o, const void* const* i, const uint32_t* s,
-                        uint32_t shared_rows) {
+                        uint32_t shared_rows, bool tree = false) {
   PagedAttentionArgs a;
   a.out = o;
   a.query = i[0];
@@ -627,10 +636,105 @@ int run_attention_pages(ipus_context* c, void* o, const void* const* i, const ui
   a.key_heads = s[4];
   a.width = s[5];
   a.query_row_stride = s[6];
-  a.causal = s[10] != 0;
+  a.causal = !tree && s[10] != 0;
+  if (tree) {
+    a.tree_mask = (const uint32_t*)i[5];
+    a.mask_words = s[10];
+  }
   a.scale = s[11] == 0 ? 1.0f / std::sqrt((float)s[5]) : bits_to_float(s[11]);
   a.workspace = context_workspace(c, true);
   return launch_attention_pages(c->stream, a);
+}
+
+// sequences, previous_sequences, pages, page_rows, table_columns.  A table's entries are
+// counted in 32 bits, beside the pages.
+int check_page_tables(const uint32_t* s) {
+  if (int e = check_pages(s[0], 0, 1, s[3])) return e;
+  if (s[2] > 0x7fffffff || (uint64_t)s[0] * s[4] > 0x7fffffff || (uint64_t)s[1] * s[4] > 0x7fffffff)
+    return IPUS_ERROR_INVALID_ARGUMENT;
+  return s[0] > kMostTableSequences || s[1] > kMostTableSequences ? IPUS_ERROR_UNAVAILABLE : 0;
+}
+int run_page_tables(ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+  PageTableArgs a;
+  a.out = (int*)o;
+  a.previous = (const int*)i[0];
+  a.source = (const int*)i[1];
+  a.lengths = (const int*)i[2];
+  a.sequences = s[0];
+  a.previous_sequences = s[1];
+  a.pages = s[2];
+  a.page_shift = (uint32_t)__builtin_ctz(s[3]);
+  a.columns = s[4];
+  return launch_page_tables(c->stream, a);
+}
+
+// sequences, rows, pages, page_rows, table_columns, mask_words.  A slot is an int32.
+int check_slot_maps(const uint32_t* s) {
+  if (int e = check_pages(s[0], s[1], 1, s[3])) return e;
+  return (uint64_t)s[2] * s[3] > 0x80000000ull ? IPUS_ERROR_INVALID_ARGUMENT : 0;
+}
+int run_slot_maps(ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+  SlotMapArgs a;
+  a.out = (int*)o;
+  a.counts = (const int*)i[0];
+  a.mask = (const uint32_t*)i[3];
+  a.batch = paged_batch(i[2], nullptr, i[1], s[0], s[2], s[3], s[4], 1, 1);
+  a.rows = s[1];
+  a.mask_words = s[5];
+  return launch_slot_maps(c->stream, a);
+}
+
+// sequences, rows, layers, key_heads, width, pages, page_rows, table_columns, path_columns.
+int check_keep_pages(const uint32_t* s) {
+  if (int e = check_pages(s[0], s[1], s[3], s[6])) return e;
+  return s[4] == 0 ? IPUS_ERROR_INVALID_ARGUMENT : 0;
+}
+int run_keep_pages(ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+  KeepArgs a;
+  a.caches = o;
+  a.batch = paged_batch(i[0], i[1], i[2], s[0], s[5], s[6], s[7], s[3], s[4]);
+  a.path = (const int*)i[3];
+  a.path_counts = (const int*)i[4];
+  a.rows = s[1];
+  a.layers = s[2];
+  a.key_heads = s[3];
+  a.width = s[4];
+  a.path_columns = s[8];
+  return launch_keep_pages(c->stream, a);
+}
+
+// sequences, rows, columns, input and output row stride, mask_words, history_columns,
+// bias_entries, allowed_words.
+int check_adjust_logits(const uint32_t* s) {
+  if (s[0] > 0x7fffffff || s[1] > 0x7fffffff || s[2] == 0 || s[2] > 0x7fffffff || s[7] > 0x7fffffff)
+    return IPUS_ERROR_INVALID_ARGUMENT;
+  if (s[3] < s[2] || s[4] < s[2]) return IPUS_ERROR_INVALID_ARGUMENT;
+  return s[8] != 0 && (uint64_t)s[8] * 32 < s[2] ? IPUS_ERROR_INVALID_ARGUMENT : 0;
+}
+int run_adjust_logits(ipus_context* c, void* o, const void* const* i, const uint32_t* s, bool f32) {
+  LogitArgs a;
+  a.out = o;
+  a.logits = i[0];
+  a.row_offsets = (const int*)i[1];
+  a.tokens = (const int*)i[2];
+  a.mask = (const uint32_t*)i[3];
+  a.history = (const int*)i[4];
+  a.history_counts = (const int*)i[5];
+  a.penalties = (const float*)i[6];
+  a.bias_offsets = (const int*)i[7];
+  a.biases = (const int*)i[8];
+  a.allowed = (const uint32_t*)i[9];
+  a.sequences = s[0];
+  a.rows = s[1];
+  a.columns = s[2];
+  a.input_row_stride = s[3];
+  a.output_row_stride = s[4];
+  a.mask_words = s[5];
+  a.history_columns = s[6];
+  a.bias_entries = s[7];
+  a.allowed_words = s[8];
+  a.f32 = f32;
+  return launch_adjust_logits(c->stream, a);
 }
 
 const std::vector<KernelEntry>& registry() {
@@ -769,6 +873,38 @@ const std::vector<KernelEntry>& registry() {
          return run_attention_pages(c, o, i, s, s[12]);
        },
        check_attention_pages},
+      // A step with drafted tokens (no reference counterpart).
+      {"ipu_stack_attention_tree_pages_f16", 6,
+       {"sequences", "rows", "max_rows", "query_heads", "key_heads", "width", "query_row_stride",
+        "pages", "page_rows", "table_columns", "mask_words", "scale_bits"},
+       [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+         return run_attention_pages(c, o, i, s, 0, true);
+       },
+       check_attention_tree},
+      {"ipu_stack_page_tables", 3,
+       {"sequences", "previous_sequences", "pages", "page_rows", "table_columns"},
+       run_page_tables, check_page_tables},
+      {"ipu_stack_slot_maps", 4,
+       {"sequences", "rows", "pages", "page_rows", "table_columns", "mask_words"},
+       run_slot_maps, check_slot_maps},
+      {"ipu_stack_keep_pages_f16", 5,
+       {"sequences", "rows", "layers", "key_heads", "width", "pages", "page_rows", "table_columns",
+        "path_columns"},
+       run_keep_pages, check_keep_pages},
+      {"ipu_stack_adjust_logits_f16", 10,
+       {"sequences", "rows", "columns", "input_row_stride", "output_row_stride", "mask_words",
+        "history_columns", "bias_entries", "allowed_words"},
+       [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+         return run_adjust_logits(c, o, i, s, false);
+       },
+       check_adjust_logits},
+      {"ipu_stack_adjust_logits_f32", 10,
+       {"sequences", "rows", "columns", "input_row_stride", "output_row_stride", "mask_words",
+        "history_columns", "bias_entries", "allowed_words"},
+       [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
+         return run_adjust_logits(c, o, i, s, true);
+       },
+       check_adjust_logits},
       {"ipu_stack_gelu_tanh_approx_f16", 1, {"element_count"},
        [](ipus_context* c, void* o, const void* const* i, const uint32_t* s) {
          return launch_gelu_f16(c->stream, o, i[0], s[0]);
