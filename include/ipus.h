@@ -286,7 +286,7 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        [bias_entries][2] (token, fp32 bits), allowed u32 [rows][allowed_words]
  *        (bit t % 32 of word t / 32: token t); sequences, rows, columns,
  *        input_row_stride, output_row_stride (elements, at least columns),
- *        mask_words, history_columns (with rows below 2^30), bias_entries,
+ *        mask_words, history_columns (with rows below 2^29), bias_entries,
  *        allowed_words.  A scalar of 0
  *        says that there is no such list, which is then not read; without a mask
  *        a row's path is its sequence's rows up to itself, else those that its

@@ -9,15 +9,16 @@
 namespace ipus {
 namespace {
 
-// A workgroup takes a chunk of the tokens and up to `group` rows of a sequence, one after the
-// other.  How often each token of the chunk stands in the history is counted in LDS, once for
-// these rows (integers: any order gives the same); each row's path is added to that and taken
-// off again.  The next row's logits and mask words are on their way while this one's are
-// adjusted.
+// Two kernels: for single rows of many sequences (a token each), where the launch and the loads
+// that wait for each other count, and for several rows of a sequence.
+//
+// Both: a workgroup takes a chunk of the tokens.  How often each of them stands in the history
+// is counted in LDS (integers: any order gives the same).
 constexpr uint32_t kLogitThreads = 512, kChunk = 4096;
-// A token's word: its uses behind the prompt, whether it stands in the prompt, and whether it
-// has a bias.
-constexpr uint32_t kInPrompt = 1u << 31, kBiased = 1u << 30, kUses = kBiased - 1;
+// A token's word: its uses behind the prompt, and whether it stands in the prompt, has a bias,
+// or stands in some row's path.
+constexpr uint32_t kInPrompt = 1u << 31, kBiased = 1u << 30, kInPath = 1u << 29, kUses = kInPath - 1;
+
 // Rows [first, first + rows) of sequence s, offsets outside the rows cut off.
 struct LogitRows {
   uint32_t first, rows;
@@ -28,15 +29,177 @@ __device__ __forceinline__ LogitRows logit_rows(const LogitArgs& a, uint32_t s) 
   return {(uint32_t)first, last > first ? (uint32_t)(last - first) : 0};
 }
 template <typename T>
-__global__ __launch_bounds__(kLogitThreads, 8) void adjust_logits_kernel(LogitArgs a, uint32_t first_unit, uint32_t group) {
-  constexpr uint32_t kPer = 16 / sizeof(T), kPacks = kChunk / (kLogitThreads * kPer);
+struct LogitPacks {
+  static constexpr uint32_t kPer = 16 / sizeof(T), kPacks = kChunk / (kLogitThreads * kPer);
   typedef T Pack __attribute__((ext_vector_type(kPer)));
   typedef Pack Loose __attribute__((aligned(sizeof(T))));  // rows of any alignment
+  static __device__ __forceinline__ uint32_t place(uint32_t i) { return (i * kLogitThreads + threadIdx.x) * kPer; }
+  // This thread's packs of a row's chunk, and the words of the row's mask that hold their bits.
+  Pack x[kPacks];
+  uint32_t bits[kPacks];
+  __device__ __forceinline__ void load(const LogitArgs& a, uint32_t row, uint32_t chunk0, uint32_t tokens) {
+    const T* from = (const T*)a.logits + (uint64_t)row * a.input_row_stride + chunk0;
+    const uint32_t* allowed = a.allowed + (uint64_t)row * a.allowed_words + chunk0 / 32;
+#pragma unroll
+    for (uint32_t i = 0; i < kPacks; ++i) {
+      const uint32_t at = place(i);
+      bits[i] = ~0u;
+      if (at < tokens && a.allowed_words) bits[i] = allowed[at / 32];
+      if (at + kPer <= tokens) {
+        x[i] = __builtin_nontemporal_load((const Loose*)(from + at));
+      } else {
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k)
+          if (at + k < tokens) x[i][k] = from[at + k];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(const LogitArgs& a, uint32_t row, uint32_t chunk0, uint32_t tokens) {
+    T* to = (T*)a.out + (uint64_t)row * a.output_row_stride + chunk0;
+#pragma unroll
+    for (uint32_t i = 0; i < kPacks; ++i) {
+      const uint32_t at = place(i), allowed = bits[i] >> at % 32;
+#pragma unroll
+      for (uint32_t k = 0; k < kPer; ++k) x[i][k] = allowed >> k & 1 ? x[i][k] : (T)-INFINITY;
+      if (at + kPer <= tokens) {
+        __builtin_nontemporal_store(x[i], (Loose*)(to + at));
+      } else {
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k)
+          if (at + k < tokens) to[at + k] = x[i][k];
+      }
+    }
+  }
+};
+struct Penalties {
+  float repetition, frequency, presence;
+  __device__ __forceinline__ bool any() const { return !(repetition == 1.0f && frequency == 0.0f && presence == 0.0f); }
+  __device__ __forceinline__ float operator()(float y, uint32_t word) const {
+    if (word & (kInPrompt | kUses)) {
+      y = y > 0.0f ? y / repetition : y * repetition;
+      if (word & kUses) y -= fmaf(frequency, (float)(word & kUses), presence);
+    }
+    return y;
+  }
+};
+__device__ __forceinline__ Penalties penalties_of(const LogitArgs& a, uint32_t s) {
+  const float* p = a.penalties + 3 * (uint64_t)s;
+  return {p[0], p[1], p[2]};
+}
+// Entries [begin, end) of the biases are sequence s's.
+struct BiasRange {
+  uint32_t begin, end;
+};
+__device__ __forceinline__ BiasRange biases_of(const LogitArgs& a, uint32_t s) {
+  if (a.bias_entries == 0) return {0, 0};
+  auto within = [&](int t) { return t <= 0 ? 0u : (uint32_t)t < a.bias_entries ? (uint32_t)t : a.bias_entries; };
+  return {within(a.bias_offsets[s]), within(a.bias_offsets[s + 1])};
+}
+// Marks the history of sequence s in a chunk's words.
+__device__ __forceinline__ void mark_history(const LogitArgs& a, uint32_t s, uint32_t* words, uint32_t chunk0, uint32_t tokens) {
   typedef int Four __attribute__((ext_vector_type(4)));
   typedef Four LooseFour __attribute__((aligned(4)));
+  if (a.history_columns == 0) return;
+  const int given = a.history_counts[2 * (uint64_t)s], known = a.history_counts[2 * (uint64_t)s + 1];
+  const uint32_t total = known <= 0 ? 0 : (uint32_t)known < a.history_columns ? (uint32_t)known : a.history_columns;
+  const uint32_t prompt = given <= 0 ? 0 : (uint32_t)given < total ? (uint32_t)given : total;
+  const int* history = a.history + (uint64_t)s * a.history_columns;
+  auto over = [&](uint32_t from, uint32_t upto, auto mark) __attribute__((always_inline)) {
+    for (uint32_t i = from + 4 * threadIdx.x; i < upto; i += 4 * kLogitThreads) {
+      Four t = {-1, -1, -1, -1};
+      if (upto - i >= 4)
+        t = *(const LooseFour*)(history + i);
+      else
+        for (uint32_t k = 0; i + k < upto; ++k) t[k] = history[i + k];
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        if (t[k] >= 0 && (uint32_t)t[k] - chunk0 < tokens) mark(words + ((uint32_t)t[k] - chunk0));
+    }
+  };
+  over(0, prompt, [](uint32_t* word) __attribute__((always_inline)) { atomicOr(word, kInPrompt); });
+  over(prompt, total, [](uint32_t* word) __attribute__((always_inline)) { atomicAdd(word, 1u); });
+}
+
+// A row's logits are loaded first of all, and adjusted in registers.
+template <typename T>
+__global__ __launch_bounds__(kLogitThreads, 8) void adjust_row_kernel(LogitArgs a, uint32_t first_row) {
+  using P = LogitPacks<T>;
   __shared__ __attribute__((aligned(16))) uint32_t words[kChunk];
-  // A biased token's 1 + last entry, then that entry's value.
-  __shared__ __attribute__((aligned(16))) uint32_t bias[kChunk];
+  __shared__ __attribute__((aligned(16))) uint32_t entry[kChunk];  // a biased token's 1 + last entry
+  const uint32_t chunk0 = blockIdx.x * kChunk, row = first_row + blockIdx.y, tid = threadIdx.x;
+  const uint32_t tokens = a.columns - chunk0 < kChunk ? a.columns - chunk0 : kChunk;
+  P p;
+  p.load(a, row, chunk0, tokens);
+  PagedBatch b{};
+  b.row_offsets = a.row_offsets;
+  b.sequences = a.sequences;
+  const uint32_t s = uniform(find_sequence(b, row));
+  if (s >= a.sequences) return;
+  const LogitRows all = logit_rows(a, s);
+  if (row < all.first) return;
+  const Penalties penalties = penalties_of(a, s);
+  const BiasRange biases = biases_of(a, s);
+  for (uint32_t i = tid; i < kChunk / 4; i += kLogitThreads) {
+    *reinterpret_cast<u32x4*>(words + 4 * i) = u32x4{0, 0, 0, 0};
+    if (biases.begin < biases.end) *reinterpret_cast<u32x4*>(entry + 4 * i) = u32x4{0, 0, 0, 0};
+  }
+  __syncthreads();
+  auto inside = [&](int t) __attribute__((always_inline)) { return t >= 0 && (uint32_t)t - chunk0 < tokens; };
+  if (penalties.any()) {
+    mark_history(a, s, words, chunk0, tokens);
+    for (uint32_t j = tid; j < all.rows; j += kLogitThreads) {
+      const bool stands = a.mask_words == 0 ? j <= row - all.first
+                                            : j / 32 < a.mask_words && (a.mask[(uint64_t)row * a.mask_words + j / 32] >> j % 32 & 1);
+      const int t = stands ? a.tokens[all.first + j] : -1;
+      if (inside(t)) atomicAdd(words + ((uint32_t)t - chunk0), 1u);
+    }
+  }
+  for (uint32_t i = biases.begin + tid; i < biases.end; i += kLogitThreads) {
+    const int t = a.biases[2 * (uint64_t)i];
+    if (inside(t)) {
+      atomicOr(words + ((uint32_t)t - chunk0), kBiased);
+      atomicMax(entry + ((uint32_t)t - chunk0), 1 + i);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < P::kPacks; ++i) {
+    const uint32_t at = P::place(i);
+    uint32_t word[P::kPer], any = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < P::kPer; k += 4) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(words + at + k);
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        word[k + e] = w[e];
+        any |= w[e];
+      }
+    }
+    if (any == 0) continue;
+#pragma unroll
+    for (uint32_t k = 0; k < P::kPer; ++k)
+      if (word[k] != 0) {
+        float y = penalties((float)p.x[i][k], word[k]);
+        if (word[k] & kBiased) y += __int_as_float(a.biases[2 * (uint64_t)(entry[at + k] - 1) + 1]);
+        p.x[i][k] = (T)y;
+      }
+  }
+  p.store(a, row, chunk0, tokens);
+}
+
+// A workgroup takes up to `group` rows of a sequence, one after the other, and counts the history
+// once for them; the few tokens that anything changes are listed.  A row's logits pass from registers through LDS back to registers, where
+// between two barriers the listed ones are adjusted, a thread each: a test of every token in
+// its registers costs more, since most waves hold a listed one.  The next row's logits and mask
+// words are on their way meanwhile.
+template <typename T>
+__global__ __launch_bounds__(kLogitThreads, 8) void adjust_rows_kernel(LogitArgs a, uint32_t first_unit, uint32_t group) {
+  using P = LogitPacks<T>;
+  constexpr uint32_t kSlots = kChunk / kLogitThreads;  // of the list, per thread
+  __shared__ __attribute__((aligned(16))) uint32_t words[kChunk];
+  // A row's logits; before the first row a biased token's 1 + last entry.
+  __shared__ __attribute__((aligned(16))) uint32_t stage[kChunk];
+  __shared__ __attribute__((aligned(16))) uint16_t list[kChunk];  // before it is written, the waves' counts of it
   const uint32_t chunk0 = blockIdx.x * kChunk, tid = threadIdx.x;
   const uint32_t tokens = a.columns - chunk0 < kChunk ? a.columns - chunk0 : kChunk;
 
@@ -54,190 +217,145 @@ __global__ __launch_bounds__(kLogitThreads, 8) void adjust_logits_kernel(LogitAr
   const uint32_t row0 = all.first + (unit - (uint32_t)found.first) * group, left = all.first + all.rows - row0;
   const uint32_t rows = left < group ? left : group;
 
-  // Pack i of a thread: the tokens from place(i) on.
-  auto place = [&](uint32_t i) __attribute__((always_inline)) { return (i * kLogitThreads + tid) * kPer; };
-  Pack next[kPacks];
-  uint32_t next_bits[kPacks], next_path = 0;
+  P next;
+  uint32_t next_path = 0;
   auto load = [&](uint32_t row) __attribute__((always_inline)) {
-    const T* from = (const T*)a.logits + (uint64_t)row * a.input_row_stride + chunk0;
-    const uint32_t* allowed = a.allowed + (uint64_t)row * a.allowed_words + chunk0 / 32;
-#pragma unroll
-    for (uint32_t i = 0; i < kPacks; ++i) {
-      const uint32_t at = place(i);
-      next_bits[i] = ~0u;
-      if (at < tokens && a.allowed_words) next_bits[i] = allowed[at / 32];
-      if (at + kPer <= tokens) {
-        next[i] = __builtin_nontemporal_load((const Loose*)(from + at));
-      } else {
-#pragma unroll
-        for (uint32_t k = 0; k < kPer; ++k)
-          if (at + k < tokens) next[i][k] = from[at + k];
-      }
-    }
+    next.load(a, row, chunk0, tokens);
     if (tid < all.rows && tid / 32 < a.mask_words) next_path = a.mask[(uint64_t)row * a.mask_words + tid / 32];
   };
   load(row0);
-  const float repetition = a.penalties[3 * (uint64_t)s], frequency = a.penalties[3 * (uint64_t)s + 1];
-  const float presence = a.penalties[3 * (uint64_t)s + 2], inverse = 1.0f / repetition;
-  const bool penal = !(repetition == 1.0f && frequency == 0.0f && presence == 0.0f);
+  const Penalties penalties = penalties_of(a, s);
+  const BiasRange biases = biases_of(a, s);
+  const uint32_t begin = biases.begin, end = biases.end;
+  const bool penal = penalties.any();
   auto inside = [&](int t) __attribute__((always_inline)) { return t >= 0 && (uint32_t)t - chunk0 < tokens; };
   const int token = tid < all.rows ? a.tokens[all.first + tid] : -1;  // of the sequence's row `tid`
-  uint32_t begin = 0, end = 0;                                       // biases
-  if (a.bias_entries > 0) {
-    auto within = [&](int t) { return t <= 0 ? 0u : (uint32_t)t < a.bias_entries ? (uint32_t)t : a.bias_entries; };
-    begin = within(a.bias_offsets[s]);
-    end = within(a.bias_offsets[s + 1]);
-  }
 
-  // ---- the history's tokens, and the biases' ----
+  // ---- the tokens of the history, the paths and the biases ----
   for (uint32_t i = tid; i < kChunk / 4; i += kLogitThreads) {
     *reinterpret_cast<u32x4*>(words + 4 * i) = u32x4{0, 0, 0, 0};
-    if (begin < end) *reinterpret_cast<u32x4*>(bias + 4 * i) = u32x4{0, 0, 0, 0};
+    if (begin < end) *reinterpret_cast<u32x4*>(stage + 4 * i) = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
-  if (penal && a.history_columns > 0) {
-    const int given = a.history_counts[2 * (uint64_t)s], known = a.history_counts[2 * (uint64_t)s + 1];
-    const uint32_t total = known <= 0 ? 0 : (uint32_t)known < a.history_columns ? (uint32_t)known : a.history_columns;
-    const uint32_t prompt = given <= 0 ? 0 : (uint32_t)given < total ? (uint32_t)given : total;
-    const int* history = a.history + (uint64_t)s * a.history_columns;
-    auto use = [&](int t, bool in_prompt) __attribute__((always_inline)) {
-      if (inside(t)) in_prompt ? atomicOr(words + (t - chunk0), kInPrompt) : atomicAdd(words + (t - chunk0), 1u);
-    };
-    for (uint32_t i = 4 * tid; i < total; i += 4 * kLogitThreads) {
-      if (total - i >= 4) {
-        const Four t = *(const LooseFour*)(history + i);
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) use(t[k], i + k < prompt);
-      } else {
-        for (uint32_t k = 0; i + k < total; ++k) use(history[i + k], i + k < prompt);
-      }
+  if (penal) {
+    mark_history(a, s, words, chunk0, tokens);
+    if (inside(token)) atomicOr(words + (token - chunk0), kInPath);
+    for (uint32_t j = tid + kLogitThreads; j < all.rows; j += kLogitThreads) {
+      const int t = a.tokens[all.first + j];
+      if (inside(t)) atomicOr(words + (t - chunk0), kInPath);
     }
   }
-  // A token's last entry is found by its number, then its value put in its place: 32 entries
-  // of a thread at a time, from the end of the list, so that later ones are there already.
-  for (uint32_t upto = end; upto > begin;) {
-    constexpr uint32_t kAtOnce = 32 * kLogitThreads;
-    const uint32_t from = upto - begin > kAtOnce ? upto - kAtOnce : begin;
-    uint32_t lasts = 0;
-    auto over = [&](auto f) __attribute__((always_inline)) {
-      for (uint32_t k = 0; k < 32 && from + k * kLogitThreads + tid < upto; ++k) {
-        const int t = a.biases[2 * (uint64_t)(from + k * kLogitThreads + tid)];
-        if (inside(t)) f(k, (uint32_t)t - chunk0);
-      }
-    };
-    over([&](uint32_t k, uint32_t at) __attribute__((always_inline)) {
-      if (!(words[at] & kBiased)) {
-        lasts |= 1u << k;
-        atomicMax(bias + at, 1 + k * kLogitThreads + tid);
-      }
-    });
-    __syncthreads();
-    over([&](uint32_t k, uint32_t at) __attribute__((always_inline)) {
-      if (bias[at] != 1 + k * kLogitThreads + tid) lasts &= ~(1u << k);
-    });
-    __syncthreads();
-    over([&](uint32_t k, uint32_t at) __attribute__((always_inline)) {
-      if (lasts >> k & 1) {
-        bias[at] = (uint32_t)a.biases[2 * (uint64_t)(from + k * kLogitThreads + tid) + 1];
-        atomicOr(words + at, kBiased);
-      }
-    });
-    upto = from;
-    if (upto > begin) __syncthreads();
+  for (uint32_t i = begin + tid; i < end; i += kLogitThreads) {
+    const int t = a.biases[2 * (uint64_t)i];
+    if (inside(t)) {
+      atomicOr(words + (t - chunk0), kBiased);
+      atomicMax(stage + (t - chunk0), 1 + i);
+    }
   }
+  __syncthreads();
+  // The list.
+  uint32_t count = 0;
+  {
+    uint32_t mine = 0;
+    u32x4 w[kSlots / 4];
+#pragma unroll
+    for (uint32_t q = 0; q < kSlots / 4; ++q) {
+      w[q] = *reinterpret_cast<const u32x4*>(words + 4 * (q * kLogitThreads + tid));
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) mine += w[q][k] != 0;
+    }
+    const uint32_t upto = scan(mine), wave = tid / kWave;
+    uint32_t* const counts = reinterpret_cast<uint32_t*>(list);
+    if (tid % kWave == kWave - 1) counts[wave] = upto;
+    __syncthreads();
+    uint32_t at = upto - mine;
+#pragma unroll
+    for (uint32_t v = 0; v < kLogitThreads / kWave; ++v) {
+      if (v == wave) at += count;
+      count += counts[v];
+    }
+    count = uniform(count);
+    __syncthreads();
+#pragma unroll
+    for (uint32_t q = 0; q < kSlots / 4; ++q)
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        if (w[q][k] != 0) list[at++] = (uint16_t)(4 * (q * kLogitThreads + tid) + k);
+  }
+  if (count > 0) __syncthreads();
+  float value[kSlots];  // biases of this thread's listed tokens
+#pragma unroll
+  for (uint32_t u = 0; u < kSlots; ++u) {
+    value[u] = 0.0f;
+    const uint32_t e = u * kLogitThreads + tid;
+    if (begin < end && e < count && (words[list[e]] & kBiased))
+      value[u] = __int_as_float(a.biases[2 * (uint64_t)(stage[list[e]] - 1) + 1]);
+  }
+  if (begin < end && count > 0) __syncthreads();
 
+  T* const logits = reinterpret_cast<T*>(stage);
   uint32_t before = 0;  // whether this thread's token stood in the path of the row before
   for (uint32_t r = 0; r < rows; ++r) {
     const uint32_t row = row0 + r, path = next_path;
-    Pack x[kPacks];
-    uint32_t bits[kPacks];
-#pragma unroll
-    for (uint32_t i = 0; i < kPacks; ++i) {
-      x[i] = next[i];
-      bits[i] = next_bits[i];
-    }
+    P p = next;
     if (r + 1 < rows) load(row + 1);
-    if (penal) {
-      if (r > 0) __syncthreads();  // the row before has read its words
-      // This row's path on, the last one's off.
-      const uint32_t index = row - all.first;
-      const uint32_t mine = inside(token) && (a.mask_words ? path >> tid % 32 & 1 : tid <= index);
-      if (mine != before) mine ? atomicAdd(words + (token - chunk0), 1u) : atomicSub(words + (token - chunk0), 1u);
-      before = mine;
-      for (uint32_t j = tid + kLogitThreads; j < all.rows; j += kLogitThreads) {  // long paths
-        auto stands = [&](uint32_t i) __attribute__((always_inline)) {
-          if (a.mask_words == 0) return j <= i;
-          return j / 32 < a.mask_words && (a.mask[(uint64_t)(all.first + i) * a.mask_words + j / 32] >> j % 32 & 1) != 0;
-        };
-        const bool now = stands(index), was = r > 0 && stands(index - 1);
-        if (now == was) continue;
-        const int t = a.tokens[all.first + j];
-        if (inside(t)) now ? atomicAdd(words + (t - chunk0), 1u) : atomicSub(words + (t - chunk0), 1u);
-      }
-    }
-    if (penal || r == 0) __syncthreads();
-
-    auto adjust = [&](float y, uint32_t word, uint32_t at) __attribute__((always_inline)) {
-      const uint32_t uses = word & kUses;
-      if (word & ~kBiased) {
-        // y / repetition, rounded once: the quotient by the inverse, and what it leaves.
-        const float quotient = y * inverse, rest = fmaf(-quotient, repetition, y), better = fmaf(rest, inverse, quotient);
-        const float less = fabsf(better) < INFINITY ? better : y / repetition;
-        y = y > 0.0f ? less : y * repetition;
-        if (uses > 0) y -= fmaf(frequency, (float)uses, presence);
-      }
-      if (word & kBiased) y += __uint_as_float(bias[at]);
-      return y;
-    };
-    T* to = (T*)a.out + (uint64_t)row * a.output_row_stride + chunk0;
+    if (count > 0) {
 #pragma unroll
-    for (uint32_t i = 0; i < kPacks; ++i) {
-      const uint32_t at = place(i);
-      if (at >= tokens) continue;
-      uint32_t word[kPer], any = 0;
-#pragma unroll
-      for (uint32_t k = 0; k < kPer; k += 4) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(words + at + k);
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-          word[k + e] = w[e];
-          any |= w[e];
+      for (uint32_t i = 0; i < P::kPacks; ++i) *reinterpret_cast<typename P::Pack*>(logits + P::place(i)) = p.x[i];
+      if (penal) {
+        // This row's path on, the last one's off.
+        const uint32_t index = row - all.first;
+        const uint32_t mine = inside(token) && (a.mask_words ? path >> tid % 32 & 1 : tid <= index);
+        if (mine != before) mine ? atomicAdd(words + (token - chunk0), 1u) : atomicSub(words + (token - chunk0), 1u);
+        before = mine;
+        for (uint32_t j = tid + kLogitThreads; j < all.rows; j += kLogitThreads) {  // long paths
+          auto stands = [&](uint32_t i) __attribute__((always_inline)) {
+            if (a.mask_words == 0) return j <= i;
+            return j / 32 < a.mask_words && (a.mask[(uint64_t)(all.first + i) * a.mask_words + j / 32] >> j % 32 & 1) != 0;
+          };
+          const bool now = stands(index), was = r > 0 && stands(index - 1);
+          if (now == was) continue;
+          const int t = a.tokens[all.first + j];
+          if (inside(t)) now ? atomicAdd(words + (t - chunk0), 1u) : atomicSub(words + (t - chunk0), 1u);
         }
       }
-      if (any) {
+      __syncthreads();
 #pragma unroll
-        for (uint32_t k = 0; k < kPer; ++k)
-          if (word[k]) x[i][k] = (T)adjust((float)x[i][k], word[k], at + k);
+      for (uint32_t u = 0; u < kSlots; ++u) {
+        if (u * kLogitThreads >= count) break;
+        const uint32_t e = u * kLogitThreads + tid;
+        if (e >= count) break;
+        const uint32_t at = list[e], word = words[at];
+        float y = penalties((float)logits[at], word);
+        if (word & kBiased) y += value[u];
+        logits[at] = (T)y;
       }
-      const uint32_t allowed = bits[i] >> at % 32;
+      __syncthreads();
 #pragma unroll
-      for (uint32_t k = 0; k < kPer; ++k) x[i][k] = allowed >> k & 1 ? x[i][k] : (T)-INFINITY;
-      if (at + kPer <= tokens) {
-        __builtin_nontemporal_store(x[i], (Loose*)(to + at));
-      } else {
-#pragma unroll
-        for (uint32_t k = 0; k < kPer; ++k)
-          if (at + k < tokens) to[at + k] = x[i][k];
-      }
+      for (uint32_t i = 0; i < P::kPacks; ++i) p.x[i] = *reinterpret_cast<const typename P::Pack*>(logits + P::place(i));
     }
+    p.store(a, row, chunk0, tokens);
   }
 }
 
-// Rows of a workgroup: all of a sequence's, as far as that leaves two rounds of the workgroups
-// that the chip holds (four per CU).
+// Several rows per workgroup where sequences have them and there are enough for two rounds of the
+// workgroups that the chip holds (four per CU), but not so many that the last round is long.
 template <typename T>
 int launch_as(hipStream_t stream, const LogitArgs& a) {
   constexpr uint64_t kWant = 2 * 4 * 256, kMostUnits = 65535;  // the grid's second dimension
+  constexpr uint64_t kMostGroup = sizeof(T) == 4 ? 4 : 8;
   const uint64_t chunks = ((uint64_t)a.columns + kChunk - 1) / kChunk;
   uint64_t group = a.rows * chunks / kWant;
-  group = group < 1 ? 1 : group > 64 ? 64 : group;
-  if (a.sequences * chunks >= kWant) group = 64;
+  group = group < 1 || a.rows <= a.sequences ? 1 : group > kMostGroup ? kMostGroup : group;
   // At most a partial group more for each sequence.
-  uint64_t units = a.rows / group + a.sequences;
+  uint64_t units = group == 1 ? a.rows : a.rows / group + a.sequences;
   if (units > a.rows) units = a.rows;
   for (uint64_t done = 0; done < units; done += kMostUnits) {
-    hipLaunchKernelGGL(adjust_logits_kernel<T>, dim3((uint32_t)chunks, (uint32_t)(units - done < kMostUnits ? units - done : kMostUnits)),
-                       dim3(kLogitThreads), 0, stream, a, (uint32_t)done, (uint32_t)group);
+    const dim3 grid((uint32_t)chunks, (uint32_t)(units - done < kMostUnits ? units - done : kMostUnits));
+    if (group == 1)
+      hipLaunchKernelGGL(adjust_row_kernel<T>, grid, dim3(kLogitThreads), 0, stream, a, (uint32_t)done);
+    else
+      hipLaunchKernelGGL(adjust_rows_kernel<T>, grid, dim3(kLogitThreads), 0, stream, a, (uint32_t)done, (uint32_t)group);
     if (int e = hip_status(hipGetLastError())) return e;
   }
   return 0;

@@ -708,8 +708,8 @@ int run_keep_pages(ipus_context* c, void* o, const void* const* i, const uint32_
 int check_adjust_logits(const uint32_t* s) {
   if (s[0] > 0x7fffffff || s[1] > 0x7fffffff || s[2] == 0 || s[2] > 0x7fffffff || s[7] > 0x7fffffff)
     return IPUS_ERROR_INVALID_ARGUMENT;
-  // A token's uses are counted in 30 bits.
-  if (s[3] < s[2] || s[4] < s[2] || (uint64_t)s[6] + s[1] >= 1u << 30) return IPUS_ERROR_INVALID_ARGUMENT;
+  // A token's uses are counted in 29 bits.
+  if (s[3] < s[2] || s[4] < s[2] || (uint64_t)s[6] + s[1] >= 1u << 29) return IPUS_ERROR_INVALID_ARGUMENT;
   return s[8] != 0 && (uint64_t)s[8] * 32 < s[2] ? IPUS_ERROR_INVALID_ARGUMENT : 0;
 }
 int run_adjust_logits(ipus_context* c, void* o, const void* const* i, const uint32_t* s, bool f32) {
