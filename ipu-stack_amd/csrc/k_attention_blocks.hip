@@ -81,6 +81,68 @@ __device__ __forceinline__ uint64_t blocks_of(const BatchSequence& q, uint32_t g
   return queries <= few ? 0 : (uint64_t)((queries + Queries - 1) / Queries) * key_heads;
 }
 
+// A tree's rows all read their sequence's keys, and a batch's sequences may be of very different
+// lengths: the key blocks of a part at most, by all of them, so that the work is even.  Costs
+// in key blocks: of as many parts as the chip holds workgroups, the longest; of twice as many,
+// which follow one another, an even share and the longest; the join, where there are parts.
+// Parts of fewer than kTreePart cost more than they save.  us, 32 query heads on 8 x 128, so /
+// by the rule of the other rows: 64 trees of 8 to 16 rows against 256 to 4096 keys 101 / 118, 40
+// of 12 to 24 against up to 3000 (96 columns) 47 / 77, 16 of 64 against 8192 186 / 198; where
+// no part is of use the join's launch is lost, 20 of 64 against 2000 77 / 74.
+constexpr uint32_t kJoinBlocks = 8, kTreePart = 12, kPlannedSequences = 256;
+struct TreeWork {
+  uint32_t blocks, key_blocks;  // query blocks of all key heads of a sequence, key blocks of each
+  __device__ __forceinline__ uint32_t parts(uint32_t each) const {
+    return key_blocks < kLeastSplit || each >= key_blocks ? 1 : (key_blocks + each - 1) / each;
+  }
+};
+// held: of the first 64 sequences, one per lane.
+template <typename F>
+__device__ __forceinline__ uint32_t tree_part(const PagedBatch& b, uint32_t most_parts, const TreeWork& held, F work) {
+  const uint32_t lane = threadIdx.x % kWave;
+  uint64_t steps = (uint64_t)held.blocks * held.key_blocks, total = held.blocks;
+  uint32_t longest = held.blocks > 0 ? held.key_blocks : 0;
+  for (uint32_t s = kWave + lane; s < b.sequences; s += kWave) {
+    const TreeWork w = work(s);
+    steps += (uint64_t)w.blocks * w.key_blocks;
+    total += w.blocks;
+    if (w.blocks > 0 && w.key_blocks > longest) longest = w.key_blocks;
+  }
+  longest = largest(longest);
+  total = from_lane(scan(total), kWave - 1);
+  if (most_parts <= 1 || longest < kLeastSplit || total > 2 * kFullChip || b.sequences > kPlannedSequences) return longest;
+  const uint32_t share = (uint32_t)((from_lane(scan(steps), kWave - 1) + kFullChip - 1) / kFullChip);
+  uint32_t least = (longest + most_parts - 1) / most_parts;
+  if (least < kTreePart) least = kTreePart;
+  auto smallest = [&](uint32_t room) __attribute__((always_inline)) {  // of which there are at most `room`
+    uint32_t low = least, high = longest;
+    while (low < high) {
+      const uint32_t each = (low + high) / 2;
+      uint32_t items = held.blocks * held.parts(each);
+      for (uint32_t s = kWave + lane; s < b.sequences; s += kWave) {
+        const TreeWork w = work(s);
+        items += w.blocks * w.parts(each);
+      }
+      if ((uint32_t)__builtin_amdgcn_readlane(scan(items), kWave - 1) <= room)
+        high = each;
+      else
+        low = each + 1;
+    }
+    return low;
+  };
+  uint32_t best = longest, cost = total <= kFullChip ? longest : share + longest;
+  if (total <= kFullChip) {
+    const uint32_t each = smallest(kFullChip);
+    if (each + kJoinBlocks < cost) {
+      best = each;
+      cost = each + kJoinBlocks;
+    }
+  }
+  if (share + least + kJoinBlocks >= cost) return best;
+  const uint32_t each = smallest(2 * kFullChip);
+  return share + each + kJoinBlocks < cost ? each : best;
+}
+
 // Shared: the rows of the whole batch over the keys below shared_rows, as parts for
 // another launch.  Tree: the masks of a sequence's rows, looked up for the key blocks that hold
 // their keys.
@@ -111,7 +173,34 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   uint32_t queries;                   // of the sequence
   uint64_t block;                     // in the line of all blocks
   uint32_t part, splits = split.parts;
-  {
+  if constexpr (Tree) {
+    auto work = [&](uint32_t x) __attribute__((always_inline)) {
+      const BatchSequence w = sequence_at(b, x, a.rows);
+      return TreeWork{(uint32_t)blocks_of<kQueries>(w, group, a.key_heads, few), (w.keys + kKeys - 1) / kKeys};
+    };
+    const TreeWork held = lane < b.sequences ? work(lane) : TreeWork{0, 0};
+    const uint32_t each = tree_part(b, split.parts, held, work);
+    auto items_in = [&](uint32_t x) __attribute__((always_inline)) {
+      const TreeWork w = work(x);
+      return (uint64_t)w.blocks * w.parts(each);
+    };
+    UnitLine line{scan((uint64_t)held.blocks * held.parts(each)), 0};
+    line.total = from_lane(line.upto, kWave - 1);
+    if (b.sequences > (uint32_t)kWave) line = count_units(b, items_in);
+    // An XCD's range of the line: what reads the same keys stands together.
+    const uint64_t per_xcd = (line.total + 7) / 8, local = blockIdx.x / 8, item = blockIdx.x % 8 * per_xcd + local;
+    if (local >= per_xcd || item >= line.total || item >= gridDim.x) return;
+    const UnitPlace place = find_unit(b, line, item, items_in);
+    s = place.sequence;
+    q = uniform(sequence_at(b, s, a.rows));
+    queries = q.rows * group;
+    const uint32_t per_head = (queries + kQueries - 1) / kQueries, within = (uint32_t)(item - place.first);
+    splits = work(s).parts(each);
+    const uint32_t keys_of = within / per_head;  // of one key head and part
+    key_head = keys_of / splits;
+    part = keys_of - key_head * splits;
+    query0 = (within - keys_of * per_head) * kQueries;
+  } else {
     auto blocks_in = [&](uint32_t x) __attribute__((always_inline)) {
       return blocks_of<kQueries>(sequence_at(b, x, a.rows), group, a.key_heads, few);
     };
@@ -222,8 +311,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   // This part's: every part has a block of keys, but for the first of none at all.
   const uint32_t all_blocks = (key_end + kKeys - 1) / kKeys;
   uint32_t per_part = (all_blocks + splits - 1) / splits;
-  if (!Shared && splits > 1 && per_part < kLeastPart) per_part = kLeastPart;
-  if (!Shared && all_blocks < kLeastSplit) per_part = all_blocks;
+  if (!Shared && !Tree && splits > 1 && per_part < kLeastPart) per_part = kLeastPart;
+  if (!Shared && !Tree && all_blocks < kLeastSplit) per_part = all_blocks;
   if (per_part == 0) per_part = 1;
   uint32_t parts = (all_blocks + per_part - 1) / per_part;
   if (parts == 0) parts = 1;
@@ -350,7 +439,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
   };
   // Of the 64 keys from key0 on, those that the mask of query 16 qt + l % 16 names.
   auto seen = [&](uint32_t qt, uint32_t key0) __attribute__((always_inline)) {
-    uint32_t m = wave0 + 16 * qt + r16;
+    uint32_t m = threadIdx.x % 16;
+    asm volatile("" : "+v"(m));  // nothing of this is kept in registers
+    m += wave0 + 16 * qt;
     m = m < queries ? m : queries - 1;
     return tree_window(a.tree_mask + (uint64_t)(q.first + m / group) * a.mask_words, tree, key0);
   };
@@ -635,8 +726,11 @@ int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2,
   uint64_t least = 0;
   if (few == 0 && (uint64_t)a.batch.sequences * a.max_rows == a.rows)
     least = ((uint64_t)a.max_rows * (a.query_heads / a.key_heads) + kQueries - 1) / kQueries * a.batch.sequences * a.key_heads;
-  const bool may_split = least < kFullChip / 2 && reach > (uint64_t)(kLeastSplit - 1) * Block<D, QT>::kKeys;
-  if (!Shared && a.workspace.data && blocks < kFullChip && may_split) {
+  const uint64_t room = Tree ? 2 * kFullChip + 1 : kFullChip / 2;  // tree_part
+  const bool may_split = least < room && !(Tree && a.batch.sequences > kPlannedSequences) &&
+                         reach > (uint64_t)(kLeastSplit - 1) * Block<D, QT>::kKeys;
+  const uint64_t most = Tree ? 4 * kFullChip : kFullChip;
+  if (!Shared && a.workspace.data && blocks < most && may_split) {
     const uint64_t rows = (uint64_t)a.rows * a.query_heads;
     uint64_t parts = a.workspace.bytes / sizeof(float) / rows;  // floats per row, then parts
     parts = parts > 0 ? (parts - 1) / (a.width + 2) : 0;
@@ -650,14 +744,16 @@ int launch_as(hipStream_t stream, const PagedAttentionArgs& a, float scale_log2,
   }
   // Split blocks make at most kFullChip workgroups, in ranges of whole blocks' parts (Shared: the
   // given parts of each).
+  // Tree: whole blocks, or parts of which there are at most twice kFullChip.
   uint64_t grid = Shared ? blocks * split.parts : split.parts > 1 ? kFullChip + 8 * kMaxSplits : blocks;
+  if (Tree) grid = split.parts > 1 && blocks < 2 * kFullChip ? 2 * kFullChip : blocks;
   grid = (grid + 7) / 8 * 8;
   if (grid > 0xffffffull) return IPUS_ERROR_UNAVAILABLE;  // a grid dimension holds less than 2^32 threads
   hipLaunchKernelGGL((attention_blocks_kernel<D, DC, QT, Shared, Tree>), dim3((uint32_t)grid), dim3(kThreads), 0, stream, a,
                      scale_log2, few, split);
   if (int e = hip_status(hipGetLastError())) return e;
   if (Shared || split.parts <= 1) return 0;
-  // Fewer than kFullChip blocks hold fewer than 2^16 rows.
+  // So few blocks hold fewer than 2^20 rows.
   hipLaunchKernelGGL(join_parts_kernel, dim3(a.rows, (a.query_heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, a,
                      few, split);
   return hip_status(hipGetLastError());

@@ -120,7 +120,8 @@ __device__ __forceinline__ void mark_history(const LogitArgs& a, uint32_t s, uin
   over(prompt, total, [](uint32_t* word) __attribute__((always_inline)) { atomicAdd(word, 1u); });
 }
 
-// A row's logits are loaded first of all, and adjusted in registers.
+// A row's logits are on their way while its history is counted, and adjusted in registers.
+// They are asked for behind what the counting waits for: loads arrive in order.
 template <typename T>
 __global__ __launch_bounds__(kLogitThreads, 8) void adjust_row_kernel(LogitArgs a, uint32_t first_row) {
   using P = LogitPacks<T>;
@@ -129,7 +130,6 @@ __global__ __launch_bounds__(kLogitThreads, 8) void adjust_row_kernel(LogitArgs 
   const uint32_t chunk0 = blockIdx.x * kChunk, row = first_row + blockIdx.y, tid = threadIdx.x;
   const uint32_t tokens = a.columns - chunk0 < kChunk ? a.columns - chunk0 : kChunk;
   P p;
-  p.load(a, row, chunk0, tokens);
   PagedBatch b{};
   b.row_offsets = a.row_offsets;
   b.sequences = a.sequences;
@@ -139,6 +139,7 @@ __global__ __launch_bounds__(kLogitThreads, 8) void adjust_row_kernel(LogitArgs 
   if (row < all.first) return;
   const Penalties penalties = penalties_of(a, s);
   const BiasRange biases = biases_of(a, s);
+  p.load(a, row, chunk0, tokens);
   for (uint32_t i = tid; i < kChunk / 4; i += kLogitThreads) {
     *reinterpret_cast<u32x4*>(words + 4 * i) = u32x4{0, 0, 0, 0};
     if (biases.begin < biases.end) *reinterpret_cast<u32x4*>(entry + 4 * i) = u32x4{0, 0, 0, 0};
