@@ -381,6 +381,10 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
     const uint32_t queries = q.rows * group - query0;  // left, at least 1
     half8_t qf[MT][kKS];
     uint32_t limit[MT];  // keys that this lane's query may read
+    // Its mask, where that is one word, asked for with the query (in the last tile, where it is
+    // used, its load would be waited for: 4 trees of 8 rows against 1000 keys 13.3 us, so 13.9).
+    constexpr bool kEarly = Tree && MT == 1;
+    uint32_t early = 0;
 #pragma unroll
     for (uint32_t mt = 0; mt < MT; ++mt) {
       uint32_t m = 16 * mt + r16;
@@ -391,6 +395,7 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
                            (uint64_t)(key_head * group + head) * a.width;
       const int position = row_position(q.length, q.end, row);
       limit[mt] = real ? readable_keys(q, position, a.causal) : 0;
+      if (kEarly) early = a.tree_mask[(uint64_t)row * a.mask_words];
 #pragma unroll
       for (uint32_t ks = 0; ks < kKS; ++ks) {
         const uint32_t d0 = ks * 32 + g4 * 8;
@@ -485,6 +490,7 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
       half8_t high[kHalves][MT], low[kHalves][MT];
       // Of the tile's keys, those that the query's mask names.
       auto seen = [&](uint32_t mt) __attribute__((always_inline)) {
+        if (kEarly && tree.bits <= 32) return tree_window(&early, tree, key0);
         uint32_t m = 16 * mt + opaque(lane) % 16;
         m = m < queries ? m : queries - 1;
         const uint32_t row = q.first + (query0 + m) / group;
