@@ -260,8 +260,8 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        of the previous rows; what sequences need is taken from the end, the
  *        sequences in order.  missing: how many there were too few; the sequences
  *        then hold fewer (their table ends earlier).  A first state: all pages
- *        free, previous_sequences 0.  Up to 4096 sequences; the states must not
- *        overlap.  A page is held once: no prefix is shared.
+ *        free, previous_sequences 0.  Up to 4096 sequences; the new state lies
+ *        apart from the inputs.  A page is held once: no prefix is shared.
  *   ipu_stack_slot_maps   out int32 row_offsets [sequences + 1], positions [rows],
  *        slots [rows], one after the other; counts [sequences] (new rows, below 0
  *        as 0), lengths [sequences] (with them), page_table, the tree's mask;
@@ -271,7 +271,8 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        page_rows + row in the page, -1 where the place has no page.  Its
  *        position is the place, in a tree lengths[s] - n + how many other rows it
  *        reads (its depth), -1 below 0.  Rows behind the last sequence: position
- *        0, slot -1.  pages x page_rows <= 2^31.
+ *        0, slot -1.  pages x page_rows <= 2^31; the output lies apart from the
+ *        inputs.
  *   ipu_stack_attention_tree_pages_f16   as ipu_stack_attention_pages_f16 with the
  *        tree's mask behind the inputs and mask_words (at least 1) in the place of
  *        causal: row i of sequence s reads the keys before its sequence's rows,

@@ -9,6 +9,10 @@
 namespace ipus {
 namespace {
 
+// Whether `bytes` from a on share memory with `others` from b on.
+inline bool overlaps(const void* a, uint64_t bytes, const void* b, uint64_t others) {
+  return (uintptr_t)a < (uintptr_t)b + others && (uintptr_t)b < (uintptr_t)a + bytes;
+}
 inline int hip_status(hipError_t e) { return e == hipSuccess ? 0 : IPUS_ERROR_HIP_BASE - (int)e; }
 
 // Sum over the threads up to this one of a workgroup of Waves waves, and of all; `waves`:
@@ -38,61 +42,71 @@ __device__ __forceinline__ T scan_threads(T x, T* waves, T* all) {
 // state: one launch without a word between workgroups.  Entry i of the list of free pages is
 // the previous list's, behind it the pages given back in the order of the previous rows;
 // pages are taken from its end.
+// The words that decide are loaded first, together, and so is what each thread will most
+// likely write; all else is LDS.
 constexpr uint32_t kTableThreads = 512, kTableWaves = kTableThreads / kWave;
 __global__ __launch_bounds__(kTableThreads) void page_tables_kernel(PageTableArgs a) {
   extern __shared__ uint32_t lds[];
-  uint32_t* const need = lds;                          // [sequences] pages
-  uint32_t* const wanted = need + a.sequences;         // pages to take, of the sequences up to and with
-  uint32_t* const owner = wanted + a.sequences;        // [previous] the sequence that goes on with the row
-  uint32_t* const back = owner + a.previous_sequences;  // pages given back, of the rows up to and with
+  uint32_t* const need = lds;                           // [sequences] pages
+  uint32_t* const wanted = need + a.sequences;          // first the sources; then pages to take, of those up to and with
+  uint32_t* const owner = wanted + a.sequences;         // [previous] the sequence that goes on with the row
+  uint32_t* const back = owner + a.previous_sequences;  // first those held; then given back, of the rows up to and with
   __shared__ uint32_t waves[kTableWaves];
   const uint32_t tid = threadIdx.x;
   const int* const spare = a.previous + 2;
   const int* const held = spare + a.pages;
   const int* const old = held + a.previous_sequences;
-  auto held_at = [&](uint32_t p) __attribute__((always_inline)) {
-    const int h = held[p];
-    return h <= 0 ? 0u : (uint32_t)h < a.columns ? (uint32_t)h : a.columns;
+  auto within = [](int x, uint32_t most) __attribute__((always_inline)) {
+    return x <= 0 ? 0u : (uint32_t)x < most ? (uint32_t)x : most;
   };
-  const int listed = a.previous[0];
-  const uint32_t free = listed <= 0 ? 0u : (uint32_t)listed < a.pages ? (uint32_t)listed : a.pages;
+  const uint32_t across = (a.columns + kTableThreads - 1) / kTableThreads;
+  const uint64_t spare0 = (uint64_t)blockIdx.x * kTableThreads + tid;
+  const uint32_t s0 = across > 0 && blockIdx.x / across < a.sequences ? blockIdx.x / across : 0;
+  const uint32_t c0 = (blockIdx.x - s0 * across) * kTableThreads + tid;
 
-  for (uint32_t p = tid; p < a.previous_sequences; p += kTableThreads) owner[p] = a.sequences;
+  const uint32_t free = within(a.previous[0], a.pages);
+  const int early_spare = spare0 < a.pages ? spare[spare0] : -1;
+  for (uint32_t p = tid; p < a.previous_sequences; p += kTableThreads) {
+    owner[p] = a.sequences;
+    back[p] = within(held[p], a.columns);
+  }
   for (uint32_t s = tid; s < a.sequences; s += kTableThreads) {
     const int length = a.lengths[s];
     const uint32_t pages = length <= 0 ? 0 : (((uint32_t)length - 1) >> a.page_shift) + 1;
     need[s] = pages < a.columns ? pages : a.columns;
+    wanted[s] = (uint32_t)a.source[s];
   }
   __syncthreads();
+  const uint32_t from0 = a.sequences > 0 ? wanted[s0] : ~0u;
+  const int early_page = from0 < a.previous_sequences && c0 < a.columns ? old[(uint64_t)from0 * a.columns + c0] : -1;
   for (uint32_t s = tid; s < a.sequences; s += kTableThreads) {
-    const uint32_t from = (uint32_t)a.source[s];
+    const uint32_t from = wanted[s];
     if (from < a.previous_sequences) atomicMin(owner + from, s);
   }
   __syncthreads();
   uint32_t given = 0, taken = 0;  // in all
-  for (uint32_t p0 = 0; p0 < a.previous_sequences; p0 += kTableThreads) {
-    const uint32_t p = p0 + tid;
-    uint32_t x = 0, all;
-    if (p < a.previous_sequences) {
-      const uint32_t h = held_at(p), o = owner[p], stay = o < a.sequences ? need[o] : 0;
-      x = h > stay ? h - stay : 0;
-    }
-    const uint32_t upto = given + scan_threads<kTableWaves>(x, waves, &all);
-    if (p < a.previous_sequences) back[p] = upto;
-    given += all;
-    __syncthreads();
-  }
-  for (uint32_t s0 = 0; s0 < a.sequences; s0 += kTableThreads) {
-    const uint32_t s = s0 + tid;
+  for (uint32_t s1 = 0; s1 < a.sequences; s1 += kTableThreads) {
+    const uint32_t s = s1 + tid;
     uint32_t x = 0, all;
     if (s < a.sequences) {
-      const uint32_t from = (uint32_t)a.source[s];
-      const uint32_t base = from < a.previous_sequences && owner[from] == s ? held_at(from) : 0;
+      const uint32_t from = wanted[s], base = from < a.previous_sequences && owner[from] == s ? back[from] : 0;
       x = need[s] > base ? need[s] - base : 0;
     }
     const uint32_t upto = taken + scan_threads<kTableWaves>(x, waves, &all);
     if (s < a.sequences) wanted[s] = upto;
     taken += all;
+    __syncthreads();
+  }
+  for (uint32_t p0 = 0; p0 < a.previous_sequences; p0 += kTableThreads) {
+    const uint32_t p = p0 + tid;
+    uint32_t x = 0, all;
+    if (p < a.previous_sequences) {
+      const uint32_t h = back[p], o = owner[p], stay = o < a.sequences ? need[o] : 0;
+      x = h > stay ? h - stay : 0;
+    }
+    const uint32_t upto = given + scan_threads<kTableWaves>(x, waves, &all);
+    if (p < a.previous_sequences) back[p] = upto;
+    given += all;
     __syncthreads();
   }
   const uint32_t total = free + given;
@@ -108,22 +122,25 @@ __global__ __launch_bounds__(kTableThreads) void page_tables_kernel(PageTableArg
       low = before ? low + half + 1 : low;
       count = before ? count - half - 1 : half;
     }
-    const uint32_t first = low > 0 ? back[low - 1] : 0, column = held_at(low) - (back[low] - first) + (i - first);
+    const uint32_t first = low > 0 ? back[low - 1] : 0;
+    const uint32_t column = within(held[low], a.columns) - (back[low] - first) + (i - first);
     return old[(uint64_t)low * a.columns + column];
   };
   int* const out_spare = a.out + 2;
   int* const out_held = out_spare + a.pages;
   int* const out_table = out_held + a.sequences;
-  for (uint64_t i = (uint64_t)blockIdx.x * kTableThreads + tid; i < a.pages; i += (uint64_t)gridDim.x * kTableThreads)
-    out_spare[i] = i < left ? listed_page((uint32_t)i) : -1;
-  const uint32_t across = (a.columns + kTableThreads - 1) / kTableThreads;
+  for (uint64_t i = spare0; i < a.pages; i += (uint64_t)gridDim.x * kTableThreads) {
+    int page = -1;
+    if (i < left) page = i == spare0 && i < free ? early_spare : listed_page((uint32_t)i);
+    out_spare[i] = page;
+  }
   for (uint64_t unit = blockIdx.x; unit < (uint64_t)a.sequences * across; unit += gridDim.x) {
     const uint32_t s = (uint32_t)(unit / across), c = (uint32_t)(unit - (uint64_t)s * across) * kTableThreads + tid;
     if (c >= a.columns) continue;
     const uint32_t before = s > 0 ? wanted[s - 1] : 0, kept = need[s] - (wanted[s] - before);
     int page = -1;
     if (c < kept) {
-      page = old[(uint64_t)(uint32_t)a.source[s] * a.columns + c];
+      page = unit == blockIdx.x ? early_page : old[(uint64_t)(uint32_t)a.source[s] * a.columns + c];
     } else if (c < need[s]) {
       const uint32_t turn = before + (c - kept);
       if (turn < total) page = listed_page(total - 1 - turn);
@@ -272,12 +289,15 @@ __global__ __launch_bounds__(kKeepThreads) void keep_pages_kernel(KeepArgs a, ui
 int launch_page_tables(hipStream_t stream, const PageTableArgs& a) {
   if (((uintptr_t)a.out | (uintptr_t)a.previous | (uintptr_t)a.source | (uintptr_t)a.lengths) % 4 != 0)
     return IPUS_ERROR_INVALID_ARGUMENT;
-  // The previous state is read while the new one is written.
-  const uint64_t rows = 1 + (uint64_t)a.columns;
-  const uintptr_t out = (uintptr_t)a.out, before = (uintptr_t)a.previous;
-  const uint64_t out_bytes = 4 * (2 + a.pages + a.sequences * rows), bytes = 4 * (2 + a.pages + a.previous_sequences * rows);
-  if (out < before + bytes && before < out + out_bytes) return IPUS_ERROR_INVALID_ARGUMENT;
-  constexpr uint64_t kEach = 4 * kTableThreads, kMostGroups = 1024;
+  // The inputs are read while the new state is written.
+  const uint64_t rows = 1 + (uint64_t)a.columns, bytes = 4 * (2 + a.pages + a.sequences * rows);
+  if (overlaps(a.out, bytes, a.previous, 4 * (2 + a.pages + a.previous_sequences * rows)) ||
+      overlaps(a.out, bytes, a.source, 4ull * a.sequences) || overlaps(a.out, bytes, a.lengths, 4ull * a.sequences))
+    return IPUS_ERROR_INVALID_ARGUMENT;
+  // A word per thread, up to two workgroups per CU, whose own sums then take longer than the
+  // words of another (us, a word per thread / four: 64 sequences x 256 pages 4.2 / 5.0; 2000 x 500
+  // pages 12.0 of 512 workgroups, 12.2 of 1024, 14.5 of 256).
+  constexpr uint64_t kEach = kTableThreads, kMostGroups = 512;
   uint64_t groups = (a.pages + a.sequences * rows + kEach - 1) / kEach;
   groups = groups < 1 ? 1 : groups > kMostGroups ? kMostGroups : groups;
   const uint32_t lds = 8 * (a.sequences + a.previous_sequences);
@@ -287,6 +307,11 @@ int launch_page_tables(hipStream_t stream, const PageTableArgs& a) {
 
 int launch_slot_maps(hipStream_t stream, const SlotMapArgs& a) {
   if ((batch_addresses(a.batch) | (uintptr_t)a.counts | (uintptr_t)a.mask | (uintptr_t)a.out) % 4 != 0)
+    return IPUS_ERROR_INVALID_ARGUMENT;
+  const uint64_t sequences = a.batch.sequences, bytes = 4 * (sequences + 1 + 2ull * a.rows);
+  if (overlaps(a.out, bytes, a.counts, 4 * sequences) || overlaps(a.out, bytes, a.batch.lengths, 4 * sequences) ||
+      overlaps(a.out, bytes, a.batch.table, 4 * sequences * a.batch.table_columns) ||
+      overlaps(a.out, bytes, a.mask, 4ull * a.rows * a.mask_words))
     return IPUS_ERROR_INVALID_ARGUMENT;
   constexpr uint64_t kMostBlocks = 1u << 22;  // a grid dimension holds less than 2^32 threads
   const uint64_t blocks = a.rows == 0 ? 1 : ((uint64_t)a.rows + kSlotThreads - 1) / kSlotThreads;

@@ -124,6 +124,7 @@ def test_masks_hold_for_any_content(tmp_path):
 
 
 GRIDS = r"""
+#include <algorithm>
 #include "host_runtime.h"
 static char memory[1 << 16] __attribute__((aligned(256)));
 static ipus_context* ctx;
@@ -136,23 +137,37 @@ int main() {
   const char* m = memory;
   const uint64_t threads = 1ull << 32;
   // Page tables: the new state apart from the previous one.
-  CHECK(run("ipu_stack_page_tables", m, {m + 4 * 51, m, m}, {2, 2, 27, 16, 10}) == 0 && entries.size() == 1);
-  CHECK(run("ipu_stack_page_tables", m, {m + 4 * 50, m, m}, {2, 2, 27, 16, 10}) == IPUS_ERROR_INVALID_ARGUMENT);
-  CHECK(run("ipu_stack_page_tables", m + 4 * 50, {m, m, m}, {2, 2, 27, 16, 10}) == IPUS_ERROR_INVALID_ARGUMENT);
-  CHECK(run("ipu_stack_page_tables", m + 4 * 29, {m, m, m}, {2, 0, 27, 16, 10}) == 0);
-  CHECK(run("ipu_stack_page_tables", m, {m, m, m}, {2, 2, 27, 16, 10}) == IPUS_ERROR_INVALID_ARGUMENT);
-  CHECK(run("ipu_stack_page_tables", m + 2, {m + 1024, m, m}, {2, 2, 27, 16, 10}) == IPUS_ERROR_INVALID_ARGUMENT);
+  const char* n = m + 4096;
+  auto tables = [&](const char* out, const char* previous, uint32_t before, const char* source, const char* lengths) {
+    return run("ipu_stack_page_tables", out, {previous, source, lengths}, {2, before, 27, 16, 10});
+  };
+  CHECK(tables(m, m + 4 * 51, 2, n, n) == 0 && entries.size() == 1);
+  CHECK(tables(m + 4 * 29, m, 0, n, n) == 0 && tables(m, n, 2, m + 4 * 51, m + 4 * 51) == 0);
+  CHECK(tables(m, n, 2, m + 4 * 51, n + 2) == IPUS_ERROR_INVALID_ARGUMENT);
+  CHECK(tables(m, m + 4 * 50, 2, n, n) == IPUS_ERROR_INVALID_ARGUMENT && tables(m + 4 * 50, m, 2, n, n) == IPUS_ERROR_INVALID_ARGUMENT);
+  CHECK(tables(m, m, 2, n, n) == IPUS_ERROR_INVALID_ARGUMENT && tables(m + 2, n, 2, n, n) == IPUS_ERROR_INVALID_ARGUMENT);
+  CHECK(tables(m, n, 2, m + 4 * 50, n) == IPUS_ERROR_INVALID_ARGUMENT && tables(m, n, 2, n, m) == IPUS_ERROR_INVALID_ARGUMENT);
+  CHECK(tables(m + 4, n, 2, n, m) == IPUS_ERROR_INVALID_ARGUMENT && tables(m + 8, n, 2, n, m) == 0);
+  // Slot maps likewise: 3 + 1 + 2 x 5 words.
+  for (int input = 0; input < 4; ++input) {
+    std::vector<const void*> in = {n, n, n, n};
+    in[input] = m + 4 * 13;
+    CHECK(run("ipu_stack_slot_maps", m, in, {3, 5, 10, 16, 4, 1}) == IPUS_ERROR_INVALID_ARGUMENT);
+    in[input] = m + 4 * 14;
+    CHECK(run("ipu_stack_slot_maps", m, in, {3, 5, 10, 16, 4, 1}) == 0);
+  }
+  CHECK(run("ipu_stack_slot_maps", m, {n, n, n, m}, {3, 5, 10, 16, 4, 0}) == 0);  // a mask that is not read
   for (uint32_t sequences : {0u, 1u, 4096u})
     for (uint32_t columns : {0u, 1u, 2048u, 500000u})
       for (uint32_t pages : {0u, 3u, 0x7fffffffu}) {
-        CHECK(run("ipu_stack_page_tables", m, {(const void*)(1ull << 40), m, m}, {sequences, 4096, pages, 1, columns}) == 0);
+        CHECK(run("ipu_stack_page_tables", m, {(const void*)(1ull << 40), m - 65536, m - 65536}, {sequences, 4096, pages, 1, columns}) == 0);
         CHECK(entries.size() == 1 && entries[0].grid.x >= 1 && (uint64_t)entries[0].grid.x * entries[0].block.x < threads);
         CHECK(entries[0].shared == 8 * (sequences + 4096) && entries[0].shared <= 65536);
       }
   // Slot maps: a thread per row, one workgroup at least (for the offsets).
   first_words = 1;
   for (uint32_t rows : {0u, 1u, 512u, 513u, 1u << 30, 0x7fffffffu}) {
-    CHECK(run("ipu_stack_slot_maps", m, {m, m, m, m}, {3, rows, 10, 16, 4, 0}) == 0);
+    CHECK(run("ipu_stack_slot_maps", m, {m - 4096, m - 4096, m - 4096, m}, {3, rows, 10, 16, 4, 0}) == 0);
     uint64_t next = 0;
     for (const Entry& e : entries) {
       CHECK(e.words[0] == next && (uint64_t)e.grid.x * e.block.x < threads);
@@ -188,6 +203,21 @@ int main() {
   CHECK(run("ipu_stack_adjust_logits_f16", m + 2, in, {3, 70, 100, 100, 100, 0, 0, 0, 0}) == 0);
   CHECK(run("ipu_stack_adjust_logits_f16", m, in, {3, 0, 100, 100, 100, 0, 0, 0, 0}) == 0 && entries.empty());
   CHECK(run("ipu_stack_adjust_logits_f16", m, in, {0, 3, 100, 100, 100, 0, 0, 0, 0}) == 0 && entries.empty());
+  // Every chunk of every group of rows has a workgroup, whatever the sequences' rows: a group
+  // takes up to 8 fp16 rows of a sequence, each sequence a partial one more at most.
+  for (uint32_t sequences : {1u, 3u, 64u, 1000u, 70000u})
+    for (uint32_t rows : {1u, 5u, 700u, 4000u, 200000u, 1u << 28})
+      for (uint32_t columns : {1u, 4096u, 4097u, 131072u, 1000001u}) {
+        CHECK(run("ipu_stack_adjust_logits_f16", m, in, {sequences, rows, columns, columns, columns, 0, 0, 0, 0}) == 0);
+        const uint64_t chunks = (columns + 4095) / 4096, fill = rows * chunks / 2048;
+        const uint64_t group = rows <= sequences || fill < 1 ? 1 : fill > 8 ? 8 : fill;
+        uint64_t next = 0;
+        for (const Entry& e : entries) {
+          CHECK(e.words[0] == next && e.grid.x == chunks && e.grid.y <= 65535 && e.block.x == 512);
+          next += e.grid.y;
+        }
+        CHECK(next == std::min<uint64_t>(rows, group == 1 ? rows : rows / group + sequences));
+      }
   // A tree's mask has whole words.
   std::vector<const void*> tree = {m, m, m, m, m, m + 2};
   CHECK(run("ipu_stack_attention_tree_pages_f16", m, tree, {2, 8, 4, 8, 2, 64, 512, 10, 16, 4, 1, 0}) == IPUS_ERROR_INVALID_ARGUMENT);

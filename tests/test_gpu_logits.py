@@ -109,6 +109,40 @@ def test_logits(ctx, kind, rows, columns, history, biases, masks, allowed, pad):
     check(ctx, Step(rng, rows, columns, history, biases, masks, allowed, pad), kind)
 
 
+# Enough rows for several per workgroup: of few and of many sequences, some without rows, of one
+# of more rows than a workgroup has threads; with lists and without.
+@pytest.mark.parametrize("kind,rows,columns,history,biases,masks,allowed", [
+    ("f16", [64, 0, 70, 100, 3] * 3, 30000, 2000, 200, True, True), ("f32", [64, 70, 100, 3] * 3, 30001, 2000, 0, True, False),
+    ("f32", [9, 0, 11] * 33, 28673, 300, 40, True, True), ("f16", [9, 8, 1] * 40, 28680, 0, 0, False, False),
+    ("f32", [700, 3], 28700, 100, 20, False, True), ("f16", [650, 3], 28700, 5000, 100, True, True),
+    ("f16", [33] * 250, 4100, 20, 3, True, False), ("f32", [33] * 125, 4097, 0, 300, True, True),
+    ("f16", [40] * 52, 12288, 12000, 3000, True, False)])
+def test_several_rows_per_workgroup(ctx, kind, rows, columns, history, biases, masks, allowed):
+    rng = np.random.default_rng(columns)
+    step = Step(rng, rows, columns, history, biases, masks, allowed, 2)
+    for s in range(0, len(rows), 5):
+        step.penalties[s] = [1.0, 0.0, 0.0]  # none
+    check(ctx, step, kind)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_several_rows_in_place_of_any_content(ctx, kind):
+    """As below, in place, with strides, and logits that are not finite."""
+    rng = np.random.default_rng(27)
+    step = Step(rng, [90, 7, 60], 60001, 60, 50, True, True, twice=True)
+    step.history[:, ::7] = [[-1], [60001], [2 ** 31 - 1]]
+    step.tokens[::5] = -2 ** 31
+    step.bias_tokens[::4] = 60001
+    step.counts[:] = [[5, 90], [-1, 60], [2 ** 31 - 1, 30]]
+    step.words = 2
+    step.masks = [m & (1 << 64) - 1 for m in step.masks]
+    step.allowed[3] = False
+
+    def change(x):
+        x[:, 5], x[:, 6], x[:, 40], x[:, 41] = np.nan, np.inf, -np.inf, np.finfo(x.dtype).min
+    check(ctx, step, kind, strides=(60005, 60005), offset=1, in_place=True, change=change)
+
+
 @pytest.mark.parametrize("kind", sorted(TYPES))
 @pytest.mark.parametrize("strides,extra,offset,in_place", [
     ((1001, 1001), 0, 0, True), ((1008, 1001), 3, 0, False), ((1003, 1020), 0, 1, False), ((1024, 1024), 0, 3, True),

@@ -73,6 +73,13 @@ SHAPES = [
     ([10], [37], 2, 2, 520, 16, 0),
     ([3] * 220, [3 + i % 90 for i in range(220)], 16, 4, 128, 16, 1),
     ([2, 5, 1] * 90, [40 + i % 20 for i in range(270)], 8, 8, 64, 8, 0),
+    # Parts of the keys by all lengths: of up to 64 sequences and more, of more than those are
+    # planned for, beside short ones, and a second round of workgroups.
+    ([20, 33, 40, 9] * 5, [60, 1500, 3300, 9, 800] * 4, 4, 1, 64, 16, 1),
+    ([20, 33, 40] * 30, [60, 1500, 33, 2300, 800] * 18, 2, 1, 32, 16, 0),
+    ([40, 18] * 150, [300, 90, 1300] * 100, 1, 1, 32, 64, 0),
+    ([130, 40, 0, 300], [2500, 40, 0, 1400], 4, 4, 96, 32, 0),
+    ([40] * 9, [1100 + 300 * i for i in range(9)], 2, 2, 256, 16, 0),
 ]
 
 
