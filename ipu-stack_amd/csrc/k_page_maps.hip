@@ -42,6 +42,8 @@ __device__ __forceinline__ T scan_threads(T x, T* waves, T* all) {
 // state: one launch without a word between workgroups.  Entry i of the list of free pages is
 // the previous list's, behind it the pages given back in the order of the previous rows;
 // pages are taken from its end.
+// Entries and free pages are below 2^31 each (checked with the scalars), and a grid has at most
+// 2^18 threads: their numbers fit 32 bits.
 // The words that decide are loaded first, together, and so is what each thread will most
 // likely write; all else is LDS.
 constexpr uint32_t kTableThreads = 512, kTableWaves = kTableThreads / kWave;
@@ -59,13 +61,11 @@ __global__ __launch_bounds__(kTableThreads) void page_tables_kernel(PageTableArg
   auto within = [](int x, uint32_t most) __attribute__((always_inline)) {
     return x <= 0 ? 0u : (uint32_t)x < most ? (uint32_t)x : most;
   };
-  const uint32_t across = (a.columns + kTableThreads - 1) / kTableThreads;
-  const uint64_t spare0 = (uint64_t)blockIdx.x * kTableThreads + tid;
-  const uint32_t s0 = across > 0 && blockIdx.x / across < a.sequences ? blockIdx.x / across : 0;
-  const uint32_t c0 = (blockIdx.x - s0 * across) * kTableThreads + tid;
+  const uint32_t entries = a.sequences * a.columns, stride = gridDim.x * kTableThreads;
+  const uint32_t i0 = blockIdx.x * kTableThreads + tid;  // this thread's first entry and free page
 
   const uint32_t free = within(a.previous[0], a.pages);
-  const int early_spare = spare0 < a.pages ? spare[spare0] : -1;
+  const int early_spare = i0 < a.pages ? spare[i0] : -1;
   for (uint32_t p = tid; p < a.previous_sequences; p += kTableThreads) {
     owner[p] = a.sequences;
     back[p] = within(held[p], a.columns);
@@ -77,8 +77,11 @@ __global__ __launch_bounds__(kTableThreads) void page_tables_kernel(PageTableArg
     wanted[s] = (uint32_t)a.source[s];
   }
   __syncthreads();
-  const uint32_t from0 = a.sequences > 0 ? wanted[s0] : ~0u;
-  const int early_page = from0 < a.previous_sequences && c0 < a.columns ? old[(uint64_t)from0 * a.columns + c0] : -1;
+  int early_page = -1;
+  if (i0 < entries) {
+    const uint32_t s = i0 / a.columns, from = wanted[s];
+    if (from < a.previous_sequences) early_page = old[(uint64_t)from * a.columns + (i0 - s * a.columns)];
+  }
   for (uint32_t s = tid; s < a.sequences; s += kTableThreads) {
     const uint32_t from = wanted[s];
     if (from < a.previous_sequences) atomicMin(owner + from, s);
@@ -129,23 +132,22 @@ __global__ __launch_bounds__(kTableThreads) void page_tables_kernel(PageTableArg
   int* const out_spare = a.out + 2;
   int* const out_held = out_spare + a.pages;
   int* const out_table = out_held + a.sequences;
-  for (uint64_t i = spare0; i < a.pages; i += (uint64_t)gridDim.x * kTableThreads) {
+  for (uint32_t i = i0; i < a.pages; i += stride) {
     int page = -1;
-    if (i < left) page = i == spare0 && i < free ? early_spare : listed_page((uint32_t)i);
+    if (i < left) page = i == i0 && i < free ? early_spare : listed_page(i);
     out_spare[i] = page;
   }
-  for (uint64_t unit = blockIdx.x; unit < (uint64_t)a.sequences * across; unit += gridDim.x) {
-    const uint32_t s = (uint32_t)(unit / across), c = (uint32_t)(unit - (uint64_t)s * across) * kTableThreads + tid;
-    if (c >= a.columns) continue;
+  for (uint32_t i = i0; i < entries; i += stride) {
+    const uint32_t s = i / a.columns, c = i - s * a.columns;
     const uint32_t before = s > 0 ? wanted[s - 1] : 0, kept = need[s] - (wanted[s] - before);
     int page = -1;
     if (c < kept) {
-      page = unit == blockIdx.x ? early_page : old[(uint64_t)(uint32_t)a.source[s] * a.columns + c];
+      page = i == i0 ? early_page : old[(uint64_t)(uint32_t)a.source[s] * a.columns + c];
     } else if (c < need[s]) {
       const uint32_t turn = before + (c - kept);
       if (turn < total) page = listed_page(total - 1 - turn);
     }
-    out_table[(uint64_t)s * a.columns + c] = page;
+    out_table[i] = page;
   }
   if (blockIdx.x > 0) return;
   for (uint32_t s = tid; s < a.sequences; s += kTableThreads) {
