@@ -51,6 +51,22 @@ def test_tables_over_many_steps(ctx, sequences, columns, page_rows, pages):
         assert np.array_equal(got, state), step
 
 
+def test_tables_of_the_most_sequences(ctx):
+    """4096 rows before and after, in another order."""
+    rng = np.random.default_rng(10)
+    pages, columns, page_rows, count = 20000, 6, 8, 4096
+    free, rows = [int(p) for p in rng.permutation(pages)], []
+    state = table_state(free, rows, pages, columns)
+    for step in range(3):
+        previous = len(rows)
+        source = [int(p) for p in rng.permutation(count)] if step else [-1] * count
+        lengths = [int(x) for x in rng.integers(0, 45, count)]
+        got = launch_tables(ctx, state, source, lengths, previous, pages, page_rows, columns)
+        free, rows, missing = fit_tables(free, rows, source, lengths, page_rows, columns)
+        state = table_state(free, rows, pages, columns, missing)
+        assert np.array_equal(got, state)
+
+
 def test_tables_of_any_content(ctx):
     """A state that the operator did not write: what comes out is bounded, and what lies
     behind it untouched (no values are promised)."""
