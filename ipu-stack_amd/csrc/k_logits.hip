@@ -3,7 +3,9 @@
 //        the row's path, then x' - (f g + p [g > 0]) with g its uses behind the prompt,
 //   then x' + its bias, and -inf for a token that the row's mask does not allow.
 // The path of a row is the rows of its sequence that its mask names, or those up to itself.
-// Bound by HBM: the logits once in, once out.
+// Bound by HBM, the logits once in, once out, where there are rows enough: 64 trees of 8 to 16 rows
+// x 131072 fp32 behind 8192 tokens with 300 biases and masks 145 us, 5.7 TB/s, fp16 81 us, 5.0;
+// by latency where there are few (64 single rows x 50001 fp16 7.1 us, 13 MB).
 #include "attention_pages.h"
 
 namespace ipus {
@@ -340,7 +342,9 @@ __global__ __launch_bounds__(kLogitThreads, 8) void adjust_rows_kernel(LogitArgs
 }
 
 // Several rows per workgroup where sequences have them and there are enough for two rounds of the
-// workgroups that the chip holds (four per CU), but not so many that the last round is long.
+// workgroups that the chip holds (four per CU), but not so many that the last round is long (us,
+// 64 trees of 8 to 16 rows x 131072: fp32 3 / 4 / 6 / 8 rows 145 / 146 / 151 / 155, fp16 8 / 12 / 16
+// rows 81 / 83 / 83).
 template <typename T>
 int launch_as(hipStream_t stream, const LogitArgs& a) {
   constexpr uint64_t kWant = 2 * 4 * 256, kMostUnits = 65535;  // the grid's second dimension

@@ -42,6 +42,8 @@ __device__ __forceinline__ T scan_threads(T x, T* waves, T* all) {
 // state: one launch without a word between workgroups.  Entry i of the list of free pages is
 // the previous list's, behind it the pages given back in the order of the previous rows;
 // pages are taken from its end.
+// Bound by the launch and the loads that wait for each other: 64 sequences x 256 pages 3.6 us on
+// the GPU, 512 x 2048 with 624,000 pages in the pool 7.5 us (7.7 MB), in two rounds of workgroups.
 // Entries and free pages are below 2^31 each (checked with the scalars), and a grid has at most
 // 2^18 threads: their numbers fit 32 bits.
 // The words that decide are loaded first, together, and so is what each thread will most
@@ -165,7 +167,8 @@ __global__ __launch_bounds__(kTableThreads) void page_tables_kernel(PageTableArg
 // Slot maps
 // ---------------------------------------------------------------------------
 // A thread per row; every workgroup adds the counts up for itself, a thread per sequence at
-// a time, and looks its rows up among the sums.  The first one writes the offsets too.
+// a time, and looks its rows up among the sums.  The first one writes the offsets too.  Bound
+// by latency (count, sum, length, table entry): 64 rows 2.7 us on the GPU, 1000 trees of 64 rows 4.6.
 constexpr uint32_t kSlotThreads = 512, kSlotWaves = kSlotThreads / kWave;
 __global__ __launch_bounds__(kSlotThreads) void slot_maps_kernel(SlotMapArgs a, uint32_t first_block) {
   __shared__ uint32_t ends[kSlotThreads];  // of the sequences' rows, within a.rows
@@ -234,7 +237,9 @@ __global__ __launch_bounds__(kSlotThreads) void slot_maps_kernel(SlotMapArgs a, 
 // Row path[i] of a sequence's new rows moves to row i, in the caches of all layers.  The path
 // increases, so that a row is read before, or by the same entry as, it is written when entries
 // go in order: a thread takes the same columns of all of them, in groups whose loads are in
-// flight together.
+// flight together.  Bound by HBM behind three loads that wait for each other (path, page, row):
+// 64 sequences x up to 12 rows x 16 layers x 8 heads x 128, 52 MB, 11.3 us (4.6 TB/s; sixteen rows
+// in flight 11.2, but 7.0 against 6.3 for paths of up to 4 in 32 layers).
 constexpr uint32_t kKeepThreads = 256, kKeepEntries = 64, kKeepAtOnce = 8;
 template <int V>
 __global__ __launch_bounds__(kKeepThreads) void keep_pages_kernel(KeepArgs a, uint32_t first_sequence) {
