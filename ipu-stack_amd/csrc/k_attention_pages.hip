@@ -182,7 +182,7 @@ constexpr uint32_t kMostResident = 512;  // workgroups on the chip at most (Deco
 //    shared keys, 256 x 16 x 52 of 64 columns 54 / 93, 256 x 8 x 52 of 128 55 / 71, but 113 x 12 x
 //    30 of 256 columns 151 / 92);
 //  - no segment of more than 16 tiles: all whole;
-//  - at least 40 tiles per resident workgroup: the tiles of all segments are one line, cut
+//  - at least 40 tiles per resident workgroup (of trees 200): the tiles of all segments are one line, cut
 //    into an equal chunk for each, wherever the cuts fall (128 segments of 125 tiles, 31 per
 //    workgroup, 61.6 us so, in parts 54.6);
 //  - in between: every segment in parts of its own, of at least 8 tiles, one per
@@ -191,7 +191,12 @@ constexpr uint32_t kMostResident = 512;  // workgroups on the chip at most (Deco
 //    about one per CU (two make twice the parts to join: 8 segments of 500 tiles 24.5 us
 //    against 21.6, 32 of 66 18.2 against 16.1).
 // The line's units are tiles (part_tiles = 0) or parts of at most part_tiles tiles.
-constexpr uint32_t kAloneTiles = 32, kAloneShared = 8;
+// Trees: hundreds of segments of very different lengths are whole, or in few parts, up to 200
+// tiles per workgroup, which begins the next one as it ends (us, so / in equal chunks from 40 on,
+// 8 key heads x 128: 128 trees against 125 to 2000 keys 95 / 125, 64 against 250 to 4000 84 / 91, 128
+// against 250 to 4000 164 / 177; 64 against 500 to 8000 148 / 144, of equal lengths the same).  Single
+// rows and causal ones keep the 40, and with it the order in which their parts are added.
+constexpr uint32_t kAloneTiles = 32, kAloneShared = 8, kChunkTiles = 40, kTreeChunkTiles = 200;
 struct Shares {
   uint32_t part_tiles;
   uint64_t chunk;  // units per workgroup, or per wave
@@ -205,9 +210,9 @@ struct Shares {
   }
 };
 __device__ __forceinline__ Shares share_out(uint64_t tiles, uint64_t segments, uint32_t longest, uint32_t groups,
-                                            uint32_t resident, bool may_split, uint32_t alone_tiles) {
+                                            uint32_t resident, bool may_split, uint32_t alone_tiles, uint32_t chunk_tiles) {
   constexpr uint32_t kAloneSegments = 600;
-  constexpr uint32_t kWholeTiles = 16, kLeastTiles = 8, kChunkTiles = 40, kCus = 256;
+  constexpr uint32_t kWholeTiles = 16, kLeastTiles = 8, kCus = 256;
   if (longest <= alone_tiles && (uint64_t)longest * kAloneSegments <= tiles) {
     const uint32_t waves = groups * kWaves;
     return {0xffffffffu, quotient(segments + waves - 1, waves), segments, true};
@@ -216,7 +221,7 @@ __device__ __forceinline__ Shares share_out(uint64_t tiles, uint64_t segments, u
     return {0xffffffffu, quotient(segments + groups - 1, groups), segments, false};
   if (resident > groups) resident = groups;
   const uint64_t each = quotient(tiles + resident - 1, resident);
-  if (each < kChunkTiles) {
+  if (each < chunk_tiles) {
     uint32_t part = (uint32_t)((tiles + kCus - 1) / kCus);
     if (part < kLeastTiles) part = kLeastTiles;
     const uint32_t least = (longest + kMaxParts - 1) / kMaxParts;
@@ -322,7 +327,8 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
   longest = largest(longest);
   if (segments == 0) return;
   const Shares shares = share_out(tiles, segments, longest, gridDim.x, C::kResident, split.rows != nullptr,
-                                  !Shared ? kAloneTiles : D <= 128 ? kAloneShared : 0);
+                                  !Shared ? kAloneTiles : D <= 128 ? kAloneShared : 0,
+                                  Tree ? kTreeChunkTiles : kChunkTiles);
   auto line_units = [&](const Units& u) __attribute__((always_inline)) { return u.segments * shares.units(u.tiles); };
   auto units_in = [&](uint32_t s) __attribute__((always_inline)) { return line_units(units_at(s)); };
   UnitLine line{scan(line_units(held)), 0};
