@@ -9,9 +9,11 @@
 namespace ipus {
 namespace {
 
-// Whether `bytes` from a on share memory with `others` from b on.
+// Whether `bytes` from a on share memory with `others` from b on: none of an empty list,
+// whose address may be any.
 inline bool overlaps(const void* a, uint64_t bytes, const void* b, uint64_t others) {
-  return (uintptr_t)a < (uintptr_t)b + others && (uintptr_t)b < (uintptr_t)a + bytes;
+  if (bytes == 0 || others == 0) return false;
+  return (uintptr_t)a < (uintptr_t)b ? (uintptr_t)b - (uintptr_t)a < bytes : (uintptr_t)a - (uintptr_t)b < others;
 }
 inline int hip_status(hipError_t e) { return e == hipSuccess ? 0 : IPUS_ERROR_HIP_BASE - (int)e; }
 
