@@ -298,8 +298,9 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        not allowed gets -inf, whatever it was.  fp32 arithmetic, one rounding.
  *        Tokens outside [0, columns) count for nothing (-1: a prompt's rows, whose
  *        tokens stand in the history).  Rows outside every sequence are left as
- *        they were.  The output is the input (with its stride) or does not overlap
- *        it.
+ *        they were.  The output is the input (with its stride), or its rows share
+ *        no memory with the input's; nor do they with a list that is read.  Other
+ *        addresses are refused.
  *   ipu_stack_keep_pages_f16   out the caches of all layers, fp16 [layers][pages][2]
  *        [key_heads][page_rows][width]; page_table, row_offsets, lengths, path
  *        [sequences][path_columns], path_counts [sequences]; sequences, rows, layers

@@ -224,8 +224,9 @@ __global__ __launch_bounds__(kLogitThreads, 8) void adjust_rows_kernel(LogitArgs
   const uint32_t s = uniform(found.sequence);
   if (s >= a.sequences) return;
   const LogitRows all = logit_rows(a, s);
-  const uint32_t row0 = all.first + (unit - (uint32_t)found.first) * group, left = all.first + all.rows - row0;
-  const uint32_t rows = left < group ? left : group;
+  const uint32_t ahead = (unit - (uint32_t)found.first) * group;
+  if (ahead >= all.rows) return;  // offsets that change meanwhile
+  const uint32_t row0 = all.first + ahead, left = all.rows - ahead, rows = left < group ? left : group;
 
   P next;
   uint32_t next_path = 0;
@@ -373,6 +374,45 @@ int launch_as(hipStream_t stream, const LogitArgs& a) {
   return 0;
 }
 
+// Rows of `bytes` each, `stride` apart (at least their bytes).
+struct RowSpan {
+  uint64_t at, stride, rows, bytes;
+  uint64_t end() const { return at + (rows - 1) * stride + bytes; }
+  // Whether one of them shares memory with `count` bytes from `from` on.
+  bool meets(uint64_t from, uint64_t count) const {
+    if (count == 0 || from + count <= at || from >= end()) return false;
+    uint64_t row = (from + count - 1 - at) / stride;  // the last that begins before their end
+    if (row >= rows) row = rows - 1;
+    return at + row * stride + bytes > from;
+  }
+  bool meets(const RowSpan& other) const {
+    if (other.end() <= at || other.at >= end()) return false;
+    // With one stride a pair's distance goes by its rows' difference alone: pairs with the first or the
+    // last row are all that there are.
+    const uint64_t step = stride == other.stride && other.rows > 1 ? other.rows - 1 : 1;
+    for (uint64_t r = 0; r < other.rows; r += step)
+      if (meets(other.at + r * other.stride, other.bytes)) return true;
+    return false;
+  }
+};
+// Whether the output shares memory with an input other than row by row, in place: workgroups
+// read the lists, and rows ahead of the one that they write, while others write.  Where the tokens'
+// list begins at the logits' own address, all are taken for placeholders, of a launch that is
+// only looked at.
+bool races(const LogitArgs& a) {
+  if ((const void*)a.tokens == a.logits) return a.out == a.logits && a.input_row_stride != a.output_row_stride;
+  const uint64_t element = a.f32 ? 4 : 2, sequences = a.sequences, rows = a.rows;
+  const RowSpan out{(uintptr_t)a.out, a.output_row_stride * element, rows, a.columns * element};
+  const RowSpan in{(uintptr_t)a.logits, a.input_row_stride * element, rows, a.columns * element};
+  if (!(out.at == in.at && out.stride == in.stride) && out.meets(in)) return true;
+  auto over = [&](const void* list, uint64_t bytes) { return out.meets((uintptr_t)list, bytes); };
+  return over(a.row_offsets, 4 * (sequences + 1)) || over(a.tokens, 4 * rows) || over(a.penalties, 12 * sequences) ||
+         over(a.mask, 4 * rows * a.mask_words) || over(a.history, 4 * sequences * a.history_columns) ||
+         (a.history_columns && over(a.history_counts, 8 * sequences)) ||
+         (a.bias_entries && over(a.bias_offsets, 4 * (sequences + 1))) || over(a.biases, 8ull * a.bias_entries) ||
+         over(a.allowed, 4 * rows * a.allowed_words);
+}
+
 }  // namespace
 
 int launch_adjust_logits(hipStream_t stream, const LogitArgs& a) {
@@ -382,8 +422,8 @@ int launch_adjust_logits(hipStream_t stream, const LogitArgs& a) {
                           (uintptr_t)a.biases | (uintptr_t)a.allowed;
   if (words % 4 != 0 || ((uintptr_t)a.out | (uintptr_t)a.logits) % (a.f32 ? 4 : 2) != 0)
     return IPUS_ERROR_INVALID_ARGUMENT;
-  // In place only where every element is read and written by the same thread.
-  if (a.out == a.logits && a.input_row_stride != a.output_row_stride) return IPUS_ERROR_INVALID_ARGUMENT;
+  // In place every element is read and written by the same thread.
+  if (races(a)) return IPUS_ERROR_INVALID_ARGUMENT;
   return a.f32 ? launch_as<float>(stream, a) : launch_as<half_t>(stream, a);
 }
 
