@@ -267,12 +267,16 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        as 0), lengths [sequences] (with them), page_table, the tree's mask;
  *        sequences, rows, pages, page_rows, table_columns, mask_words (0: none,
  *        and not read).  Offsets are cut off at `rows`.  Row i of the n of
- *        sequence s is stored at place lengths[s] - n + i: its slot is page *
- *        page_rows + row in the page, -1 where the place has no page.  Its
- *        position is the place, in a tree lengths[s] - n + how many other rows it
- *        reads (its depth), -1 below 0.  Rows behind the last sequence: position
- *        0, slot -1.  pages x page_rows <= 2^31; the output lies apart from the
- *        inputs.
+ *        sequence s, as the offsets say, is stored at place lengths[s] - n + i: its
+ *        slot is page * page_rows + row in the page, -1 where the place has no
+ *        page.  Its position is the place, in a tree lengths[s] - n + how many
+ *        other rows it reads (its depth), -1 below 0.  Rows behind the last
+ *        sequence: position 0, slot -1.  n is what the append and the attention
+ *        take from the offsets, so where the counts pass `rows`, lengths are to be
+ *        those with the rows that are left (lengths[s] less the rows cut off, as
+ *        many of the last ones): else the rows left stand at the last ones' places,
+ *        behind keys that nobody has written.  pages x page_rows <= 2^31; the
+ *        output lies apart from the inputs.
  *   ipu_stack_attention_tree_pages_f16   as ipu_stack_attention_pages_f16 with the
  *        tree's mask behind the inputs and mask_words (at least 1) in the place of
  *        causal: row i of sequence s reads the keys before its sequence's rows,

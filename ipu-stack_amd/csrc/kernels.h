@@ -166,7 +166,8 @@ struct PageTableArgs {
 int launch_page_tables(hipStream_t stream, const PageTableArgs& a);
 
 // Row offsets, positions and cache slots of a step's rows: int32 [sequences + 1],
-// [rows], [rows].  batch.row_offsets is not read.
+// [rows], [rows].  batch.row_offsets is not read.  A sequence that the last row cuts off
+// has the rows that are left, as for the kernels that take the offsets.
 struct SlotMapArgs {
   int* out;
   const int* counts;     // [sequences] new rows

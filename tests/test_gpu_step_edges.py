@@ -5,8 +5,10 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from step_forms import within
+from decoder_forms import Batch
+from step_forms import slot_maps, tree, within, words
 from test_gpu_logits import TYPES, Step
+from test_gpu_page_maps import launch_slots
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +30,24 @@ def test_logits_between_the_rows_of_their_input(ctx, kind, rows):
     assert np.all(inside) and np.array_equal(got[:, 0], x[:, 0]) and np.all(within(got[:, 1], want, bound, dtype))
     for b in bufs + [buffer]:
         b.free()
+
+
+@pytest.mark.parametrize("trees", [False, True])
+def test_slots_of_a_step_that_is_cut_off(ctx, trees):
+    """Fewer rows than the counts' sum: with lengths less the rows cut off, the rows that are
+    left stand where they stand in the whole step."""
+    rng = np.random.default_rng(3)
+    counts, lengths = [40, 3, 0, 70, 5], [90, 60, 7, 70, 200]
+    b = Batch(rng, counts, lengths, 16)
+    masks = [m for n in counts for m in tree(rng, n, 0.1)]
+    count, sequences = 3 if trees else 0, len(counts)
+    whole = launch_slots(ctx, counts, lengths, b.table, b.rows, 16, b.pages, words(masks, count))
+    for rows in (0, 1, 39, 40, 42, 43, 44, 112, 113, 117):
+        left = [int(min(rows, end) - min(rows, end - n)) for n, end in zip(counts, np.cumsum(counts))]
+        shorter = [length - n + m for length, n, m in zip(lengths, counts, left)]
+        got = launch_slots(ctx, counts, shorter, b.table, rows, 16, b.pages, words(masks[:rows], count))
+        assert list(got[:sequences + 1]) == [0] + list(np.cumsum(left))
+        for part in (0, 1):  # positions, slots
+            here, there = sequences + 1 + part * rows, sequences + 1 + part * b.rows
+            assert np.array_equal(got[here:here + rows], whole[there:there + rows])
+        assert np.array_equal(got, slot_maps(counts, shorter, b.table, rows, 16, b.pages, masks if trees else None))
