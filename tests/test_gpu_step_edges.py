@@ -6,9 +6,9 @@ import numpy as np
 import pytest
 
 from decoder_forms import Batch
-from step_forms import slot_maps, tree, within, words
+from step_forms import fit_tables, slot_maps, table_state, tree, within, words
 from test_gpu_logits import TYPES, Step
-from test_gpu_page_maps import launch_slots
+from test_gpu_page_maps import launch_slots, launch_tables
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,26 @@ def test_slots_of_a_step_that_is_cut_off(ctx, trees):
             here, there = sequences + 1 + part * rows, sequences + 1 + part * b.rows
             assert np.array_equal(got[here:here + rows], whole[there:there + rows])
         assert np.array_equal(got, slot_maps(counts, shorter, b.table, rows, 16, b.pages, masks if trees else None))
+
+
+@pytest.mark.parametrize("sequences,columns,page_rows,pages", [(300, 1200, 4, 400000), (4096, 70, 16, 290000), (2, 200000, 1, 270000)])
+def test_tables_of_more_words_than_threads(ctx, sequences, columns, page_rows, pages):
+    """More entries and more free pages than the largest grid has threads (2^18): requests
+    begin, grow, shrink, end and change places."""
+    assert sequences * columns > 1 << 18 and pages > 1 << 18
+    rng = np.random.default_rng(columns)
+    free, rows = [int(p) for p in rng.permutation(pages)], []
+    state = table_state(free, rows, pages, columns)
+    most = columns * page_rows
+    for step in range(6):
+        previous = len(rows)
+        count = sequences if step < 2 else int(rng.integers(max(1, sequences // 2), sequences + 1))
+        source = [int(p) for p in rng.permutation(max(previous, count))[:count]]
+        # Some begin, and one names a row that another goes on with.
+        source = [p if p < previous and rng.random() < 0.8 else int(rng.integers(-2, previous + 2)) for p in source]
+        # Few pages at first, so that most stay free, then as many as there are.
+        lengths = [int(rng.integers(0, most // (8 if step % 3 == 0 else 1) + 1)) for _ in range(count)]
+        got = launch_tables(ctx, state, source, lengths, previous, pages, page_rows, columns)
+        free, rows, missing = fit_tables(free, rows, source, lengths, page_rows, columns)
+        state = table_state(free, rows, pages, columns, missing)
+        assert np.array_equal(got, state), step
