@@ -9,6 +9,7 @@ from decoder_forms import Batch
 from step_forms import fit_tables, slot_maps, table_state, tree, within, words
 from test_gpu_logits import TYPES, Step
 from test_gpu_page_maps import launch_slots, launch_tables
+from test_gpu_tree_attention import check as check_trees, masks_of
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +75,30 @@ def test_tables_of_more_words_than_threads(ctx, sequences, columns, page_rows, p
         free, rows, missing = fit_tables(free, rows, source, lengths, page_rows, columns)
         state = table_state(free, rows, pages, columns, missing)
         assert np.array_equal(got, state), step
+
+
+@pytest.mark.parametrize("rows,lengths,heads,width", [
+    ([2] * 130, [40 + 9 * (37 * i % 130) for i in range(130)], 16, 128),      # one tile of 16 queries
+    ([20, 3] * 65, [100 + 18 * (37 * i % 130) for i in range(130)], 16, 64),  # two, tiles of 64 keys
+    ([3] * 150, [20 + 7 * (41 * i % 150) for i in range(150)], 14, 192)])
+def test_trees_cut_anywhere(ipus, ctx, rows, lengths, heads, width):
+    """More segments (sequence and key head) than workgroups, the longest of more than 32 tiles of
+    keys: all of their tiles are one line, cut into equal chunks wherever the cuts fall, through
+    the tiles that hold a tree's own keys too."""
+    rng = np.random.default_rng(width)
+    b = Batch(rng, rows, lengths, 16, 1)
+    check_trees(ipus, ctx, b, masks_of(rng, b, 0.3), heads, heads, width)
+
+
+def test_long_trees_cut_anywhere(ipus, ctx):
+    """Chunks shorter than a segment, so that its parts are those of three and more workgroups: 200
+    tiles of keys and more for each.  The sequences read the same pages, in other orders."""
+    rng = np.random.default_rng(4)
+    lengths = [34000 + 2001 * (7 * i % 10) for i in range(10)]
+    b = Batch(rng, [3] * 10, [max(lengths)] + [3] * 9, 64)
+    pages = b.table[0, :-(-max(lengths) // 64)].copy()
+    for s, length in enumerate(lengths):
+        b.table[s, :len(pages)] = rng.permutation(pages)
+    b.k, b.lengths = lengths, np.array(lengths, np.int32)
+    assert sum(-(-x // 64) for x in lengths) * 16 >= 200 * 512
+    check_trees(ipus, ctx, b, masks_of(rng, b, 0.3), 16, 16, 32)
