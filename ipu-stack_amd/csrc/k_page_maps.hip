@@ -45,7 +45,10 @@ __device__ __forceinline__ T scan_threads(T x, T* waves, T* all) {
 // the previous list's, behind it the pages given back in the order of the previous rows;
 // pages are taken from its end.
 // Bound by the launch and the loads that wait for each other: 64 sequences x 256 pages 3.6 us on
-// the GPU, 512 x 2048 with 624,000 pages in the pool 7.5 us (7.7 MB), in two rounds of workgroups.
+// the GPU; of 512 sequences the sums alone 4.3 us (2 columns, 2000 pages), 5.7 with a word of the
+// state for every thread (256 columns, 80,000 pages), 7.5 with seven (2048 columns, 624,000 pages,
+// 7.7 MB): all workgroups are on the chip at once, and a thread's words behind its first take turns,
+// an entry's with a division and two loads that wait for each other (its source, then the page).
 // Entries and free pages are below 2^31 each (checked with the scalars), and a grid has at most
 // 2^18 threads: their numbers fit 32 bits.
 // The words that decide are loaded first, together, and so is what each thread will most
@@ -240,8 +243,8 @@ __global__ __launch_bounds__(kSlotThreads) void slot_maps_kernel(SlotMapArgs a, 
 // increases, so that a row is read before, or by the same entry as, it is written when entries
 // go in order: a thread takes the same columns of all of them, in groups whose loads are in
 // flight together.  Bound by HBM behind three loads that wait for each other (path, page, row):
-// 64 sequences x up to 12 rows x 16 layers x 8 heads x 128, 52 MB, 11.3 us (4.6 TB/s; sixteen rows
-// in flight 11.2, but 7.0 against 6.3 for paths of up to 4 in 32 layers).
+// 64 sequences x up to 12 rows x 16 layers x 8 heads x 128, 52 MB, 11.3 us (4.6 TB/s; 12.4 on another
+// card; sixteen rows in flight 11.2, but 7.0 against 6.3 for paths of up to 4 in 32 layers).
 constexpr uint32_t kKeepThreads = 256, kKeepEntries = 64, kKeepAtOnce = 8;
 template <int V>
 __global__ __launch_bounds__(kKeepThreads) void keep_pages_kernel(KeepArgs a, uint32_t first_sequence) {
