@@ -142,10 +142,13 @@ __device__ __forceinline__ void clear_non_finite(uint8_t* tile, uint32_t thread,
 // Adds the products of a tile's non-finite values, in the layout of the kernels' MFMAs: o[dt][qt][c]
 // is column 16 dt + 4 (l / 16) + c of query 16 qt + l % 16, and p(kk, qt, e) the probability of
 // key 32 kk + 4 (l / 16) + e % 4 + 16 (e / 4).  chunk(row, column): where 4 columns lie in the tile;
-// reads(qt, row): whether this lane's query reads the tile's key `row`.
-template <uint32_t Halves, uint32_t DT, uint32_t QT, typename P, typename Chunk, typename Reads>
+// this lane's query reads the keys below limit of which named(qt, row) says so by the tile's row.
+struct AllNamed {
+  __device__ __forceinline__ bool operator()(uint32_t, uint32_t) const { return true; }
+};
+template <uint32_t Halves, uint32_t DT, uint32_t QT, typename P, typename Chunk, typename Named = AllNamed>
 __device__ __forceinline__ void add_non_finite(float4_t (&o)[DT][QT], P p, const uint8_t* tile, Chunk chunk,
-                                               Reads reads) {
+                                               const uint32_t (&limit)[QT], uint32_t key0, Named named = {}) {
 #pragma unroll
   for (uint32_t kk = 0; kk < Halves; ++kk)
 #pragma unroll
@@ -168,7 +171,7 @@ __device__ __forceinline__ void add_non_finite(float4_t (&o)[DT][QT], P p, const
             const float v = (float)x[c];
             const bool bad = !(fabsf(v) <= 65504.0f);
 #pragma unroll
-            for (uint32_t qt = 0; qt < QT; ++qt) o[dt][qt][c] += bad && reads(qt, row) ? w[qt] * v : 0.0f;
+            for (uint32_t qt = 0; qt < QT; ++qt) o[dt][qt][c] += bad && key0 + row < limit[qt] && named(qt, row) ? w[qt] * v : 0.0f;
           }
         }
       }

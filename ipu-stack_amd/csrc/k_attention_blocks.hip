@@ -536,17 +536,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(PagedAtte
     if (lane == 0) wave_word[wave] = mine;
     __syncthreads();
     if (wave_word[0] | wave_word[1] | wave_word[2] | wave_word[3]) {
-      uint64_t bits[QT];
+      auto weight = [&](uint32_t kk, uint32_t qt, uint32_t e) __attribute__((always_inline)) { return (float)pp[kk][qt][e]; };
+      auto chunk = [&](uint32_t row, uint32_t column) __attribute__((always_inline)) {
+        return row * kRowBytes + (((column / 8) ^ value_swizzle<D>(row)) << 4) + column % 8 * 2;
+      };
+      if constexpr (Tree) {
+        uint64_t bits[QT];
 #pragma unroll
-      for (uint32_t qt = 0; qt < QT; ++qt) bits[qt] = Tree ? seen(qt, j * kKeys) : ~0ull;
-      add_non_finite<kHalves, kDT, QT>(
-          o, [&](uint32_t kk, uint32_t qt, uint32_t e) __attribute__((always_inline)) { return (float)pp[kk][qt][e]; }, lv,
-          [&](uint32_t row, uint32_t column) __attribute__((always_inline)) {
-            return row * kRowBytes + (((column / 8) ^ value_swizzle<D>(row)) << 4) + column % 8 * 2;
-          },
-          [&](uint32_t qt, uint32_t row) __attribute__((always_inline)) {
-            return j * kKeys + row < limit[qt] && (!Tree || (bits[qt] >> row & 1));
-          });
+        for (uint32_t qt = 0; qt < QT; ++qt) bits[qt] = seen(qt, j * kKeys);
+        add_non_finite<kHalves, kDT, QT>(o, weight, lv, chunk, limit, j * kKeys,
+                                         [&](uint32_t qt, uint32_t row) __attribute__((always_inline)) { return bits[qt] >> row & 1; });
+      } else {
+        add_non_finite<kHalves, kDT, QT>(o, weight, lv, chunk, limit, j * kKeys);
+      }
       __syncthreads();
       clear_non_finite<kTile>(lv, threadIdx.x, kThreads);
       __syncthreads();

@@ -540,19 +540,21 @@ __global__ __launch_bounds__(kThreads, (Decode<D, MT>::kPerCu)) void attention_p
       }
       __builtin_amdgcn_sched_barrier(0);
       if (upto > least && has_non_finite<kTile>(lv)) {
-        std::conditional_t<kKeys == 64, uint64_t, uint32_t> bits[MT];
+        auto weight = [&](uint32_t kk, uint32_t mt, uint32_t e) __attribute__((always_inline)) {
+          return (float)high[kk][mt][e] + (float)low[kk][mt][e];
+        };
+        auto chunk = [&](uint32_t row, uint32_t column) __attribute__((always_inline)) {
+          return row * kRowBytes + (((column / 8) ^ tile_swizzle<D>(row)) << 4) + column % 8 * 2;
+        };
+        if constexpr (Tree) {
+          std::conditional_t<kKeys == 64, uint64_t, uint32_t> bits[MT];
 #pragma unroll
-        for (uint32_t mt = 0; mt < MT; ++mt) if (Tree) bits[mt] = seen(mt);
-        add_non_finite<kHalves, kDT, MT>(
-            o, [&](uint32_t kk, uint32_t mt, uint32_t e) __attribute__((always_inline)) {
-              return (float)high[kk][mt][e] + (float)low[kk][mt][e];
-            }, lv,
-            [&](uint32_t row, uint32_t column) __attribute__((always_inline)) {
-              return row * kRowBytes + (((column / 8) ^ tile_swizzle<D>(row)) << 4) + column % 8 * 2;
-            },
-            [&](uint32_t mt, uint32_t row) __attribute__((always_inline)) {
-              return key0 + row < limit[mt] && (!Tree || (bits[mt] >> row & 1));
-            });
+          for (uint32_t mt = 0; mt < MT; ++mt) bits[mt] = seen(mt);
+          add_non_finite<kHalves, kDT, MT>(o, weight, lv, chunk, limit, key0,
+                                           [&](uint32_t mt, uint32_t row) __attribute__((always_inline)) { return bits[mt] >> row & 1; });
+        } else {
+          add_non_finite<kHalves, kDT, MT>(o, weight, lv, chunk, limit, key0);
+        }
         clear_non_finite<kTile>(lv, lane, kWave);
       }
       uint32_t vbase_v = vbase;
