@@ -298,8 +298,10 @@ int ipus_event_elapsed_ms(ipus_event *start, ipus_event *end, float *millisecond
  *        mask names.  With g how often a token stands in the path and the history
  *        behind the prompt: a token of prompt, history or path has its logit x
  *        divided by r (x > 0) or multiplied by it, and if g > 0 lessened by f g +
- *        p; then its bias is added (of several entries the last); a token that is
- *        not allowed gets -inf, whatever it was.  fp32 arithmetic, one rounding.
+ *        p; then its bias is added (of several entries the last), so that no penalty
+ *        scales it (one that is to be scaled is added in a launch before, with
+ *        penalties 1, 0, 0); a token that is not allowed gets -inf, whatever it
+ *        was.  fp32 arithmetic, one rounding.
  *        Tokens outside [0, columns) count for nothing (-1: a prompt's rows, whose
  *        tokens stand in the history).  Rows outside every sequence are left as
  *        they were.  The output is the input (with its stride), or its rows share

@@ -33,6 +33,31 @@ def test_logits_between_the_rows_of_their_input(ctx, kind, rows):
         b.free()
 
 
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_biases_before_penalties(ctx, kind):
+    """A launch with the biases alone, then one with the penalties alone, in place."""
+    dtype, columns = TYPES[kind], 5001
+    step = Step(np.random.default_rng(5), [3, 1, 6], columns, 200, 400, allowed=False)
+    x = (3 * np.random.default_rng(6).standard_normal((step.rows, columns))).astype(dtype)
+    penalties, logits = step.penalties, ctx.upload(x)
+    for penal in (False, True):
+        step.penalties = penalties if penal else np.tile(np.array([1, 0, 0], np.float32), (3, 1))
+        if penal:
+            step.bias_offsets = np.zeros(4, np.int32)
+            step.bias_tokens, step.bias_values = step.bias_tokens[:0], step.bias_values[:0]
+        bufs, scalars = step.upload(ctx)
+        assert (scalars[2] == 0) == penal
+        ctx.launch("ipu_stack_adjust_logits_" + kind, logits, [logits] + bufs,
+                   [3, step.rows, columns, columns, columns] + scalars)
+        got = logits.download(dtype).reshape(x.shape)
+        want, bound, inside = step.exact(x)
+        assert np.all(inside) and np.all(within(got, want, bound, dtype)) and np.any(got != x)
+        x = got  # what the next launch begins with
+        for b in bufs:
+            b.free()
+    logits.free()
+
+
 @pytest.mark.parametrize("trees", [False, True])
 def test_slots_of_a_step_that_is_cut_off(ctx, trees):
     """Fewer rows than the counts' sum: with lengths less the rows cut off, the rows that are
