@@ -142,7 +142,7 @@ __device__ __forceinline__ void clear_non_finite(uint8_t* tile, uint32_t thread,
 // Adds the products of a tile's non-finite values, in the layout of the kernels' MFMAs: o[dt][qt][c]
 // is column 16 dt + 4 (l / 16) + c of query 16 qt + l % 16, and p(kk, qt, e) the probability of
 // key 32 kk + 4 (l / 16) + e % 4 + 16 (e / 4).  chunk(row, column): where 4 columns lie in the tile;
-// this lane's query reads the keys below limit of which named(qt, row) says so by the tile's row.
+// this lane's query reads the keys below its limit that named(qt, row) names, by their row of the tile.
 struct AllNamed {
   __device__ __forceinline__ bool operator()(uint32_t, uint32_t) const { return true; }
 };

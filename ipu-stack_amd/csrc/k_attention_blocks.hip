@@ -15,8 +15,8 @@
 // (4 x 2048 rows against 8192 keys 1304 us against 955, 5 x 796 rows 39.9 against 31.6; trees, which
 // wait for HBM too, 8 to 25% more: 16 of 64 rows against 8192 keys 229 us against 186, 64 of 8 to 16
 // against 256 to 4096 121 against 106, 7 of 50 to 99 against up to 3001 (16 heads of 72 columns) 27.3
-// against 23.1).  Against float64 the results are off by 2.9e-4 at most so, where their own rounding
-// to fp16 is off by 2.1e-4.
+// against 23.1).  Against float64 trees' results are off by 2.6e-4 to 2.9e-4 of their size so (root
+// mean square), where their own rounding to fp16 alone makes 2.1e-4.
 //
 // A workgroup finds its block by a scan over the sequences; workgroups of one XCD
 // take a contiguous range of blocks, the query blocks of one (sequence, key head)
